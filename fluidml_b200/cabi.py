@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -17,9 +18,11 @@ _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib",
                          "libfluidml_b200_kernels.so")
 
 F32, I32, I64, BOOL = 1, 6, 7, 9
+F16, BF16 = 10, 16  # the operators of a decoder's serving step only
 _CODE = {np.dtype(np.float32): F32, np.dtype(np.int32): I32, np.dtype(np.int64): I64,
          np.dtype(np.bool_): BOOL}
 _NP = {F32: np.float32, I32: np.int32, I64: np.int64, BOOL: np.bool_}
+_SERVING_CODE = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16, "torch.int32": I32, "torch.int64": I64}
 
 # fml_ew_op
 ADD, MUL, DIV, SUB, POW, EQUAL = 0, 1, 2, 3, 4, 5
@@ -417,6 +420,105 @@ def device_count() -> int:
     n = ctypes.c_int()
     check(lib().fml_device_count(ctypes.byref(n)))
     return n.value
+
+
+# ------------------------------------------------------------------ a decoder's serving step
+ROTARY_HALVES, ROTARY_INTERLEAVED = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK, ROTARY_BANDS, ROTARY_RAMP = range(5)
+
+
+class RotarySpec(ctypes.Structure):
+    _fields_ = [("rot", ctypes.c_int32), ("scaling", ctypes.c_int32), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("trained_length", ctypes.c_double), ("turns_low", ctypes.c_double), ("turns_high", ctypes.c_double)]
+
+
+class ScoreRules(ctypes.Structure):
+    _fields_ = [("divisor", ctypes.c_float), ("cap", ctypes.c_float), ("causal", ctypes.c_int32)]
+
+
+_DTYPES: dict = {}  # dtype object of another library -> code
+_PACK = [struct.Struct(f"Qii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x").pack for r in range(MAX_RANK + 1)]
+
+
+def _arg(t):
+    """What the serving operators take: a DeviceTensor, a Tensor, None, or any object with data_ptr(), dtype, shape and stride()
+    (a torch tensor on the current device).  Returns a value ctypes passes as a pointer to the description, which the call reads
+    before it returns."""
+    if t is None:
+        return None
+    if hasattr(t, "data_ptr"):
+        code = _DTYPES.get(t.dtype)
+        if code is None:
+            code = _SERVING_CODE.get(str(t.dtype))
+            if code is None:
+                raise FmlError(2, f"no kernel takes {t.dtype}")
+            _DTYPES[t.dtype] = code
+        if t.device.type != "cuda":
+            raise FmlError(1, f"a tensor on {t.device} was given where device memory is needed")
+        shape = t.shape
+        if len(shape) > MAX_RANK:
+            raise FmlError(1, f"at most {MAX_RANK} dims")
+        return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape, *t.stride())
+    return ctypes.byref(t if isinstance(t, Tensor) else t.c())
+
+
+def _serving(name, *types):
+    """A function of the library with its argument types set (once)."""
+    f = getattr(lib(), name)
+    if f.argtypes is None:
+        f.argtypes = list(types)
+    return f
+
+
+_P, _F, _I = ctypes.c_void_p, ctypes.c_float, ctypes.c_int
+
+
+def rotary_positions(q, k, v, positions, slots, frequencies, q_out, k_out, v_out, magnitude=1.0, layout=ROTARY_HALVES, stream=None):
+    """Turns q and k by their positions; with slots, k and v go into a paged cache (fml_rotary_positions)."""
+    f = _serving("fml_rotary_positions", _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P, _P)
+    check(f(_arg(q), _arg(k), _arg(v), _arg(positions), _arg(slots), _arg(frequencies), magnitude, layout, _arg(q_out), _arg(k_out),
+            _arg(v_out), stream))
+
+
+def rotary_frequencies(rot, scaling=ROTARY_PLAIN, base=10000.0, factor=1.0, trained_length=0.0, turns_low=1.0, turns_high=4.0):
+    """(frequencies [rot / 2] as a numpy array, magnitude) of a scaling for long contexts (fml_rotary_frequencies)."""
+    out, magnitude = np.empty(max(rot // 2, 1), np.float32), ctypes.c_float()
+    spec = RotarySpec(rot, scaling, base, factor, trained_length, turns_low, turns_high)
+    check(lib().fml_rotary_frequencies(ctypes.byref(spec), out.ctypes.data_as(ctypes.c_void_p), ctypes.byref(magnitude)))
+    return out, magnitude.value
+
+
+def attention_rules(q, k, v, out, divisor, cap=0.0, causal=False, slopes=None, prefix=None, q_documents=None, k_documents=None, stream=None):
+    """Attention over a prompt with capped scores, a distance bias, documents and a prefix (fml_attention_rules)."""
+    f = _serving("fml_attention_rules", *[_P] * 10)
+    rules = ScoreRules(divisor, cap, 1 if causal else 0)
+    check(f(_arg(q), _arg(k), _arg(v), _arg(slopes), _arg(prefix), _arg(q_documents), _arg(k_documents), ctypes.byref(rules), _arg(out), stream))
+
+
+def attention_tree_workspace(requests, tokens, heads, kv_heads, head_size) -> int:
+    """Bytes that attention_tree needs as its workspace (fml_attention_tree_workspace); host only."""
+    f = _serving("fml_attention_tree_workspace", *[ctypes.c_int64] * 5)
+    f.restype = ctypes.c_size_t
+    return f(requests, tokens, heads, kv_heads, head_size)
+
+
+def attention_tree(q, k_cache, v_cache, block_table, context, query_start, tree, out, workspace, divisor, cap=0.0, slopes=None, stream=None):
+    """Attention of new tokens (a chain, or with `tree` a tree of drafts) over a paged cache (fml_attention_tree).
+    `workspace`: a DeviceBuffer, or any array of bytes on the device with data_ptr() and numel()."""
+    f = _serving("fml_attention_tree", *[_P] * 11, ctypes.c_size_t, _P)
+    rules = ScoreRules(divisor, cap, 1)
+    if isinstance(workspace, DeviceBuffer):
+        place, size = workspace.ptr, workspace.nbytes
+    else:
+        place, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    check(f(_arg(q), _arg(k_cache), _arg(v_cache), _arg(block_table), _arg(context), _arg(query_start), _arg(tree), _arg(slopes),
+            ctypes.byref(rules), _arg(out), place, size, stream))
+
+
+def sample(logits, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, probabilities=None, stream=None):
+    """One token per row of logits from given random numbers (fml_sample)."""
+    f = _serving("fml_sample", *[_P] * 9)
+    check(f(_arg(logits), _arg(uniform), _arg(temperature), _arg(top_k), _arg(top_p), _arg(min_p), _arg(tokens), _arg(probabilities), stream))
 
 
 # ------------------------------------------------------------------ resident stage program

@@ -1,0 +1,125 @@
+// Rules of fml_attention_rules that its two kernels share: which keys a query sees, which tiles of keys a tile of queries sees,
+// and the repair of rows that are not finite.
+#pragma once
+#include "flash_mma.cuh"
+
+namespace fml {
+
+struct RulesArgs {
+  const void *q, *k, *v;
+  void *out;
+  int64_t q_s[4], k_s[4], v_s[4], o_s[4];  // element strides
+  const float *slopes;
+  int64_t slopes_s;
+  IndexView prefix, q_documents, k_documents;  // documents: p of batch 0, stride along the length
+  int64_t q_documents_row, k_documents_row;    // element strides over the batch
+  int batch, heads, group, Sq, Sk, D, causal;
+  Cap cap;
+  int q_vec, k_vec, v_vec;  // rows take 16-byte accesses
+  int *status;
+};
+
+__device__ __forceinline__ int64_t document_at(const IndexView &v, int64_t row, int batch, int i) {
+  const int64_t e = batch * row + i * v.stride;
+  return v.wide ? static_cast<const int64_t *>(v.p)[e] : (int64_t)static_cast<const int32_t *>(v.p)[e];
+}
+
+// What a query goes by: its position, the last key + 1 that causal and prefix leave it, its document and slope (units of ln 2).
+struct RowRules {
+  int at, last;
+  int64_t document;
+  float slope;
+};
+__device__ __forceinline__ int last_key_of(const RulesArgs &a, int batch, int row) {
+  if (!a.causal) return a.Sk;
+  int64_t last = (int64_t)row + a.Sk - a.Sq + 1;
+  if (a.prefix.p) last = max(last, index_at(a.prefix, batch));
+  return (int)max((int64_t)0, min(last, (int64_t)a.Sk));
+}
+__device__ __forceinline__ RowRules row_rules(const RulesArgs &a, int batch, int head, int row) {
+  RowRules r;
+  r.at = row + a.Sk - a.Sq;
+  r.last = last_key_of(a, batch, row);
+  r.document = a.q_documents.p ? document_at(a.q_documents, a.q_documents_row, batch, row) : 0;
+  r.slope = a.slopes ? a.slopes[head * a.slopes_s] * kLog2e : 0.0f;
+  return r;
+}
+__device__ __forceinline__ bool key_seen(const RulesArgs &a, const RowRules &r, int key, int64_t document) {
+  return key < r.last && (!a.q_documents.p || document == r.document);
+}
+
+// What the queries [row0, row1) of a tile see of a tile of keys: none, all of them every key, or some.
+enum TileView { kTileNone = 0, kTileSome = 1, kTileAll = 2 };
+struct TileRange {
+  int first_key, last_key;  // every query sees the keys below first_key, none those from last_key on (documents apart)
+  int64_t low, high;        // the queries' smallest and largest document
+};
+__device__ __forceinline__ int64_t warp_min(int64_t v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = min(v, (int64_t)__shfl_xor_sync(0xffffffffu, (long long)v, o));
+  return v;
+}
+// By a whole warp.
+__device__ __forceinline__ TileRange tile_range(const RulesArgs &a, int batch, int row0, int row1) {
+  TileRange t;
+  t.first_key = last_key_of(a, batch, row0);  // (grows with the row)
+  t.last_key = last_key_of(a, batch, row1 - 1);
+  t.low = INT64_MAX;
+  t.high = INT64_MIN;
+  if (a.q_documents.p) {
+    for (int i = row0 + (int)(threadIdx.x & 31); i < row1; i += 32) {
+      const int64_t x = document_at(a.q_documents, a.q_documents_row, batch, i);
+      t.low = min(t.low, x);
+      t.high = max(t.high, x);
+    }
+    t.low = warp_min(t.low);
+    t.high = ~warp_min(~t.high);
+  }
+  return t;
+}
+__device__ __forceinline__ int tile_view(const RulesArgs &a, int batch, const TileRange &t, int key0, int keys) {
+  if (key0 >= t.last_key) return kTileNone;
+  bool all = key0 + keys <= t.first_key;
+  if (a.k_documents.p) {
+    int64_t low = INT64_MAX, high = INT64_MIN;
+    for (int i = key0 + (int)(threadIdx.x & 31); i < min(key0 + keys, t.last_key); i += 32) {
+      const int64_t x = document_at(a.k_documents, a.k_documents_row, batch, i);
+      low = min(low, x);
+      high = max(high, x);
+    }
+    low = warp_min(low);
+    high = ~warp_min(~high);
+    if (low > t.high || high < t.low) return kTileNone;
+    all = all && low == high && t.low == t.high;
+  }
+  return all ? kTileAll : kTileSome;
+}
+
+// A row whose context came out as not finite: keys that it does not see may hold infinities or NaN, which weights of zero do
+// not cancel.  Done again by a warp, key by key, over those it sees (one of them may be the cause: then it stays).
+template <typename T> __device__ __noinline__ void redo_rules_row(const RulesArgs &a, int batch, int head, int row) {
+  const int lane = threadIdx.x & 31, kv = head / a.group;
+  const RowRules r = row_rules(a, batch, head, row);
+  const T *q = static_cast<const T *>(a.q) + batch * a.q_s[0] + head * a.q_s[1] + (int64_t)row * a.q_s[2];
+  const T *k0 = static_cast<const T *>(a.k) + batch * a.k_s[0] + kv * a.k_s[1], *v0 = static_cast<const T *>(a.v) + batch * a.v_s[0] + kv * a.v_s[1];
+  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
+  for (int key = 0; key < r.last; ++key) {
+    if (a.k_documents.p && document_at(a.k_documents, a.k_documents_row, batch, key) != r.document) continue;
+    const T *k = k0 + (int64_t)key * a.k_s[2], *v = v0 + (int64_t)key * a.v_s[2];
+    float s = 0.0f;
+    for (int d = lane; d < a.D; d += 32) s = fmaf(to_f32(q[d * a.q_s[3]]), to_f32(k[d * a.k_s[3]]), s);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+    s *= a.cap.scale;
+    if (a.cap.cap > 0.0f) s = a.cap.cap * tanhf(s);
+    if (a.slopes) s -= r.slope * (float)abs(r.at - key);
+    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn, keep = ex2_approx(m - base), p = ex2_approx(s - base);
+    m = mn;
+    l = l * keep + p;
+    for (int i = 0, d = lane; d < a.D; ++i, d += 32) o[i] = o[i] * keep + p * to_f32(v[d * a.v_s[3]]);
+  }
+  T *dst = static_cast<T *>(a.out) + batch * a.o_s[0] + head * a.o_s[1] + (int64_t)row * a.o_s[2];
+  for (int i = 0, d = lane; d < a.D; ++i, d += 32) dst[d * a.o_s[3]] = from_f32<T>(l == 0.0f ? 0.0f : o[i] / l);
+}
+
+}  // namespace fml

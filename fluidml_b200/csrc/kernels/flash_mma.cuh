@@ -1,0 +1,236 @@
+// Attention on warp-wide matrix instructions, shared by attention_rules.cu and attention_tree.cu: a warp owns 16 rows, whose
+// queries, running maximum, sum and context stay in its registers, and takes keys and values from tiles in shared memory.
+//
+//   s = q k^T;  m' = max(m, s);  p = 2^(s - m');  l = l 2^(m - m') + sum p;  o = o 2^(m - m') + p v
+//
+// 16-bit types: m16n8k16 with fp32 sums; p is rounded to the type (half a step of a weight, as the values carry), its sum is
+// not.  fp32: every operand is split into two TF32 numbers, hi + lo to 2^-22, and three products of four are kept.
+#pragma once
+#include "serving_common.cuh"
+#include "tc_common.cuh"
+
+namespace fml {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {  // zeros when not valid
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t *r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t *r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T> __device__ __forceinline__ void mma16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16<__half>(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8_tf32(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  const float rest = x - __uint_as_float(hi);
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Tiles in shared memory and products with them.  DP: the head size the tiles are laid out for (features from the real one on
+// are zeros).  at(row, chunk): byte offset of 16 bytes of a row of a K (or Q) tile; at_v: of a V tile.
+template <typename T, int DP> struct Flash {
+  static constexpr int kChunk = 8, kChunks = DP / 8, kPitch = DP * 2, kPitchV = DP * 2;
+  struct Q { uint32_t r[DP / 16][4]; };
+  // the 16-byte chunks of a row are permuted by its index: a matrix load of 8 rows meets 8 different bank groups
+  __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((chunk ^ (row & 7)) << 4)); }
+  __device__ __forceinline__ static uint32_t at_v(int row, int chunk) { return at(row, chunk); }
+  __device__ __forceinline__ static void load_q(Q &q, uint32_t tile, int row0) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) ldmatrix4(tile + at(row0 + (lane & 15), 2 * k + (lane >> 4)), q.r[k]);
+  }
+  template <int NT> __device__ __forceinline__ static void scores(float (&s)[NT][4], const Q &q, uint32_t, int, uint32_t tile, int key0) {
+    static_assert(NT % 2 == 0, "two groups of eight keys per matrix load");
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t b[4];
+        ldmatrix4(tile + at(key0 + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
+        mma16<T>(s[n], q.r[k], b[0], b[1]);
+        mma16<T>(s[n + 1], q.r[k], b[2], b[3]);
+      }
+    }
+  }
+  template <int NT> __device__ __forceinline__ static void context(float (&o)[DP / 8][4], const float (&p)[NT][4], uint32_t tile, int key0) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < NT / 2; ++k) {
+      const uint32_t a[4] = {pack2<T>(p[2 * k][0], p[2 * k][1]), pack2<T>(p[2 * k][2], p[2 * k][3]), pack2<T>(p[2 * k + 1][0], p[2 * k + 1][1]),
+                             pack2<T>(p[2 * k + 1][2], p[2 * k + 1][3])};
+#pragma unroll
+      for (int n = 0; n < DP / 8; n += 2) {
+        uint32_t b[4];
+        ldmatrix4_trans(tile + at(key0 + k * 16 + (lane & 15), n + (lane >> 4)), b);
+        mma16<T>(o[n], a, b[0], b[1]);
+        mma16<T>(o[n + 1], a, b[2], b[3]);
+      }
+    }
+  }
+};
+
+template <int DP> struct Flash<float, DP> {
+  // rows are padded so that the loads below meet every bank once: K by pairs of features, V by single ones
+  static constexpr int kChunk = 4, kChunks = DP / 4, kPitch = (DP + 8) * 4, kPitchV = (DP + 4) * 4;
+  struct Q {};  // (hi and lo of 16 x DP queries would fill the registers: read again for every tile)
+  __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + (chunk << 4)); }
+  __device__ __forceinline__ static uint32_t at_v(int row, int chunk) { return (uint32_t)(row * kPitchV + (chunk << 4)); }
+  __device__ __forceinline__ static void load_q(Q &, uint32_t, int) {}
+  __device__ __forceinline__ static float2 pair(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+  }
+  __device__ __forceinline__ static float one(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+  }
+  // k index t of an instruction is feature 2 t of its eight, t + 4 is 2 t + 1 (the order of a sum is free)
+  template <int NT>
+  __device__ __forceinline__ static void scores(float (&s)[NT][4], const Q &, uint32_t q_tile, int row0, uint32_t tile, int key0) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+    const uint32_t qa = q_tile + (uint32_t)((row0 + g) * kPitch + t * 8), ka = tile + (uint32_t)((key0 + g) * kPitch + t * 8);
+#pragma unroll 4
+    for (int k = 0; k < DP / 8; ++k) {
+      const float2 q0 = pair(qa + k * 32), q1 = pair(qa + k * 32 + 8 * kPitch);
+      uint32_t hi[4], lo[4];
+      split_tf32(q0.x, hi[0], lo[0]);
+      split_tf32(q1.x, hi[1], lo[1]);
+      split_tf32(q0.y, hi[2], lo[2]);
+      split_tf32(q1.y, hi[3], lo[3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float2 b = pair(ka + n * 8 * kPitch + k * 32);
+        uint32_t bh[2], bl[2];
+        split_tf32(b.x, bh[0], bl[0]);
+        split_tf32(b.y, bh[1], bl[1]);
+        mma8_tf32(s[n], lo, bh[0], bh[1]);
+        mma8_tf32(s[n], hi, bl[0], bl[1]);
+        mma8_tf32(s[n], hi, bh[0], bh[1]);
+      }
+    }
+  }
+  template <int NT> __device__ __forceinline__ static void context(float (&o)[DP / 8][4], const float (&p)[NT][4], uint32_t tile, int key0) {
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    const uint32_t va = tile + (uint32_t)((key0 + 2 * t) * kPitchV + g * 4);
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      uint32_t hi[4], lo[4];
+      split_tf32(p[k][0], hi[0], lo[0]);
+      split_tf32(p[k][2], hi[1], lo[1]);
+      split_tf32(p[k][1], hi[2], lo[2]);
+      split_tf32(p[k][3], hi[3], lo[3]);
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) {
+        uint32_t bh[2], bl[2];
+        split_tf32(one(va + k * 8 * kPitchV + n * 32), bh[0], bl[0]);
+        split_tf32(one(va + k * 8 * kPitchV + n * 32 + kPitchV), bh[1], bl[1]);
+        mma8_tf32(o[n], lo, bh[0], bh[1]);
+        mma8_tf32(o[n], hi, bl[0], bl[1]);
+        mma8_tf32(o[n], hi, bh[0], bh[1]);
+      }
+    }
+  }
+};
+
+// The two rows of a thread: lane / 4 and lane / 4 + 8 of the warp's 16.
+template <int DP> struct Running {
+  float o[DP / 8][4], m[2], l[2];  // m, and the scores, in units of ln 2; m is -infinity before the first visible key
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.0f;
+  }
+};
+
+// One tile's keys key0 .. key0 + 8 NT - 1.  shape(s): scores in units of ln 2 in place of q . k, -infinity for keys not seen.
+template <typename F, int DP, int NT, typename S>
+__device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &q, uint32_t q_tile, int row0, uint32_t k_tile, uint32_t v_tile,
+                                           int key0, S shape) {
+  float s[NT][4];
+  F::template scores<NT>(s, q, q_tile, row0, k_tile, key0);
+  shape(s);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float m = r.m[h];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const float base = m == -INFINITY ? 0.0f : m;  // (no key so far: every p below is 2^-infinity)
+    const float keep = ex2_approx(r.m[h] - base);
+    r.m[h] = m;
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      s[n][2 * h] = ex2_approx(s[n][2 * h] - base);
+      s[n][2 * h + 1] = ex2_approx(s[n][2 * h + 1] - base);
+      sum += s[n][2 * h] + s[n][2 * h + 1];
+    }
+    r.l[h] = r.l[h] * keep + sum;  // (this thread's keys: the four lanes of a row are added up at the end)
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) { r.o[n][2 * h] *= keep; r.o[n][2 * h + 1] *= keep; }
+  }
+  F::template context<NT>(r.o, s, v_tile, key0);
+}
+
+// cap * tanh(s / cap) in units of ln 2, s = x * inv_divisor.
+struct Cap {
+  float scale, cap, inv;  // without a cap scale = log2(e) / divisor; with one scale = 1 / (divisor cap), cap in units of ln 2
+  __host__ static Cap make(float divisor, float cap) {
+    Cap c;
+    c.cap = cap > 0.0f ? cap * kLog2e : 0.0f;
+    c.scale = cap > 0.0f ? 1.0f / (divisor * cap) : kLog2e / divisor;
+    c.inv = 0.0f;
+    return c;
+  }
+};
+template <bool EXACT> __device__ __forceinline__ float tanh_of(float x) {
+  if (EXACT) return tanhf(x);
+  // 1 - 2 / (e^2x + 1): 1e-7 of the whole, where 16-bit weights carry 2^-9 and more
+  return 1.0f - __fdividef(2.0f, ex2_approx(x * (2.0f * kLog2e)) + 1.0f);
+}
+
+}  // namespace fml

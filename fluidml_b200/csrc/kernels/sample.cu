@@ -1,0 +1,548 @@
+// One token per row of logits from given random numbers (fml_sample): temperature, top-k, top-p, min-p.
+//
+// A cluster of CTAs holds a row in shared memory, read once from HBM.  No sort: a cut through the order (logit, then index) is
+// a logit and an index, found by histograms that narrow a range of logits, 1024 bins at a time.
+//
+//   1  largest logit
+//   2  counts in bins linear in (largest - logit) / temperature: the logits of a vocabulary spread over all of them, where the
+//      leading bits of their encoding would put most into a dozen and serialise the atomics
+//   3  top-k: the bin that holds the k-th token, as a range of keys (integers in the order of the logits), is binned by key
+//      until a bin is one key; of equal logits the lowest indexes are kept
+//   4  top-p: the counts bound every bin's weight, which leaves a few bins for the cut; one pass sums the weights of all
+//      tokens and of those above these bins exactly and bins the rest by key, as in 3, with weights in place of counts
+//   5  the draw: sums of the kept weights per warp, in the vocabulary's order, then the warp that holds the token walks its part
+//
+// Weights are integers, 2^44 for the largest: their sums are exact in any order, so neither the atomics nor the split over warps
+// and CTAs changes a result, and a cumulative sum lies within 2^-27 of the largest weight of the real one however many tokens
+// there are (a rounded half unit each, 2^18 tokens).  The exponential is evaluated in 64 bits: its fp32 error, 2^-23 of a
+// weight, is as wide as the steps of the random numbers, and would move one token in some thousand draws.
+#include "serving_common.cuh"
+#include <algorithm>
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
+
+namespace fml {
+namespace {
+
+using u64 = unsigned long long;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kMaxCluster = 8;
+constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest logit
+constexpr float kSpan = 32.0f;             // the bins reach e^-32, below which every weight is a unit
+
+struct SampleArgs {
+  const void *logits;
+  int64_t row_stride, col_stride, rows;
+  const float *uniform, *temperature, *top_p, *min_p;
+  int64_t uniform_s, temperature_s, top_p_s, min_p_s;
+  IndexView top_k;
+  void *tokens;
+  float *probabilities;
+  int64_t tokens_s, probabilities_s;
+  int vocab, slice, tokens_wide, vec;  // slice: tokens per CTA; vec: rows take 16-byte accesses
+};
+
+struct Shared {
+  u64 hist[kBins], merged[kBins];
+  uint32_t counts[kBins];
+  u64 part[kWarps];
+  u64 exchange[2][kMaxCluster];
+  u64 found[4];
+  double top;
+};
+
+// Integers in the order of the logits; both zeros are one.
+__device__ __forceinline__ uint32_t key_of(float z) {
+  const uint32_t u = __float_as_uint(z + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+constexpr uint32_t kNone = 0x007fffffu;  // key of -infinity: nothing to draw
+
+// 2^x for -1100 < x <= 0: the fraction's Taylor series (terms ln(2)^n / n!) to the 11th power, 6e-15 on half a unit.
+__device__ __forceinline__ double exp2_64(double x) {
+  const double n = rint(x), f = (x - n) * 0.6931471805599453;
+  double p = 1.0 / 39916800.0;
+  p = fma(p, f, 1.0 / 3628800.0);
+  p = fma(p, f, 1.0 / 362880.0);
+  p = fma(p, f, 1.0 / 40320.0);
+  p = fma(p, f, 1.0 / 5040.0);
+  p = fma(p, f, 1.0 / 720.0);
+  p = fma(p, f, 1.0 / 120.0);
+  p = fma(p, f, 1.0 / 24.0);
+  p = fma(p, f, 1.0 / 6.0);
+  p = fma(p, f, 0.5);
+  p = fma(p, f, 1.0);
+  p = fma(p, f, 1.0);
+  return ldexp(p, (int)n);
+}
+
+struct Row {
+  double top, rate;  // weight = 2^((z - top) * rate)
+  float topf, scale;  // bins: (topf - z) / 2 * scale
+  double least;       // log2 of min-p, -infinity when off
+  uint32_t cut_key;   // kept: a key above cut_key, or equal and an index up to cut_index
+  int cut_index;
+};
+
+__device__ __forceinline__ double exponent_of(const Row &r, float z) { return z == r.topf ? 0.0 : ((double)z - r.top) * r.rate; }
+__device__ __forceinline__ u64 weight_of(const Row &r, float z) {
+  const double t = exponent_of(r, z);
+  if (t < -45.0) return t > -1075.0 ? 1ull : 0ull;  // (a weight that 64 bits hold; NaN, of an infinite rate: none)
+  if (!(t >= -45.0)) return 0ull;
+  const u64 w = (u64)__double2ull_rn(exp2_64(t) * kOne);
+  return w ? w : 1ull;
+}
+__device__ __forceinline__ int bin_of(const Row &r, float z) {
+  // (halves: the difference of two finite logits may not be finite; NaN goes last)
+  return z >= r.topf ? 0 : (int)fminf((0.5f * r.topf - 0.5f * z) * r.scale, (float)(kBins - 1));
+}
+__device__ __forceinline__ bool kept_by_cut(const Row &r, uint32_t key, int index) {
+  return key > r.cut_key || (key == r.cut_key && index <= r.cut_index);
+}
+
+template <typename T> struct Sampler {
+  static constexpr int V = 16 / sizeof(T);  // logits per access
+  const T *data;
+  Shared *sh;
+  cg::cluster_group cluster;
+  int rank, ranks, base, seg, warp, lane, phase;
+
+  // f(logit, index in the vocabulary) over the warp's part, in order by lane; the part is whole accesses
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    for (int i = warp * seg + lane * V; i < (warp + 1) * seg; i += 32 * V) {
+      const uint4 raw = *reinterpret_cast<const uint4 *>(data + i);
+      const T *x = reinterpret_cast<const T *>(&raw);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f(to_f32(x[j]), base + i + j);
+    }
+  }
+  __device__ __forceinline__ u64 warp_sum(u64 v) const {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+  // Every CTA's `mine` (of its first thread) to all CTAs: exchange[phase][rank]; ends with a cluster barrier.
+  __device__ __forceinline__ const u64 *to_all(u64 mine) {
+    phase ^= 1;
+    if (threadIdx.x < ranks) *cluster.map_shared_rank(&sh->exchange[phase][rank], threadIdx.x) = mine;
+    cluster.sync();
+    return sh->exchange[phase];
+  }
+  // Sum over the cluster of the threads' values (MAX: the largest).
+  template <bool MAX> __device__ u64 reduce(u64 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
+      v = MAX ? max(v, w) : v + w;
+    }
+    __syncthreads();
+    if (lane == 0) sh->part[warp] = v;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all = MAX ? max(all, sh->part[w]) : all + sh->part[w];
+    const u64 *x = to_all(all);
+    all = 0;
+    for (int i = 0; i < ranks; ++i) all = MAX ? max(all, x[i]) : all + x[i];
+    return all;
+  }
+  __device__ void clear() {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh->hist[i] = 0;
+    __syncthreads();
+  }
+  // hist of all CTAs, added up, into every CTA's merged.
+  __device__ void merge() {
+    cluster.sync();
+    const int share = kBins / ranks;
+    for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += kThreads) {
+      u64 sum = 0;
+      for (int c = 0; c < ranks; ++c) sum += *cluster.map_shared_rank(&sh->hist[i], c);
+      for (int c = 0; c < ranks; ++c) *cluster.map_shared_rank(&sh->merged[i], c) = sum;
+    }
+    cluster.sync();
+  }
+  // The first bin b of values(b) whose running sum, from `above` on, has reached(sum): found[0] = b, found[1] = the sum before it,
+  // the last bin if none has.  Two neighbouring bins per thread.
+  template <typename U, typename G, typename R> __device__ void first_bin(U above, G values, R reached, int *bin, U *before) {
+    const U a = values(2 * threadIdx.x), b = values(2 * threadIdx.x + 1);
+    U run = a + b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const U up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    U *part = reinterpret_cast<U *>(sh->part);
+    U *found = reinterpret_cast<U *>(sh->found);
+    __syncthreads();
+    if (lane == 31) part[warp] = run;
+    if (threadIdx.x == 0) *reinterpret_cast<volatile int *>(sh->found + 2) = kBins;
+    __syncthreads();
+    U start = above;
+    for (int w = 0; w < warp; ++w) start += part[w];
+    start += run - a - b;
+    // (sums of non-negative numbers: once reached, always; only the first says so and its predecessor does not)
+    int *at = reinterpret_cast<int *>(sh->found + 2);
+    const bool r0 = reached(start + a), r1 = reached(start + a + b);
+    if (r0) atomicMin(at, 2 * (int)threadIdx.x);
+    else if (r1) atomicMin(at, 2 * (int)threadIdx.x + 1);
+    __syncthreads();
+    const int got = min(*at, kBins - 1);
+    if (got == 2 * (int)threadIdx.x) found[0] = start;
+    if (got == 2 * (int)threadIdx.x + 1) found[0] = start + a;
+    __syncthreads();
+    *bin = got;
+    *before = found[0];
+    __syncthreads();
+  }
+  // The keys of bins [b1, b2]: bin_of is monotone, so they are an interval, whose ends two searches find.
+  __device__ __forceinline__ void keys_of(const Row &r, int b1, int b2, uint32_t *lo, uint32_t *hi) const {
+    uint32_t l = kNone + 1, h = key_of(r.topf);  // smallest key of a bin up to b2
+    while (l < h) {
+      const uint32_t m = l + (h - l) / 2;
+      if (bin_of(r, value_of(m)) <= b2) h = m; else l = m + 1;
+    }
+    *lo = l;
+    l = *lo; h = key_of(r.topf);  // largest key of a bin from b1 on
+    while (l < h) {
+      const uint32_t m = l + (h - l + 1) / 2;
+      if (bin_of(r, value_of(m)) >= b1) l = m; else h = m - 1;
+    }
+    *hi = l;
+  }
+  // Narrows the range of keys [lo, hi], above which lies `above` of the measure, to the one key at which the running sum has
+  // reached(sum).  first: the histogram of the range is merged already (by (hi - key) >> shift_of).
+  template <typename M, typename R>
+  __device__ void narrow(uint32_t lo, uint32_t hi, u64 above, bool first, M measure, R reached, uint32_t *key, u64 *before, u64 *ties) {
+    for (;;) {
+      const int shift = shift_of(lo, hi);
+      if (!first) {
+        clear();
+        each([&](float z, int i) {
+          const uint32_t k = key_of(z);
+          if (k >= lo && k <= hi) {
+            const u64 m = measure(z, k, i);
+            if (m) atomicAdd(&sh->hist[(hi - k) >> shift], m);
+          }
+        });
+        merge();
+      }
+      first = false;
+      int b;
+      first_bin<u64>(above, [&](int i) { return sh->merged[i]; }, reached, &b, &above);
+      const u64 inside = sh->merged[b];
+      hi = hi - min((uint32_t)b << shift, hi - lo);
+      if (shift == 0) {
+        *key = hi; *before = above; *ties = inside;
+        return;
+      }
+      lo = max(lo, hi - min(hi, (1u << shift) - 1u));
+    }
+  }
+  __device__ __forceinline__ static int shift_of(uint32_t lo, uint32_t hi) { return max(0, 22 - __clz((int)((hi - lo) | 1u))); }
+
+  // The first index, in the vocabulary's order, at which the running sum of measure(z, key, index) has reached(sum); -1: none.
+  template <typename M, typename R> __device__ int locate(M measure, R reached, u64 *total) {
+    u64 mine = 0;
+    each([&](float z, int i) { mine += measure(z, key_of(z), i); });
+    mine = warp_sum(mine);
+    __syncthreads();
+    if (lane == 0) sh->part[warp] = mine;
+    __syncthreads();
+    u64 start = 0, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp) start = all;
+      all += sh->part[w];
+    }
+    const u64 *x = to_all(all);
+    u64 sum = 0;
+    for (int c = 0; c < ranks; ++c) {
+      if (c == rank) start += sum;
+      sum += x[c];
+    }
+    *total = sum;
+    if (threadIdx.x == 0) sh->found[3] = ~0ull;
+    cluster.sync();
+    if (!reached(start, sum) && reached(start + mine, sum)) {  // (one warp of the cluster)
+      bool done = false;
+      for (int i = warp * seg + lane * V; i < (warp + 1) * seg && !done; i += 32 * V) {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(data + i);
+        const T *v = reinterpret_cast<const T *>(&raw);
+        u64 m[V], own = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float z = to_f32(v[j]);
+          m[j] = measure(z, key_of(z), base + i + j);
+          own += m[j];
+        }
+        u64 run = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 up = __shfl_up_sync(0xffffffffu, run, o);
+          if (lane >= o) run += up;
+        }
+        u64 at = start + run - own;
+        if (!reached(at, sum) && reached(at + own, sum)) {
+          int j = 0;
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            at += m[k];
+            if (!reached(at, sum)) j = k + 1;
+          }
+          for (int c = 0; c < ranks; ++c) *cluster.map_shared_rank(&sh->found[3], c) = (u64)(base + i + j);
+        }
+        start = __shfl_sync(0xffffffffu, start + run, 31);
+        done = reached(start, sum);
+      }
+    }
+    cluster.sync();
+    const u64 got = sh->found[3];
+    return got == ~0ull ? -1 : (int)got;
+  }
+};
+
+template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+  extern __shared__ __align__(16) uint8_t raw[];
+  __shared__ Shared shared;
+  Sampler<T> s{reinterpret_cast<const T *>(raw), &shared, cg::this_cluster()};
+  s.rank = (int)s.cluster.block_rank();
+  s.ranks = (int)s.cluster.num_blocks();
+  s.warp = threadIdx.x >> 5; s.lane = threadIdx.x & 31;
+  s.base = s.rank * a.slice; s.seg = a.slice / kWarps; s.phase = 0;
+  const int64_t row = blockIdx.x / s.ranks;
+  pdl_prologue();
+  // ---- 1: the slice into shared memory, -infinity behind its end and for NaN
+  constexpr int V = Sampler<T>::V;
+  T *const data = reinterpret_cast<T *>(raw);
+  const T *const src = static_cast<const T *>(a.logits) + row * a.row_stride;
+  const T lowest = from_f32<T>(-INFINITY);
+  float top = -INFINITY;
+  for (int i = threadIdx.x * V; i < a.slice; i += kThreads * V) {
+    alignas(16) T x[V];
+    if (a.vec && s.base + i + V <= a.vocab) {
+      *reinterpret_cast<uint4 *>(x) = __ldg(reinterpret_cast<const uint4 *>(src + s.base + i));
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] = s.base + i + j < a.vocab ? src[(int64_t)(s.base + i + j) * a.col_stride] : lowest;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float z = to_f32(x[j]);
+      if (z != z) x[j] = lowest;
+      top = fmaxf(top, z);  // (leaves NaN out)
+    }
+    *reinterpret_cast<uint4 *>(data + i) = *reinterpret_cast<const uint4 *>(x);
+  }
+  const uint32_t top_key = (uint32_t)s.template reduce<true>(key_of(top));  // (its barriers publish the slice too)
+  float temperature = a.temperature ? a.temperature[row * a.temperature_s] : 1.0f;
+  if (temperature > 0.0f) temperature = fmaxf(temperature, 1e-30f);  // (the bins' scale stays finite)
+  int token = -1;
+  double probability = 0.0;
+  if (top_key > kNone) {
+    Row r;
+    r.topf = value_of(top_key);
+    r.top = (double)r.topf;
+    r.rate = 1.4426950408889634 / (double)temperature;
+    r.scale = 2.0f * (float)kBins / kSpan / temperature;
+    r.cut_key = kNone + 1; r.cut_index = a.vocab;
+    float p = a.top_p ? a.top_p[row * a.top_p_s] : 1.0f;
+    const float m = a.min_p ? a.min_p[row * a.min_p_s] : 0.0f;
+    r.least = m > 0.0f ? log2((double)fminf(m, 1.0f)) : -INFINITY;
+    int64_t k = a.top_k.p ? index_at(a.top_k, row) : 0;
+    if (!(temperature > 0.0f)) {
+      // the largest logit, lowest index
+      u64 total;
+      token = s.locate([&](float, uint32_t key, int) { return (u64)(key == top_key); }, [](u64 c, u64) { return c >= 1; }, &total);
+      probability = 1.0;
+    } else {
+      const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.0f;
+      // ---- 2: counts by distance from the largest
+      if (by_k || by_p) {
+        uint32_t *h = reinterpret_cast<uint32_t *>(shared.hist);
+        s.clear();
+        s.each([&](float z, int) {
+          if (z > -INFINITY) atomicAdd(&h[2 * bin_of(r, z)], 1u);
+        });
+        s.merge();  // (64-bit words whose upper halves are zero)
+        for (int i = threadIdx.x; i < kBins; i += kThreads) shared.counts[i] = (uint32_t)shared.merged[i];
+        __syncthreads();
+      }
+      // ---- 3: top-k
+      if (by_k) {
+        const u64 want = (u64)k;
+        int b;
+        u64 above;
+        s.template first_bin<u64>(0ull, [&](int i) { return (u64)shared.counts[i]; }, [&](u64 c) { return c >= want; }, &b, &above);
+        if (above + shared.counts[b] > want) {  // the cut is inside the bin
+          uint32_t lo, hi, key;
+          u64 before, ties;
+          s.keys_of(r, b, b, &lo, &hi);
+          s.narrow(lo, hi, above, false, [](float, uint32_t, int) { return 1ull; }, [&](u64 c) { return c >= want; }, &key, &before, &ties);
+          r.cut_key = key;
+          if (before + ties > want) {
+            u64 total;
+            r.cut_index = s.locate([&](float, uint32_t x, int) { return (u64)(x == key); }, [&](u64 c, u64) { return c >= want - before; }, &total);
+          }
+        } else if (above + shared.counts[b] == want) {  // behind it
+          uint32_t lo, hi;
+          s.keys_of(r, b, b, &lo, &hi);
+          r.cut_key = lo;
+        }  // (fewer tokens than k: all)
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kThreads)
+          if (i > b) shared.counts[i] = 0;
+          else if (i == b) shared.counts[i] = (uint32_t)min((u64)shared.counts[i], want - above);
+        __syncthreads();
+      }
+      // ---- 4: top-p
+      if (by_p) {
+        const double share = p > 0.0f ? (double)p : 0.0;  // (0: the first token alone)
+        // a bin's weights, in units of the largest: exp(-x) for x between its ends, with more than fp32's errors to spare
+        const double width = (double)kSpan / kBins;
+        auto most = [&](int i) { return (double)shared.counts[i] * (exp2_64(-i * width * 1.4426950408889634 * (1 - 1e-5)) * 1.0001 + 1e-13); };
+        auto least = [&](int i) {
+          return i == kBins - 1 ? 0.0 : (double)shared.counts[i] * fmax(0.0, exp2_64(-(i + 1) * width * 1.4426950408889634 * (1 + 1e-5)) * 0.9999 - 1e-13);
+        };
+        int b1, b2, last;
+        double x, most_all, least_all;
+        s.template first_bin<double>(0.0, most, [](double) { return false; }, &last, &x);
+        most_all = x + most(last);
+        s.template first_bin<double>(0.0, least, [](double) { return false; }, &last, &x);
+        least_all = x + least(last);
+        s.template first_bin<double>(0.0, most, [&](double c) { return c >= share * least_all * (1 - 1e-9); }, &b1, &x);
+        s.template first_bin<double>(0.0, least, [&](double c) { return c >= share * most_all * (1 + 1e-9); }, &b2, &x);
+        b2 = max(b1, b2);
+        uint32_t lo, hi;
+        s.keys_of(r, b1, b2, &lo, &hi);
+        const int shift = Sampler<T>::shift_of(lo, hi);
+        u64 all = 0, over = 0;
+        s.clear();
+        s.each([&](float z, int i) {
+          const uint32_t key = key_of(z);
+          if (key > kNone && kept_by_cut(r, key, i)) {
+            const u64 w = weight_of(r, z);
+            all += w;
+            if (key > hi) over += w;
+            else if (key >= lo && w) atomicAdd(&shared.hist[(hi - key) >> shift], w);
+          }
+        });
+        s.merge();
+        all = s.template reduce<false>(all);
+        over = s.template reduce<false>(over);
+        const double want = share * (double)all;
+        uint32_t key;
+        u64 before, ties;
+        s.narrow(lo, hi, over, true, [&](float z, uint32_t x, int i) { return kept_by_cut(r, x, i) ? weight_of(r, z) : 0ull; },
+                 [&](u64 c) { return (double)c >= want && c > 0; }, &key, &before, &ties);
+        const u64 w = weight_of(r, value_of(key));
+        // of the tied tokens the first n: those before which less than `want` lies
+        u64 n = w ? (u64)fmax(ceil((want - (double)before) / (double)w), 1.0) : 1;
+        while (n > 1 && !((double)(before + (n - 1) * w) < want)) --n;
+        while (w && (double)(before + n * w) < want && n * w < ties) ++n;
+        int index = r.cut_index;
+        if (w && n * w < ties) {
+          u64 total;
+          index = s.locate([&](float, uint32_t x, int i) { return (u64)(x == key && kept_by_cut(r, x, i)); }, [&](u64 c, u64) { return c >= n; }, &total);
+        } else if (key != r.cut_key) {
+          index = a.vocab;
+        }
+        r.cut_key = key;
+        r.cut_index = index;
+      }
+      // ---- 5: the draw
+      float u = a.uniform[row * a.uniform_s];
+      u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
+      u64 total;
+      token = s.locate(
+          [&](float z, uint32_t key, int i) {
+            return key > kNone && kept_by_cut(r, key, i) && exponent_of(r, z) >= r.least ? weight_of(r, z) : 0ull;
+          },
+          [&](u64 c, u64 sum) { return (double)c > (double)u * (double)sum; }, &total);
+      if (token >= s.base && token < s.base + a.slice) {
+        const float z = to_f32(data[token - s.base]);
+        probability = exp2_64(fmax(exponent_of(r, z), -1074.0)) * kOne / (double)total;
+      }
+    }
+  }
+  if (threadIdx.x == 0 && (token < 0 ? s.rank == 0 : token >= s.base && token < s.base + a.slice)) {
+    if (a.tokens_wide) static_cast<int64_t *>(a.tokens)[row * a.tokens_s] = token;
+    else static_cast<int32_t *>(a.tokens)[row * a.tokens_s] = token;
+    if (a.probabilities) a.probabilities[row * a.probabilities_s] = (float)probability;
+  }
+}
+
+template <typename T> int launch(SampleArgs &a, cudaStream_t s) {
+  // Eight CTAs per row while that does not fill the device twice over, fewer when there are rows enough
+  constexpr int kGrain = kWarps * 32 * Sampler<T>::V;  // whole accesses for every lane
+  int ranks = kMaxCluster;
+  while (ranks > 1 && a.vocab <= kGrain * (ranks / 2)) ranks >>= 1;
+  a.slice = ((a.vocab + ranks - 1) / ranks + kGrain - 1) / kGrain * kGrain;
+  const size_t smem = (size_t)a.slice * sizeof(T);
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  FML_CUDA(cudaGetDevice(&dev));
+  if (!attr_set[dev & 63]) {
+    FML_CUDA(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+    attr_set[dev & 63] = true;
+  }
+  FML_REQUIRE(a.rows * ranks < (1ll << 31), FML_UNSUPPORTED, "fml_sample: too many rows");
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)(a.rows * ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  FML_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+  return FML_OK;
+}
+
+}  // namespace
+}  // namespace fml
+
+using namespace fml;
+
+extern "C" int fml_sample(const fml_tensor *logits, const fml_tensor *uniform, const fml_tensor *temperature, const fml_tensor *top_k,
+                          const fml_tensor *top_p, const fml_tensor *min_p, const fml_tensor *tokens, const fml_tensor *probabilities,
+                          void *stream) {
+  FML_REQUIRE(data_tensor(logits, 2), FML_BAD_ARG, "fml_sample: logits must be [rows, vocabulary] of fp32, fp16 or bf16");
+  const int64_t rows = logits->shape[0], vocab = logits->shape[1];
+  auto per_row = [&](const fml_tensor *t) { return t->shape[0] == rows; };
+  FML_REQUIRE(float_tensor(uniform, 1) && per_row(uniform), FML_BAD_ARG, "fml_sample: uniform must be [rows] of fp32");
+  FML_REQUIRE(!temperature || (float_tensor(temperature, 1) && per_row(temperature)), FML_BAD_ARG, "fml_sample: temperature must be [rows] of fp32");
+  FML_REQUIRE(!top_k || (index_tensor(top_k, 1) && per_row(top_k)), FML_BAD_ARG, "fml_sample: top_k must be [rows] of int32 or int64");
+  FML_REQUIRE(!top_p || (float_tensor(top_p, 1) && per_row(top_p)), FML_BAD_ARG, "fml_sample: top_p must be [rows] of fp32");
+  FML_REQUIRE(!min_p || (float_tensor(min_p, 1) && per_row(min_p)), FML_BAD_ARG, "fml_sample: min_p must be [rows] of fp32");
+  FML_REQUIRE(index_tensor(tokens, 1) && per_row(tokens), FML_BAD_ARG, "fml_sample: tokens must be [rows] of int32 or int64");
+  FML_REQUIRE(!probabilities || (float_tensor(probabilities, 1) && per_row(probabilities)), FML_BAD_ARG,
+              "fml_sample: probabilities must be [rows] of fp32");
+  FML_REQUIRE(vocab >= 1 && vocab <= (1 << 18), FML_UNSUPPORTED, "fml_sample: 1 to %d tokens", 1 << 18);
+  if (rows == 0) return FML_OK;
+  FML_REQUIRE(on_current_device(tokens->data) && (!probabilities || on_current_device(probabilities->data)), FML_BAD_ARG,
+              "fml_sample: an output is not memory of the current device");
+  SampleArgs a;
+  memset(&a, 0, sizeof(a));
+  auto floats = [](const fml_tensor *t, const float **p, int64_t *s) { if (t) { *p = static_cast<const float *>(t->data); *s = t->stride[0]; } };
+  floats(uniform, &a.uniform, &a.uniform_s);
+  floats(temperature, &a.temperature, &a.temperature_s);
+  floats(top_p, &a.top_p, &a.top_p_s);
+  floats(min_p, &a.min_p, &a.min_p_s);
+  a.top_k = index_view(top_k);
+  a.logits = logits->data;
+  a.rows = rows; a.row_stride = logits->stride[0]; a.col_stride = logits->stride[1];
+  a.vocab = (int)vocab;
+  a.tokens = tokens->data; a.tokens_s = tokens->stride[0]; a.tokens_wide = tokens->dtype == FML_I64;
+  if (probabilities) { a.probabilities = static_cast<float *>(probabilities->data); a.probabilities_s = probabilities->stride[0]; }
+  const int64_t v = 16 / (int64_t)data_size(logits->dtype);
+  a.vec = a.col_stride == 1 && (rows == 1 || a.row_stride % v == 0) && aligned16(a.logits);
+  if (logits->dtype == FML_F32) return launch<float>(a, as_stream(stream));
+  if (logits->dtype == FML_F16) return launch<__half>(a, as_stream(stream));
+  return launch<__nv_bfloat16>(a, as_stream(stream));
+}

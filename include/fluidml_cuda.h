@@ -50,7 +50,8 @@ typedef enum fml_status {
 } fml_status;
 
 typedef enum fml_dtype {
-  FML_F32 = 1, FML_I32 = 6, FML_I64 = 7, FML_BOOL = 9
+  FML_F32 = 1, FML_I32 = 6, FML_I64 = 7, FML_BOOL = 9,
+  FML_F16 = 10, FML_BF16 = 16 /* operators of a decoder's serving step only (below) */
 } fml_dtype;
 
 typedef struct fml_tensor {
@@ -511,6 +512,93 @@ int fml_conv_uses_tensor_cores(const fml_tensor *x, const fml_tensor *w, const f
  * averagepool.cpp:19-87): 2-D windows, no padding.  mode 0 = max, 1 = average. */
 int fml_pool2d(const fml_tensor *x, const fml_tensor *y, int mode, const int64_t *kernel,
                const int64_t *strides, void *stream);
+
+/* ---------------------------------------------------------------- a decoder's serving step
+ * What a program that answers with a decoder runs besides the products: positions onto queries and keys and the append to
+ * a paged cache, attention over a prompt, attention of new tokens over the cache, the choice of a token.  None has a
+ * counterpart in the reference, which runs a model of static shapes.
+ *
+ * Data (queries, keys, values, caches, logits, outputs) is fp32, fp16 or bf16, one type per call; indices are int32 or
+ * int64.  Sums, softmax statistics and scores are fp32 or wider; a result is rounded once, to its type.  Strides are free
+ * unless a function says otherwise; outputs must not overlap themselves or, but where it is said, inputs.  Tensors and
+ * stream are the current device's (FML_BAD_ARG for an output elsewhere).  Nothing is allocated and nothing kept between
+ * calls, so calls may run on several streams at once and in captured graphs; a workspace belongs to one call at a time. */
+
+/* Rotary positions: x [tokens, heads, head size], its first 2 * n features turned by the n `frequencies` (fp32, radians per
+ * position):  (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),  c, s = magnitude * cos, sin(positions[t] * frequency), the rest copied.
+ * Pair i is features (i, i + n) or (2 i, 2 i + 1).  The angle is formed and reduced in 64 bits.  q and k are turned, v is
+ * copied; each may be NULL together with its output.  Without `slots` an output has its input's shape and may be the input
+ * itself (same strides).  With `slots` k_out and v_out are paged caches [pages, page size, kv heads, head size]: token t
+ * goes to position slots[t] % page size of page slots[t] / page size; a negative slot (padding) is skipped, one beyond the
+ * cache is skipped and recorded in the device status word; which of several tokens with one slot stays is not defined. */
+typedef enum fml_rotary_layout { FML_ROTARY_HALVES = 0, FML_ROTARY_INTERLEAVED = 1 } fml_rotary_layout;
+int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, const fml_tensor *v, const fml_tensor *positions,
+                         const fml_tensor *slots, const fml_tensor *frequencies, float magnitude, int layout,
+                         const fml_tensor *q_out, const fml_tensor *k_out, const fml_tensor *v_out, void *stream);
+
+/* The rot / 2 frequencies f_i = base^(-2 i / rot), scaled for contexts beyond the trained length:
+ *   LINEAR  f / factor
+ *   NTK     base * factor^(rot / (rot - 2)) in place of base
+ *   BANDS   f ((1 - m) / factor + m), m = clamp((turns - turns_low) / (turns_high - turns_low), 0, 1), turns = trained_length f / 2 pi
+ *   RAMP    the same with m linear in i between the (whole) pairs that turn turns_high and turns_low times; magnitude
+ *           0.1 ln(factor) + 1 (1 with the others)
+ * Host computation; `frequencies` is a host array. */
+typedef enum fml_rotary_scaling {
+  FML_ROTARY_PLAIN = 0, FML_ROTARY_LINEAR = 1, FML_ROTARY_NTK = 2, FML_ROTARY_BANDS = 3, FML_ROTARY_RAMP = 4
+} fml_rotary_scaling;
+typedef struct fml_rotary_spec {
+  int32_t rot, scaling;
+  double base, factor, trained_length, turns_low, turns_high;
+} fml_rotary_spec;
+int fml_rotary_frequencies(const fml_rotary_spec *spec, float *frequencies, float *magnitude);
+
+/* How scores become weights: s = q . k / divisor;  with cap > 0  s = cap * tanh(s / cap);  with slopes  s -= slope[head] *
+ * |query position - key position|;  softmax over the visible keys.  A query that sees no key gives zeros.  Keys that a query
+ * does not see add nothing to it, whatever they hold. */
+typedef struct fml_score_rules {
+  float divisor, cap; /* cap 0: none */
+  int32_t causal;     /* fml_attention_rules only */
+} fml_score_rules;
+
+/* Attention over a prompt: q [batch, heads, S_q, D], k, v [batch, kv heads, S_k, D], out like q; heads a multiple of kv heads
+ * (consecutive heads share one); D a multiple of 4 up to 128.  Query i stands at position i + S_k - S_q, key j at j.
+ * Key j is visible when
+ *   - rules->causal is 0, or j <= the query's position, or prefix is given and j < prefix[batch], and
+ *   - documents are given and q_documents[batch, i] == k_documents[batch, j], or they are not.
+ * slopes [heads] fp32, prefix [batch], q_documents [batch, S_q] and k_documents [batch, S_k] may be NULL (the last two only
+ * together). */
+int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, const fml_tensor *v, const fml_tensor *slopes,
+                        const fml_tensor *prefix, const fml_tensor *q_documents, const fml_tensor *k_documents,
+                        const fml_score_rules *rules, const fml_tensor *out, void *stream);
+
+/* Attention of new tokens over a paged cache: request r has context[r] cached tokens and the new ("drafted") tokens
+ * query_start[r] .. query_start[r + 1] - 1 of q [tokens, heads, D], whose keys and values follow the context in the cache.
+ * k_cache, v_cache [pages, page size, kv heads, D], unit stride along D and rows on 16-byte boundaries (FML_MISALIGNED
+ * otherwise); block_table [requests, pages of a request] int32.  A new token sees the whole context and, with
+ * tree [tokens] int64, the new tokens j < 64 of its request whose bit j is set (its own included, if it is to see itself);
+ * without, those up to itself: the ordinary decoding step, for any number of tokens.  Positions for slopes: a cached token's
+ * index; context + depth for a new one, depth = how many of its request's tokens it sees, less one.
+ * query_start, context: int32.  Rows of out outside every request stay as they are.  Page numbers, lengths and row ranges
+ * beyond what the tensors hold are left out and recorded in the device status word.
+ * `workspace`: fml_attention_tree_workspace bytes at most, 16-byte aligned, for partial results of one call at a time. */
+size_t fml_attention_tree_workspace(int64_t requests, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_size);
+int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache, const fml_tensor *v_cache, const fml_tensor *block_table,
+                       const fml_tensor *context, const fml_tensor *query_start, const fml_tensor *tree, const fml_tensor *slopes,
+                       const fml_score_rules *rules, const fml_tensor *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* One token per row of logits [rows, vocabulary] from given random numbers.  A row's weights are exp((logit - largest) /
+ * temperature); of the tokens, ordered by logit, ties by index, it keeps the first top_k, of those the first whose weights
+ * before them sum to less than top_p of the sum (one at least), of those the ones with a weight of at least min_p; the token
+ * is the first, in the vocabulary's order, at which the running sum of kept weights exceeds uniform * their sum.
+ * temperature, top_p, min_p [rows] fp32, top_k [rows] int32 or int64: NULL = off for all rows; off for a row: temperature not
+ * above 0 (the largest logit, lowest index; below 1e-30 it counts as that), top_k <= 0, top_p >= 1, min_p <= 0, NaN.  NaN logits are never drawn; infinite
+ * ones share the draw; a row without a token to draw gives token -1, probability 0.  uniform [rows] fp32 in [0, 1).
+ * Weights are whole multiples of 2^-44 of the largest (never less than one for a token that can be drawn), so sums are exact
+ * and do not depend on their order.  tokens [rows] int32 or int64; probabilities [rows] fp32 (of the tokens among the kept
+ * ones) may be NULL.  At most 2^18 tokens. */
+int fml_sample(const fml_tensor *logits, const fml_tensor *uniform, const fml_tensor *temperature, const fml_tensor *top_k,
+               const fml_tensor *top_p, const fml_tensor *min_p, const fml_tensor *tokens, const fml_tensor *probabilities,
+               void *stream);
 
 /* ---------------------------------------------------------------- resident stage program
  * The reference runs a whole model as ONE call into one compiled function

@@ -1,0 +1,202 @@
+"""fml_attention_rules against a plain implementation in 64 bits; the bound is derived in serving_oracle.bound."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from fluidml_b200 import cabi
+from serving_oracle import TYPES, attention, close
+
+
+def randn(seed, *shape, dtype=torch.float32):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def visible_of(sq, sk, causal, prefix, qd, kd):
+    at, key = torch.arange(sq)[:, None] + sk - sq, torch.arange(sk)[None, :]
+    see = torch.ones(sq, sk, dtype=torch.bool)
+    if causal:
+        see = key <= at
+        if prefix is not None:
+            see = see | (key < prefix)
+    if qd is not None:
+        see = see & (qd[:, None] == kd[None, :])
+    return see
+
+
+def run(q, k, v, divisor=None, cap=0.0, causal=False, slopes=None, prefix=None, qd=None, kd=None, out=None, fill=7.0, heads=None):
+    """Calls the operator on views as they are and holds every row of the given heads to the oracle."""
+    b, h, sq, d = q.shape
+    kv, sk = k.shape[1:3]
+    divisor = divisor or math.sqrt(d)
+    if out is None:
+        out = torch.full((b, h, sq, d), fill, dtype=q.dtype).cuda()
+    on = lambda x: None if x is None else x.cuda()  # noqa: E731
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, divisor, cap=cap, causal=causal, slopes=on(slopes), prefix=on(prefix),
+                         q_documents=on(qd), k_documents=on(kd))
+    cabi.check_device()
+    got = out.cpu()
+    for i in range(b):
+        see = visible_of(sq, sk, causal, None if prefix is None else int(prefix[i]), None if qd is None else qd[i], None if kd is None else kd[i])
+        for j in range(h) if heads is None else heads:
+            bias = None
+            if slopes is not None:
+                bias = -slopes[j].double() * ((torch.arange(sq)[:, None] + sk - sq) - torch.arange(sk)[None, :]).abs().double()
+            want, size = attention(q[i, j].cpu(), k[i, j * kv // h].cpu(), v[i, j * kv // h].cpu(), see, divisor, cap, bias)
+            assert close(got[i, j], want, size, q.dtype), (i, j, float((got[i, j].double() - want).abs().max()))
+    return got
+
+
+SLOPES = torch.tensor([0.5, 0.25, 0.125, 0.0625])
+LENGTHS = [(1, 1), (7, 7), (64, 64), (65, 63), (77, 77), (1, 200), (130, 40), (129, 257)]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [4, 32, 64, 80, 128])
+@pytest.mark.parametrize("sq,sk", LENGTHS)
+def test_lengths_and_head_sizes(dtype, d, sq, sk):
+    t = TYPES[dtype]
+    q, k, v = randn(1, 1, 2, sq, d, dtype=t), randn(2, 1, 1, sk, d, dtype=t), randn(3, 1, 1, sk, d, dtype=t)
+    run(q, k, v)
+    run(q, k, v, causal=True)  # more queries than keys: the first see nothing and are zero
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("cap", [0.0, 5.0, 50.0])
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("kind", ["both", "causal", "prefix", "documents", "causal documents", "prefix documents"])
+def test_rules_together(dtype, cap, bias, kind):
+    t, b, s, d = TYPES[dtype], 2, 150, 64
+    q, k, v = randn(4, b, 4, s, d, dtype=t) * 2, randn(5, b, 2, s, d, dtype=t), randn(6, b, 2, s, d, dtype=t)
+    prefix = torch.tensor([0, 90], dtype=torch.int32) if "prefix" in kind else None
+    docs = torch.stack((torch.repeat_interleave(torch.arange(4), torch.tensor([1, 70, 0, 79])[torch.tensor([0, 1, 3, 2])]),
+                        torch.arange(s) % 3)) if "documents" in kind else None  # in a row, and interleaved
+    run(q, k, v, cap=cap, causal=kind != "both" and kind != "documents", slopes=SLOPES if bias else None, prefix=prefix, qd=docs, kd=docs)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_queries_whose_document_has_no_key(dtype):
+    t = TYPES[dtype]
+    q, k, v = randn(7, 1, 2, 70, 64, dtype=t), randn(8, 1, 2, 140, 64, dtype=t), randn(9, 1, 2, 140, 64, dtype=t)
+    qd = torch.arange(70)[None] // 10
+    kd = torch.arange(140)[None] // 20 * 2  # the odd ones are missing
+    got = run(q, k, v, qd=qd, kd=kd)
+    assert (got[:, :, (qd[0] % 2 == 1)] == 0).all()
+    run(q, k, v, qd=qd.to(torch.int32), kd=kd + (1 << 33))  # nothing seen at all, and numbers of either width
+    run(q, k, torch.full_like(v, math.nan), qd=qd, kd=kd + (1 << 33))
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_what_is_not_seen_adds_nothing(dtype, value):
+    t, s = TYPES[dtype], 200
+    q, k, v = randn(10, 1, 2, s, 64, dtype=t), randn(11, 1, 1, s, 64, dtype=t), randn(12, 1, 1, s, 64, dtype=t)
+    docs = torch.zeros(1, s, dtype=torch.int32)
+    docs[0, 150:] = 1
+    for x in (k, v):
+        kept = x.clone()
+        x[0, 0, 150:160] = value  # seen by the second document alone
+        out = torch.empty(1, 2, s, 64, dtype=t).cuda()
+        cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, 8.0, causal=True, q_documents=docs.cuda(), k_documents=docs.cuda())
+        for h in range(2):
+            want, size = attention(q[0, h, :150], k[0, 0, :150], v[0, 0, :150], visible_of(150, 150, True, None, None, None), 8.0)
+            assert close(out[0, h, :150], want, size, t)
+        x.copy_(kept)
+    v[0, 0, 20] = value  # seen by the later ones: theirs are not finite, the others' are as before
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, 8.0, causal=True)
+    want, size = attention(q[0, 0, :20], k[0, 0, :20], v[0, 0, :20], visible_of(20, 20, True, None, None, None), 8.0)
+    assert close(out[0, 0, :20], want, size, t) and not out[0, 0, 20:].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_strides_and_alignment(dtype):
+    t = TYPES[dtype]
+    b, s, d = 2, 70, 64
+    for make in (lambda x: x.transpose(1, 2).contiguous().transpose(1, 2),                      # heads are columns of the rows
+                 lambda x: torch.cat((x, x[..., :1]), -1).contiguous()[..., :d],                # rows of 65
+                 lambda x: torch.cat((x[..., :1], x), -1).contiguous()[..., 1:],                # and off the boundary
+                 lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)):                     # features outermost
+        q, k, v = (make(randn(i, b, h, s, d, dtype=t)).cuda() for i, h in ((13, 4), (14, 2), (15, 2)))
+        out = make(torch.zeros(b, 4, s, d, dtype=t)).cuda()
+        if out.stride() != q.stride():
+            out = torch.empty_strided(q.shape, q.stride(), dtype=t, device="cuda") if q.stride(3) != 1 or q.stride(2) == d else out
+        run(q, k, v, causal=True, out=out)
+    # one key and value for every batch and head, a documents row for every batch
+    q, k, v = randn(16, b, 4, s, d, dtype=t), randn(17, 1, 1, s, d, dtype=t).expand(b, 2, s, d), randn(18, 1, 1, s, d, dtype=t).expand(b, 2, s, d)
+    run(q, k, v, qd=(torch.arange(s) // 30).expand(b, s), kd=(torch.arange(s) // 30).expand(b, s))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("kind", ["both", "causal", "prefix bias", "documents cap"])
+def test_larger_problems(dtype, d, kind):
+    """Sizes that the fifth-generation tensor cores take; two heads are held to the oracle."""
+    t, b, s, h, kv = TYPES[dtype], 2, 1100, 16, 4
+    q, k, v = randn(19, b, h, s, d, dtype=t), randn(20, b, kv, s, d, dtype=t), randn(21, b, kv, s, d, dtype=t)
+    docs = torch.stack((torch.arange(s) // 300, (torch.arange(s) > 517).long())) if "documents" in kind else None
+    slopes = torch.tensor([2.0 ** (-(i + 1) / 2) for i in range(h)]) if "bias" in kind else None
+    run(q, k, v, cap=20.0 if "cap" in kind else 0.0, causal=kind != "both", slopes=slopes,
+        prefix=torch.tensor([700, 0]) if "prefix" in kind else None, qd=docs, kd=docs, heads=(0, 13))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_larger_problems_with_rows_that_see_nothing_and_infinities(dtype):
+    t, s, h, d = TYPES[dtype], 1300, 24, 64
+    q, k, v = randn(22, 1, h, s, d, dtype=t), randn(23, 1, h, s, d, dtype=t), randn(24, 1, h, s, d, dtype=t)
+    v[:, :, 1200:] = math.inf
+    k[:, :, 1250:] = math.nan
+    docs = torch.arange(s)[None] // 100
+    qd = docs.clone()
+    qd[:, 300:420] = 99  # see nothing
+    qd[:, 1200:] = -1
+    run(q, k, v, causal=True, qd=qd, kd=docs, heads=(0, 7))
+    run(q, k[:, :, :900], v[:, :, :900], causal=True, heads=(3,))  # more queries than keys
+
+
+def test_large_scores():
+    """Scores of hundreds: the running maximum moves, and weights of distant keys vanish."""
+    for dtype in TYPES.values():
+        q, k, v = randn(25, 1, 2, 300, 64, dtype=dtype) * 16, randn(26, 1, 2, 300, 64, dtype=dtype), randn(27, 1, 2, 300, 64, dtype=dtype)
+        out = torch.empty(1, 2, 300, 64, dtype=dtype).cuda()
+        cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, 8.0, causal=True)
+        for h in range(2):
+            want, size = attention(q[0, h], k[0, h], v[0, h], visible_of(300, 300, True, None, None, None), 8.0)
+            # scores sixteen times as large as the bound is derived for
+            step = torch.finfo(dtype).eps / 2
+            assert ((out[0, h].double().cpu() - want).abs() <= (step * (dtype != torch.float32) + 16 * 3e-4) * size + step * want.abs() + 1e-7).all()
+
+
+def test_two_streams_and_a_captured_graph():
+    t = torch.bfloat16
+    x = [(randn(30 + i, 1, 8, 1000, 64, dtype=t).cuda(), randn(40 + i, 1, 8, 1000, 64, dtype=t).cuda()) for i in range(2)]
+    want = [torch.empty_like(q) for q, _ in x]
+    for (q, k), o in zip(x, want):
+        cabi.attention_rules(q, k, k, o, 8.0, causal=True)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in x], [torch.empty_like(q) for q, _ in x]
+    for _ in range(10):
+        for (q, k), o, s in zip(x, outs, streams):
+            cabi.attention_rules(q, k, k, o, 8.0, causal=True, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, outs))
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(want[0])
+    q, k = (a.clone() for a in x[0])
+    s = streams[0]
+    with torch.cuda.graph(graph, stream=s):
+        cabi.attention_rules(q, k, k, out, 8.0, causal=True, stream=s.cuda_stream)
+    q.copy_(x[1][0]); k.copy_(x[1][1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[1])
+
+
+def test_empty():
+    e = torch.empty(0, 2, 5, 64).cuda()
+    cabi.attention_rules(e, e, e, e.clone(), 8.0)
+    q, k = torch.ones(1, 2, 5, 64).cuda(), torch.empty(1, 2, 0, 64).cuda()
+    out = torch.full_like(q, 7)
+    cabi.attention_rules(q, k, k, out, 8.0)
+    assert (out == 0).all()  # no key: zeros
+    cabi.attention_rules(torch.empty(1, 2, 0, 64).cuda(), q, q, torch.empty(1, 2, 0, 64).cuda(), 8.0)
