@@ -446,26 +446,30 @@ def _arg(t):
     before it returns."""
     if t is None:
         return None
-    if hasattr(t, "data_ptr"):
-        code = _DTYPES.get(t.dtype)
-        if code is None:
-            code = _SERVING_CODE.get(str(t.dtype))
-            if code is None:
-                raise FmlError(2, f"no kernel takes {t.dtype}")
-            _DTYPES[t.dtype] = code
-        if t.device.type != "cuda":
+    if isinstance(t, (DeviceTensor, Tensor)):
+        return ctypes.byref(t if isinstance(t, Tensor) else t.c())
+    # (one packed block of bytes: a ctypes structure costs several times as much, and a small call is mostly this)
+    shape = t.shape
+    code = _DTYPES.get(t.dtype)
+    if code is None or not t.is_cuda or len(shape) > MAX_RANK:
+        code = _DTYPES.setdefault(t.dtype, _SERVING_CODE.get(str(t.dtype), 0))
+        if code == 0:
+            raise FmlError(2, f"no kernel takes {t.dtype}")
+        if not t.is_cuda:
             raise FmlError(1, f"a tensor on {t.device} was given where device memory is needed")
-        shape = t.shape
         if len(shape) > MAX_RANK:
             raise FmlError(1, f"at most {MAX_RANK} dims")
-        return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape, *t.stride())
-    return ctypes.byref(t if isinstance(t, Tensor) else t.c())
+    return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape, *t.stride())
+
+
+_FUNCTIONS: dict = {}
 
 
 def _serving(name, *types):
-    """A function of the library with its argument types set (once)."""
-    f = getattr(lib(), name)
-    if f.argtypes is None:
+    """A function of the library with its argument types (set at its first use)."""
+    f = _FUNCTIONS.get(name)
+    if f is None:
+        f = _FUNCTIONS[name] = getattr(lib(), name)
         f.argtypes = list(types)
     return f
 
@@ -475,7 +479,7 @@ _P, _F, _I = ctypes.c_void_p, ctypes.c_float, ctypes.c_int
 
 def rotary_positions(q, k, v, positions, slots, frequencies, q_out, k_out, v_out, magnitude=1.0, layout=ROTARY_HALVES, stream=None):
     """Turns q and k by their positions; with slots, k and v go into a paged cache (fml_rotary_positions)."""
-    f = _serving("fml_rotary_positions", _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P, _P)
+    f = _FUNCTIONS.get("fml_rotary_positions") or _serving("fml_rotary_positions", _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P, _P)
     check(f(_arg(q), _arg(k), _arg(v), _arg(positions), _arg(slots), _arg(frequencies), magnitude, layout, _arg(q_out), _arg(k_out),
             _arg(v_out), stream))
 
@@ -490,7 +494,7 @@ def rotary_frequencies(rot, scaling=ROTARY_PLAIN, base=10000.0, factor=1.0, trai
 
 def attention_rules(q, k, v, out, divisor, cap=0.0, causal=False, slopes=None, prefix=None, q_documents=None, k_documents=None, stream=None):
     """Attention over a prompt with capped scores, a distance bias, documents and a prefix (fml_attention_rules)."""
-    f = _serving("fml_attention_rules", *[_P] * 10)
+    f = _FUNCTIONS.get("fml_attention_rules") or _serving("fml_attention_rules", *[_P] * 10)
     rules = ScoreRules(divisor, cap, 1 if causal else 0)
     check(f(_arg(q), _arg(k), _arg(v), _arg(slopes), _arg(prefix), _arg(q_documents), _arg(k_documents), ctypes.byref(rules), _arg(out), stream))
 
@@ -505,7 +509,7 @@ def attention_tree_workspace(requests, tokens, heads, kv_heads, head_size) -> in
 def attention_tree(q, k_cache, v_cache, block_table, context, query_start, tree, out, workspace, divisor, cap=0.0, slopes=None, stream=None):
     """Attention of new tokens (a chain, or with `tree` a tree of drafts) over a paged cache (fml_attention_tree).
     `workspace`: a DeviceBuffer, or any array of bytes on the device with data_ptr() and numel()."""
-    f = _serving("fml_attention_tree", *[_P] * 11, ctypes.c_size_t, _P)
+    f = _FUNCTIONS.get("fml_attention_tree") or _serving("fml_attention_tree", *[_P] * 11, ctypes.c_size_t, _P)
     rules = ScoreRules(divisor, cap, 1)
     if isinstance(workspace, DeviceBuffer):
         place, size = workspace.ptr, workspace.nbytes
@@ -517,7 +521,7 @@ def attention_tree(q, k_cache, v_cache, block_table, context, query_start, tree,
 
 def sample(logits, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, probabilities=None, stream=None):
     """One token per row of logits from given random numbers (fml_sample)."""
-    f = _serving("fml_sample", *[_P] * 9)
+    f = _FUNCTIONS.get("fml_sample") or _serving("fml_sample", *[_P] * 9)
     check(f(_arg(logits), _arg(uniform), _arg(temperature), _arg(top_k), _arg(top_p), _arg(min_p), _arg(tokens), _arg(probabilities), stream))
 
 

@@ -229,6 +229,7 @@ extern "C" int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, con
   a.q_vec = vec(q); a.k_vec = vec(k); a.v_vec = vec(v);
   a.status = device_status_word();
   FML_REQUIRE(a.status, FML_CUDA_ERROR, "fml_attention_rules: no device status word");
+  if (attention_rules_tc_eligible(a, q->dtype)) return launch_attention_rules_tc(a, q->dtype, as_stream(stream));
   if (q->dtype == FML_F32) return launch_mma<float>(a, as_stream(stream));
   if (q->dtype == FML_F16) return launch_mma<__half>(a, as_stream(stream));
   return launch_mma<__nv_bfloat16>(a, as_stream(stream));

@@ -19,6 +19,10 @@ struct RulesArgs {
   int *status;
 };
 
+// attention_rules_tc.cu: whether its kernel takes these operands, and its launch.
+bool attention_rules_tc_eligible(const RulesArgs &a, int dtype);
+int launch_attention_rules_tc(const RulesArgs &a, int dtype, cudaStream_t s);
+
 __device__ __forceinline__ int64_t document_at(const IndexView &v, int64_t row, int batch, int i) {
   const int64_t e = batch * row + i * v.stride;
   return v.wide ? static_cast<const int64_t *>(v.p)[e] : (int64_t)static_cast<const int32_t *>(v.p)[e];

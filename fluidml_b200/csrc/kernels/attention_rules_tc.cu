@@ -1,0 +1,495 @@
+// fml_attention_rules on the fifth-generation tensor cores: fp16 and bf16, head sizes that are multiples of 16.
+//
+// One CTA per SM takes 256 queries of a head as two tiles of 128 rows, A and B, against the same tiles of 128 keys.  Scores and
+// contexts are accumulators in tensor memory (all 512 columns of it); weights go back over their scores, in the operands' type, as
+// the A operand of the second product.
+//
+//   warps 0-3, 4-7  softmax of tile A, B: thread = query = lane of tensor memory
+//   warp 8          loads (tensor maps, 128-byte swizzle): Q once, K and V tiles into two stages each
+//   (warps 10, 11    make up the third group of four, which gives its registers to the softmax groups: 128 scores of a row stay
+//                    in registers; 2 x 128 x 224 + 128 x 56 = 384 x 168, what the launch has)
+//   warp 9          products, in the order  S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j): while one tile's softmax runs, the tensor cores
+//                   work for the other
+//
+// What bounds it.  A tile of 128 x 128 is 512 clocks of tensor core for either product at head size 128 (256 at 64) and 16384
+// exponentials at 16 a clock, 1024: per pair of products as much as they take at head size 128, twice as much at 64.  A capped
+// score by two more such instructions would triple that, so tanh is a polynomial on packed pairs (below).
+//
+// The running maximum follows only when a tile's exceeds it by more than 8 (in units of ln 2): weights then reach 2^8, which the
+// sums carry, and the context's correction, a round trip through registers, is rare.  The commit that publishes S(j) also covers
+// PV(j - 1), issued before it, so the correction needs no barrier of its own.
+#include "attention_rules.cuh"
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+namespace fml {
+namespace {
+
+constexpr int kThreads = 384, kRows = 128, kKeys = 128, kMaxTiles = 2048;
+constexpr uint32_t kColS = 0, kColO = 256;  // two of 128 columns each
+
+struct TcBarriers {  // offsets of 8 bytes
+  enum { kQ = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kS = 10, kP = 12, kDone = 14, kDrain = 15, kCount = 16 };
+};
+
+template <int DP> struct TcShape {
+  static constexpr int kTile = 128 * DP * 2;  // bytes of 128 rows
+  static constexpr int kBoxes = DP / 64;      // of 64 features: 128 bytes, one swizzle row
+  static constexpr size_t kBytes = 6 * kTile + 8 * kKeys * 8 + kMaxTiles + TcBarriers::kCount * 8 + 16;
+};
+
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float *v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]),
+        "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]),
+        "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr) : "memory");
+}
+// The values pass through the wait, so that nothing that uses them is moved in front of it.
+__device__ __forceinline__ void tmem_ld_tie(float *v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
+                 "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]),
+                 "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]),
+                 "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+               :: "memory");
+}
+
+// Two fp32 operations per instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Instruction descriptor of kind::f16 with fp32 sums: type 0 fp16, 1 bf16; M = 128; B along its columns (1) or along k (0).
+__device__ __forceinline__ uint32_t instr_desc_16(uint32_t type, int n, uint32_t b_mn_major) {
+  return (1u << 4) | (type << 7) | (type << 10) | (b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RulesArgs a) {
+  using S = TcShape<DP>;
+  using B = TcBarriers;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  // [ Q of A | Q of B | K stage 0, 1 | V stage 0, 1 | documents of a tile, per softmax warp | views | barriers ]
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * S::kTile, v_s = k_s + 2 * S::kTile;
+  int64_t *const documents = reinterpret_cast<int64_t *>(smem + 6 * S::kTile);
+  uint8_t *const views = reinterpret_cast<uint8_t *>(documents + 8 * kKeys);  // [tile]: view of A | view of B << 2
+  uint64_t *const bars = reinterpret_cast<uint64_t *>(views + kMaxTiles);
+  const uint32_t bar = smem_u32(bars);
+  uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(bars + B::kCount);
+  volatile int *const abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const bool leader = elect_one();
+  const int head = blockIdx.y, batch = blockIdx.z, kv = head / a.group;
+  const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * 2 * kRows;  // (causal: the longest first)
+  const bool two = row0 + kRows < a.Sq;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_map(&map_q);
+    tma_prefetch_map(&map_k);
+    tma_prefetch_map(&map_v);
+    for (int i = 0; i < B::kCount; ++i) mbar_init(bar + 8u * i, i >= B::kP && i < B::kP + 2 ? 4 : 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_launch_dependents();  // (only now: tensor memory)
+  pdl_wait();
+
+  // ---- what the two tiles see of each tile of keys
+  const TileRange ra = tile_range(a, batch, row0, min(row0 + kRows, a.Sq));
+  const TileRange rb = two ? tile_range(a, batch, row0 + kRows, min(row0 + 2 * kRows, a.Sq)) : ra;
+  const int tiles = (max(ra.last_key, rb.last_key) + kKeys - 1) / kKeys;
+  for (int i = warp; i < tiles; i += kThreads / 32) {
+    const int va = tile_view(a, batch, ra, i * kKeys, kKeys), vb = two ? tile_view(a, batch, rb, i * kKeys, kKeys) : 0;
+    if (lane == 0) views[i] = (uint8_t)(va | vb << 2);
+  }
+  __syncthreads();
+
+  bool ok = true;
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  if (warp == 8) {
+    // ------------------------------------------------------------ loads
+    if (g_drop_loads != 1) {
+      if (leader) {
+        for (int t = 0; t < (two ? 2 : 1); ++t) {
+          mbar_expect_tx(bar + 8u * (B::kQ + t), S::kTile);
+          for (int i = 0; i < S::kBoxes; ++i)
+            tma_load_4d(q_s + (uint32_t)(t * S::kTile + i * 16384), &map_q, bar + 8u * (B::kQ + t), 64 * i, row0 + t * kRows, a.q_s[1] ? head : 0,
+                        a.q_s[0] ? batch : 0);
+        }
+      }
+      int n = 0, n_k = 0;
+      for (int i = 0; i < tiles && ok; ++i) {
+        if (!views[i]) continue;
+        const uint32_t s = (uint32_t)n & 1u, free_parity = ((uint32_t)(n >> 1) & 1u) ^ 1u;
+        ok = mbar_wait_warp(bar + 8u * (B::kKEmpty + s), free_parity, abort_flag);
+        if (!ok) break;
+        if (leader) {
+          mbar_expect_tx(bar + 8u * (B::kKFull + s), S::kTile);
+          for (int b = 0; b < S::kBoxes; ++b)
+            tma_load_4d(k_s + s * S::kTile + b * 16384, &map_k, bar + 8u * (B::kKFull + s), 64 * b, i * kKeys, a.k_s[1] ? kv : 0, a.k_s[0] ? batch : 0);
+        }
+        ++n_k;
+        ok = mbar_wait_warp(bar + 8u * (B::kVEmpty + s), free_parity, abort_flag);
+        if (!ok) break;
+        if (leader) {
+          mbar_expect_tx(bar + 8u * (B::kVFull + s), S::kTile);
+          for (int b = 0; b < S::kBoxes; ++b)
+            tma_load_4d(v_s + s * S::kTile + b * 16384, &map_v, bar + 8u * (B::kVFull + s), 64 * b, i * kKeys, a.v_s[1] ? kv : 0, a.v_s[0] ? batch : 0);
+        }
+        ++n;
+      }
+      if (!ok) {  // bounded wait for the loads in flight
+        volatile int never = 0;
+        for (int t = 0; t < (two ? 2 : 1); ++t) mbar_wait_warp(bar + 8u * (B::kQ + t), 0u, &never);
+        for (int j = max(0, n_k - 2); j < n_k; ++j) mbar_wait_warp(bar + 8u * (B::kKFull + (j & 1)), (uint32_t)(j >> 1) & 1u, &never);
+        for (int j = max(0, n - 2); j < n; ++j) mbar_wait_warp(bar + 8u * (B::kVFull + (j & 1)), (uint32_t)(j >> 1) & 1u, &never);
+      }
+    }
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ products
+    const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc_s = instr_desc_16(type, kKeys, 0u), idesc_o = instr_desc_16(type, a.D, 1u);
+    const uint64_t desc_q = smem_desc(q_s, 16u, 1024u), desc_k = smem_desc(k_s, 16u, 1024u), desc_v = smem_desc(v_s, 16384u, 1024u);
+    const int steps = a.D / 16;
+    uint32_t n = 0, done[2] = {0u, 0u}, last_stage = 0;  // tiles of keys; weights taken per query tile; B's last tile
+    bool pending = false;                                 // B's product with V of the tile before
+    bool first_o[2] = {true, true};
+    auto scores = [&](int t, uint32_t stage) {
+      if (leader) {
+        for (int k = 0; k < steps; ++k) {
+          // 32 bytes of a swizzle row per step; four steps to a box
+          const uint64_t off = (uint64_t)((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+          umma_f16_ss(tmem + kColS + 128u * t, desc_q + (uint64_t)(t * S::kTile >> 4) + off, desc_k + (uint64_t)(stage * S::kTile >> 4) + off, idesc_s,
+                      k ? 1u : 0u);
+        }
+        umma_commit(bar + 8u * (B::kS + t));
+      }
+      __syncwarp();
+    };
+    auto context = [&](int t, uint32_t stage) {
+      ok = mbar_wait_warp(bar + 8u * (B::kP + t), done[t] & 1u, abort_flag);
+      if (!ok) return;
+      ++done[t];
+      tc_fence_after();
+      if (leader) {
+        for (int k = 0; k < kKeys / 16; ++k)
+          umma_f16_ts(tmem + kColO + 128u * t, tmem + kColS + 128u * t + 8u * k, desc_v + (uint64_t)((stage * S::kTile + k * 2048) >> 4), idesc_o,
+                      first_o[t] && k == 0 ? 0u : 1u);
+      }
+      __syncwarp();
+      first_o[t] = false;
+    };
+    auto release_v = [&](uint32_t stage) {
+      if (leader) umma_commit(bar + 8u * (B::kVEmpty + stage));
+      __syncwarp();
+    };
+    ok = mbar_wait_warp(bar + 8u * B::kQ, 0u, abort_flag) && (!two || mbar_wait_warp(bar + 8u * (B::kQ + 1), 0u, abort_flag));
+    for (int i = 0; i < tiles && ok; ++i) {
+      const int view = views[i];
+      if (!view) continue;
+      const uint32_t stage = n & 1u, parity = (n >> 1) & 1u;
+      ok = mbar_wait_warp(bar + 8u * (B::kKFull + stage), parity, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      if (view & 3) scores(0, stage);
+      if (pending) {
+        context(1, last_stage);
+        if (!ok) break;
+        release_v(last_stage);
+        pending = false;
+      }
+      if (view >> 2) scores(1, stage);
+      if (leader) umma_commit(bar + 8u * (B::kKEmpty + stage));
+      __syncwarp();
+      ok = mbar_wait_warp(bar + 8u * (B::kVFull + stage), parity, abort_flag);
+      if (!ok) break;
+      if (view & 3) context(0, stage);
+      if (!ok) break;
+      if (view >> 2) {
+        pending = true;
+        last_stage = stage;
+      } else {
+        release_v(stage);
+      }
+      ++n;
+    }
+    if (ok && pending) context(1, last_stage);
+    if (ok && leader) umma_commit(bar + 8u * B::kDone);
+    if (!ok) *abort_flag = 1;
+    if (leader) umma_drain(bar + 8u * B::kDrain);
+    __syncwarp();
+  }
+  } else {
+    // ------------------------------------------------------------ softmax: thread = query
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int t = warp >> 2, local = threadIdx.x & 127;
+    const int i = row0 + t * kRows + local, row = min(i, a.Sq - 1);
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lane_addr + kColS + 128u * t, col_o = lane_addr + kColO + 128u * t;
+    const RowRules r = row_rules(a, batch, head, row);
+    const bool whole_sign = !CAP && !BIAS && a.cap.scale > 0.0f;  // the largest product is the largest score
+    int64_t *const docs = documents + warp * kKeys;
+    float m = -INFINITY, l = 0.0f;
+    uint32_t n = 0;
+    if (t == 0 || two) {
+      for (int tile = 0; tile < tiles && ok; ++tile) {
+        const int view = views[tile] >> (2 * t) & 3;
+        if (view == kTileNone) continue;
+        const int key0 = tile * kKeys;
+        if (view == kTileSome && a.k_documents.p) {  // (a copy per warp: a barrier among warps could be left by one that gave up)
+          __syncwarp();
+          for (int j = lane; j < kKeys; j += 32)
+            docs[j] = key0 + j < a.Sk ? document_at(a.k_documents, a.k_documents_row, batch, key0 + j) : 0;
+          __syncwarp();
+        }
+        ok = mbar_wait_warp(bar + 8u * (B::kS + t), n & 1u, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        float v[kKeys];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_start(col_s + 32u * c, v + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_tie(v + 32 * c);
+        // scores in units of ln 2 (without cap and bias they stay products, scaled on the way into the exponential)
+        if (CAP) {
+          const float2 f = both(a.cap.scale);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float far = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float2 x = mul2(make_float2(v[32 * c + j], v[32 * c + j + 1]), f);
+              v[32 * c + j] = x.x;
+              v[32 * c + j + 1] = x.y;
+              far = fmaxf(far, fmaxf(fabsf(x.x), fabsf(x.y)));
+            }
+            if (__all_sync(0xffffffffu, far <= 1.0f)) {
+              // tanh(x) = x P(x^2) on [-1, 1]: least squares reweighted to the smallest largest error, 2.4e-7
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                const float2 x = make_float2(v[32 * c + j], v[32 * c + j + 1]), u = mul2(x, x);
+                float2 p = fma2(u, both(-0.00283947f), both(0.01611418f));
+                p = fma2(u, p, both(-0.05097286f));
+                p = fma2(u, p, both(0.13253525f));
+                p = fma2(u, p, both(-0.33324004f));
+                p = fma2(u, p, both(0.99999685f));
+                p = mul2(mul2(p, x), both(a.cap.cap));
+                v[32 * c + j] = p.x;
+                v[32 * c + j + 1] = p.y;
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[32 * c + j] = a.cap.cap * tanh_of<false>(v[32 * c + j]);
+            }
+          }
+        } else if (BIAS || !whole_sign) {
+#pragma unroll
+          for (int j = 0; j < kKeys; ++j) v[j] *= a.cap.scale;
+        }
+        if (BIAS) {
+          const float at = (float)(r.at - key0);
+#pragma unroll
+          for (int j = 0; j < kKeys; ++j) v[j] = fmaf(-r.slope, fabsf(at - (float)j), v[j]);
+        }
+        if (view == kTileSome) {
+          const int last = r.last - key0;
+          if (a.k_documents.p) {
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j)
+              if (j >= last || docs[j] != r.document) v[j] = -INFINITY;
+          } else {
+#pragma unroll
+            for (int j = 0; j < kKeys; ++j)
+              if (j >= last) v[j] = -INFINITY;
+          }
+        }
+        float m_tile = v[0];
+#pragma unroll
+        for (int j = 1; j < kKeys; ++j) m_tile = fmaxf(m_tile, v[j]);
+        const float scale = !CAP && !BIAS && whole_sign ? a.cap.scale : 1.0f;
+        m_tile *= scale;
+        if (n == 0) {
+          m = m_tile;
+        } else if (__any_sync(0xffffffffu, m_tile > m + 8.0f)) {
+          const float m_new = fmaxf(m, m_tile), f = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+          l *= f;
+          m = m_new;
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tmem_ld32_start(col_o + (uint32_t)c, o);
+            tmem_ld_tie(o);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] *= f;
+            tmem_st32(col_o + (uint32_t)c, reinterpret_cast<const uint32_t *>(o));
+          }
+          tmem_wait_st();
+        }
+        const float2 base = both(m == -INFINITY ? 0.0f : -m), s2 = both(scale);
+        float2 sum = both(0.0f);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float2 x = fma2(make_float2(v[64 * c + 2 * j], v[64 * c + 2 * j + 1]), s2, base);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum = add2(sum, e);
+            p[j] = pack2<T>(e.x, e.y);
+          }
+          tmem_st32(col_s + 32u * c, p);
+        }
+        l += sum.x + sum.y;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar + 8u * (B::kP + t));
+        ++n;
+      }
+      // ---- out = O / l
+      if (ok) ok = mbar_wait_warp(bar + 8u * B::kDone, 0u, abort_flag);
+      if (ok) {
+        tc_fence_after();
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros; NaN stays)
+        T *const dst = static_cast<T *>(a.out) + batch * a.o_s[0] + head * a.o_s[1] + (int64_t)row * a.o_s[2];
+        const bool wide = a.o_s[3] == 1 && a.o_s[2] % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < DP; c += 32) {
+          if (c >= a.D) break;
+          float o[32];
+          if (n > 0) {
+            __syncwarp();
+            tmem_ld32_start(col_o + (uint32_t)c, o);
+            tmem_ld_tie(o);
+          }
+          uint32_t x[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float x0 = l == 0.0f ? 0.0f : o[j] * inv, x1 = l == 0.0f ? 0.0f : o[j + 1] * inv;
+            bad = bad || (c + j < a.D && !(fabsf(x0) <= FLT_MAX && fabsf(x1) <= FLT_MAX));
+            x[j / 2] = pack2<T>(x0, x1);
+          }
+          if (i < a.Sq) {
+            if (wide) {
+#pragma unroll
+              for (int j = 0; j < 16; j += 4)
+                if (c + 2 * j < a.D) *reinterpret_cast<uint4 *>(dst + c + 2 * j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (c + j < a.D) dst[(int64_t)(c + j) * a.o_s[3]] = reinterpret_cast<const T *>(x)[j];
+            }
+          }
+        }
+        unsigned redo = __ballot_sync(0xffffffffu, bad && i < a.Sq);
+        __syncwarp();
+        while (redo) {
+          const int which = __ffs(redo) - 1;
+          redo &= redo - 1;
+          redo_rules_row<T>(a, batch, head, row0 + t * kRows + (warp & 3) * 32 + which);
+        }
+      }
+    }
+  }
+  if (!ok) {
+    if (leader) atomicOr(a.status, kStatusTimeout);
+    *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// [batch][head][row][feature] in boxes of 64 features x 128 rows, zeros outside; dims of stride 0 have extent 1.
+int rules_map(CUtensorMap *map, const void *base, int dtype, int64_t d, int64_t rows, const int64_t *s, int64_t heads, int64_t batch) {
+  EncodeTiledFn fn = encode_fn();
+  FML_REQUIRE(fn, FML_CUDA_ERROR, "fml_attention_rules: cuTensorMapEncodeTiled is not available");
+  const int64_t any = (d + 7) / 8 * 8;  // a stride that is valid where the extent is 1
+  const bool h = s[1] != 0 && heads > 1, b = s[0] != 0 && batch > 1;
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)(h ? heads : 1), (cuuint64_t)(b ? batch : 1)};
+  cuuint64_t strides[3] = {(cuuint64_t)(rows > 1 ? s[2] : any) * 2, (cuuint64_t)(h ? s[1] : any) * 2, (cuuint64_t)(b ? s[0] : any) * 2};
+  cuuint32_t box[4] = {64, 128, 1, 1}, step[4] = {1, 1, 1, 1};
+  CUresult r = fn(map, dtype == FML_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, strides,
+                  box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  FML_REQUIRE(r == CUDA_SUCCESS, FML_CUDA_ERROR, "fml_attention_rules: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FML_OK;
+}
+
+using TcKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const RulesArgs);
+template <typename T, int DP> TcKernel tc_kernel(bool cap, bool bias) {
+  return cap ? bias ? attention_rules_tc_kernel<T, DP, true, true> : attention_rules_tc_kernel<T, DP, true, false>
+             : bias ? attention_rules_tc_kernel<T, DP, false, true> : attention_rules_tc_kernel<T, DP, false, false>;
+}
+
+}  // namespace
+
+// Large enough, and laid out for tensor maps: rows of 16-byte multiples, unit stride along the head, strides that do not run
+// backwards.
+bool attention_rules_tc_eligible(const RulesArgs &a, int dtype) {
+  if ((dtype != FML_F16 && dtype != FML_BF16) || a.D % 16 != 0 || !a.q_vec || !a.k_vec || !a.v_vec || a.Sk < 1 || a.Sk > kMaxTiles * kKeys) return false;
+  for (const int64_t *s : {a.q_s, a.k_s, a.v_s})
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0 || s[i] >= (1ll << 38) || (i == 2 && s[i] == 0)) return false;
+  return a.Sq >= 128 && a.Sk >= 128;
+}
+
+int launch_attention_rules_tc(const RulesArgs &a, int dtype, cudaStream_t s) {
+  CUtensorMap mq, mk, mv;
+  int st = rules_map(&mq, a.q, dtype, a.D, a.Sq, a.q_s, a.heads, a.batch);
+  if (st == FML_OK) st = rules_map(&mk, a.k, dtype, a.D, a.Sk, a.k_s, a.heads / a.group, a.batch);
+  if (st == FML_OK) st = rules_map(&mv, a.v, dtype, a.D, a.Sk, a.v_s, a.heads / a.group, a.batch);
+  if (st != FML_OK) return st;
+  const bool cap = a.cap.cap > 0.0f, bias = a.slopes != nullptr;
+  const int dp = a.D <= 64 ? 64 : 128;
+  const TcKernel kernel = dtype == FML_F16 ? (dp == 64 ? tc_kernel<__half, 64>(cap, bias) : tc_kernel<__half, 128>(cap, bias))
+                                           : (dp == 64 ? tc_kernel<__nv_bfloat16, 64>(cap, bias) : tc_kernel<__nv_bfloat16, 128>(cap, bias));
+  // 512 columns of tensor memory: a second CTA on the SM would wait for them, so the kernel asks for most of shared memory
+  const size_t smem = std::max<size_t>(dp == 64 ? TcShape<64>::kBytes : TcShape<128>::kBytes, 120 * 1024);
+  static bool attr_set[64][16] = {};
+  int dev = 0;
+  FML_CUDA(cudaGetDevice(&dev));
+  bool &set = attr_set[dev & 63][(dtype == FML_F16) * 8 + (dp == 64) * 4 + cap * 2 + bias];
+  if (!set) {
+    FML_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    set = true;
+  }
+  FML_CUDA(launch_kernel(kernel, dim3((unsigned)((a.Sq + 2 * kRows - 1) / (2 * kRows)), (unsigned)a.heads, (unsigned)a.batch), dim3(kThreads), smem, s,
+                         mq, mk, mv, a));
+  return FML_OK;
+}
+
+}  // namespace fml
