@@ -40,7 +40,12 @@ __global__ void __launch_bounds__(kThreads) attention_rules_kernel(const __grid_
   const TileRange range = tile_range(a, batch, row0, min(row0 + kRows, a.Sq));
   const int tiles = (range.last_key + S::kKeys - 1) / S::kKeys;
   for (int i = warp; i < min(tiles, kMaxTiles); i += kThreads / 32) {
-    const int view = tile_view(a, batch, range, i * S::kKeys, S::kKeys);
+    int view = tile_view(range, i * S::kKeys, S::kKeys);
+    if (a.k_documents.p && view != kTileNone) {
+      int64_t low, high;
+      tile_documents(a, batch, i * S::kKeys, min(i * S::kKeys + S::kKeys, a.Sk), &low, &high);
+      view = document_view(view, range, low, high);
+    }
     if (lane == 0) visible[i] = (uint8_t)view;
   }
   // a tile's rows from global memory, zeros for rows from `rows` on and features from D on

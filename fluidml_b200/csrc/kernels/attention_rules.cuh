@@ -52,8 +52,9 @@ __device__ __forceinline__ bool key_seen(const RulesArgs &a, const RowRules &r, 
   return key < r.last && (!a.q_documents.p || document == r.document);
 }
 
-// What the queries [row0, row1) of a tile see of a tile of keys: none, all of them every key, or some.
-enum TileView { kTileNone = 0, kTileSome = 1, kTileAll = 2 };
+// What the queries [row0, row1) of a tile see of a tile of keys: none, all of them every key, or some (kTileLast: those up to
+// the query's last, all of its document).
+enum TileView { kTileNone = 0, kTileSome = 1, kTileAll = 2, kTileLast = 3 };
 struct TileRange {
   int first_key, last_key;  // every query sees the keys below first_key, none those from last_key on (documents apart)
   int64_t low, high;        // the queries' smallest and largest document
@@ -81,22 +82,23 @@ __device__ __forceinline__ TileRange tile_range(const RulesArgs &a, int batch, i
   }
   return t;
 }
-__device__ __forceinline__ int tile_view(const RulesArgs &a, int batch, const TileRange &t, int key0, int keys) {
-  if (key0 >= t.last_key) return kTileNone;
-  bool all = key0 + keys <= t.first_key;
-  if (a.k_documents.p) {
-    int64_t low = INT64_MAX, high = INT64_MIN;
-    for (int i = key0 + (int)(threadIdx.x & 31); i < min(key0 + keys, t.last_key); i += 32) {
-      const int64_t x = document_at(a.k_documents, a.k_documents_row, batch, i);
-      low = min(low, x);
-      high = max(high, x);
-    }
-    low = warp_min(low);
-    high = ~warp_min(~high);
-    if (low > t.high || high < t.low) return kTileNone;
-    all = all && low == high && t.low == t.high;
+__device__ __forceinline__ int tile_view(const TileRange &t, int key0, int keys) {  // documents apart
+  return key0 >= t.last_key ? kTileNone : key0 + keys <= t.first_key ? kTileAll : kTileSome;
+}
+// The smallest and largest document of the keys [key0, key1), by a whole warp.
+__device__ __forceinline__ void tile_documents(const RulesArgs &a, int batch, int key0, int key1, int64_t *low, int64_t *high) {
+  int64_t l = INT64_MAX, h = INT64_MIN;
+  for (int i = key0 + (int)(threadIdx.x & 31); i < key1; i += 32) {
+    const int64_t x = document_at(a.k_documents, a.k_documents_row, batch, i);
+    l = min(l, x);
+    h = max(h, x);
   }
-  return all ? kTileAll : kTileSome;
+  *low = warp_min(l);
+  *high = ~warp_min(~h);
+}
+__device__ __forceinline__ int document_view(int view, const TileRange &t, int64_t low, int64_t high) {
+  if (view == kTileNone || low > t.high || high < t.low) return kTileNone;
+  return low == high && t.low == t.high ? (view == kTileAll ? kTileAll : kTileLast) : kTileSome;
 }
 
 // A row whose context came out as not finite: keys that it does not see may hold infinities or NaN, which weights of zero do

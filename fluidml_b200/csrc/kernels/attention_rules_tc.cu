@@ -4,12 +4,11 @@
 // contexts are accumulators in tensor memory (all 512 columns of it); weights go back over their scores, in the operands' type, as
 // the A operand of the second product.
 //
-//   warps 0-3, 4-7  softmax of tile A, B: thread = query = lane of tensor memory
-//   warp 8          loads (tensor maps, 128-byte swizzle): Q once, K and V tiles into two stages each
-//   (warps 10, 11    make up the third group of four, which gives its registers to the softmax groups: 128 scores of a row stay
-//                    in registers; 2 x 128 x 224 + 128 x 56 = 384 x 168, what the launch has)
-//   warp 9          products, in the order  S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j): while one tile's softmax runs, the tensor cores
-//                   work for the other
+//   warps 0-7, 8-15  softmax of tile A, B: thread = query = lane of tensor memory, and 64 of the 128 keys: two threads share a
+//                    query, and tell each other its largest score
+//   warp 16          loads (tensor maps, 128-byte swizzle): Q once, K and V tiles into two stages each
+//   warp 17          products, in the order  S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j): while one tile's softmax runs, the tensor cores
+//                    work for the other
 //
 // What bounds it.  A tile of 128 x 128 is 512 clocks of tensor core for either product at head size 128 (256 at 64) and 16384
 // exponentials at 16 a clock, 1024: per pair of products as much as they take at head size 128, twice as much at 64.  A capped
@@ -26,7 +25,7 @@
 namespace fml {
 namespace {
 
-constexpr int kThreads = 384, kRows = 128, kKeys = 128, kMaxTiles = 2048;
+constexpr int kThreads = 576, kRows = 128, kKeys = 128, kHalf = 64, kMaxTiles = 2048;
 constexpr uint32_t kColS = 0, kColO = 256;  // two of 128 columns each
 
 struct TcBarriers {  // offsets of 8 bytes
@@ -36,7 +35,7 @@ struct TcBarriers {  // offsets of 8 bytes
 template <int DP> struct TcShape {
   static constexpr int kTile = 128 * DP * 2;  // bytes of 128 rows
   static constexpr int kBoxes = DP / 64;      // of 64 features: 128 bytes, one swizzle row
-  static constexpr size_t kBytes = 6 * kTile + 8 * kKeys * 8 + kMaxTiles + TcBarriers::kCount * 8 + 16;
+  static constexpr size_t kBytes = 6 * kTile + 16 * kHalf * 8 + 8 * kRows * 4 + kMaxTiles + TcBarriers::kCount * 8 + 16 + 16 * 4;
 };
 
 __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float *v) {
@@ -94,14 +93,16 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   using S = TcShape<DP>;
   using B = TcBarriers;
   extern __shared__ __align__(1024) uint8_t smem[];
-  // [ Q of A | Q of B | K stage 0, 1 | V stage 0, 1 | documents of a tile, per softmax warp | views | barriers ]
+  // [ Q of A | Q of B | K stage 0, 1 | V stage 0, 1 | documents of a tile, per softmax warp | largest scores | views | barriers ]
   const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * S::kTile, v_s = k_s + 2 * S::kTile;
   int64_t *const documents = reinterpret_cast<int64_t *>(smem + 6 * S::kTile);
-  uint8_t *const views = reinterpret_cast<uint8_t *>(documents + 8 * kKeys);  // [tile]: view of A | view of B << 2
+  float *const largest = reinterpret_cast<float *>(documents + 16 * kHalf);  // [parity][tile A, B][half of the keys][row]
+  uint8_t *const views = reinterpret_cast<uint8_t *>(largest + 8 * kRows);   // [tile]: view of A | view of B << 2
   uint64_t *const bars = reinterpret_cast<uint64_t *>(views + kMaxTiles);
   const uint32_t bar = smem_u32(bars);
   uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(bars + B::kCount);
   volatile int *const abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  unsigned *const redo_rows = tmem_slot + 2;  // [softmax warp]: rows that are not finite
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const bool leader = elect_one();
   const int head = blockIdx.y, batch = blockIdx.z, kv = head / a.group;
@@ -112,11 +113,11 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     tma_prefetch_map(&map_q);
     tma_prefetch_map(&map_k);
     tma_prefetch_map(&map_v);
-    for (int i = 0; i < B::kCount; ++i) mbar_init(bar + 8u * i, i >= B::kP && i < B::kP + 2 ? 4 : 1);
+    for (int i = 0; i < B::kCount; ++i) mbar_init(bar + 8u * i, i >= B::kP && i < B::kP + 2 ? 8 : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 512);
+  if (warp == 17) tmem_alloc(smem_u32(tmem_slot), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -128,16 +129,23 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   const TileRange ra = tile_range(a, batch, row0, min(row0 + kRows, a.Sq));
   const TileRange rb = two ? tile_range(a, batch, row0 + kRows, min(row0 + 2 * kRows, a.Sq)) : ra;
   const int tiles = (max(ra.last_key, rb.last_key) + kKeys - 1) / kKeys;
-  for (int i = warp; i < tiles; i += kThreads / 32) {
-    const int va = tile_view(a, batch, ra, i * kKeys, kKeys), vb = two ? tile_view(a, batch, rb, i * kKeys, kKeys) : 0;
-    if (lane == 0) views[i] = (uint8_t)(va | vb << 2);
+  if (!a.k_documents.p) {
+    for (int i = threadIdx.x; i < tiles; i += kThreads)
+      views[i] = (uint8_t)(tile_view(ra, i * kKeys, kKeys) | (two ? tile_view(rb, i * kKeys, kKeys) << 2 : 0));
+  } else {
+#pragma unroll 4
+    for (int i = warp; i < tiles; i += kThreads / 32) {
+      int64_t low, high;
+      tile_documents(a, batch, i * kKeys, min(i * kKeys + kKeys, a.Sk), &low, &high);
+      if (lane == 0)
+        views[i] = (uint8_t)(document_view(tile_view(ra, i * kKeys, kKeys), ra, low, high) |
+                             (two ? document_view(tile_view(rb, i * kKeys, kKeys), rb, low, high) << 2 : 0));  // (kTileLast: no documents to compare)
+    }
   }
   __syncthreads();
 
   bool ok = true;
-  if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-  if (warp == 8) {
+  if (warp == 16) {
     // ------------------------------------------------------------ loads
     if (g_drop_loads != 1) {
       if (leader) {
@@ -176,7 +184,7 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         for (int j = max(0, n - 2); j < n; ++j) mbar_wait_warp(bar + 8u * (B::kVFull + (j & 1)), (uint32_t)(j >> 1) & 1u, &never);
       }
     }
-  } else if (warp == 9) {
+  } else if (warp == 17) {
     // ------------------------------------------------------------ products
     const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t idesc_s = instr_desc_16(type, kKeys, 0u), idesc_o = instr_desc_16(type, a.D, 1u);
@@ -204,7 +212,8 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       tc_fence_after();
       if (leader) {
         for (int k = 0; k < kKeys / 16; ++k)
-          umma_f16_ts(tmem + kColO + 128u * t, tmem + kColS + 128u * t + 8u * k, desc_v + (uint64_t)((stage * S::kTile + k * 2048) >> 4), idesc_o,
+          // (each half of the keys has its weights in its own scores' place)
+          umma_f16_ts(tmem + kColO + 128u * t, tmem + kColS + 128u * t + 64u * (k >> 2) + 8u * (k & 3), desc_v + (uint64_t)((stage * S::kTile + k * 2048) >> 4), idesc_o,
                       first_o[t] && k == 0 ? 0u : 1u);
       }
       __syncwarp();
@@ -249,142 +258,172 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     if (!ok) *abort_flag = 1;
     if (leader) umma_drain(bar + 8u * B::kDrain);
     __syncwarp();
-  }
   } else {
-    // ------------------------------------------------------------ softmax: thread = query
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int t = warp >> 2, local = threadIdx.x & 127;
+    // ------------------------------------------------------------ softmax: two threads = query
+    const int t = warp >> 3, half = warp >> 2 & 1, local = (warp & 3) * 32 + lane;
     const int i = row0 + t * kRows + local, row = min(i, a.Sq - 1);
-    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lane_addr + kColS + 128u * t, col_o = lane_addr + kColO + 128u * t;
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lane_addr + kColS + 128u * t + 64u * half,
+                   col_o = lane_addr + kColO + 128u * t;
     const RowRules r = row_rules(a, batch, head, row);
-    const bool whole_sign = !CAP && !BIAS && a.cap.scale > 0.0f;  // the largest product is the largest score
-    int64_t *const docs = documents + warp * kKeys;
+    int64_t *const docs = documents + warp * kHalf;
     float m = -INFINITY, l = 0.0f;
     uint32_t n = 0;
     if (t == 0 || two) {
-      for (int tile = 0; tile < tiles && ok; ++tile) {
+      // (a warp that gave up goes on through the barriers, so that none is left waiting)
+      for (int tile = 0; tile < tiles; ++tile) {
         const int view = views[tile] >> (2 * t) & 3;
         if (view == kTileNone) continue;
-        const int key0 = tile * kKeys;
-        if (view == kTileSome && a.k_documents.p) {  // (a copy per warp: a barrier among warps could be left by one that gave up)
+        const int key0 = tile * kKeys + half * kHalf;
+        if (ok && view == kTileSome && a.k_documents.p) {
           __syncwarp();
-          for (int j = lane; j < kKeys; j += 32)
+          for (int j = lane; j < kHalf; j += 32)
             docs[j] = key0 + j < a.Sk ? document_at(a.k_documents, a.k_documents_row, batch, key0 + j) : 0;
           __syncwarp();
         }
-        ok = mbar_wait_warp(bar + 8u * (B::kS + t), n & 1u, abort_flag);
-        if (!ok) break;
-        tc_fence_after();
-        float v[kKeys];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_start(col_s + 32u * c, v + 32 * c);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_tie(v + 32 * c);
-        // scores in units of ln 2 (without cap and bias they stay products, scaled on the way into the exponential)
-        if (CAP) {
-          const float2 f = both(a.cap.scale);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+        if (ok) ok = mbar_wait_warp(bar + 8u * (B::kS + t), n & 1u, abort_flag);
+        float v[kHalf];
+        float scale = 1.0f, m_tile = -INFINITY;
+        if (ok) {
+          tc_fence_after();
+          tmem_ld32_start(col_s, v);
+          tmem_ld32_start(col_s + 32u, v + 32);
+          tmem_ld_tie(v);
+          tmem_ld_tie(v + 32);
+          // scores in units of ln 2 (without cap and bias they stay products, scaled on the way into the exponential)
+          if (CAP) {
+            const float2 f = both(a.cap.scale);
             float far = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float2 x = mul2(make_float2(v[32 * c + j], v[32 * c + j + 1]), f);
-              v[32 * c + j] = x.x;
-              v[32 * c + j + 1] = x.y;
+            for (int j = 0; j < kHalf; j += 2) {
+              const float2 x = mul2(make_float2(v[j], v[j + 1]), f);
+              v[j] = x.x;
+              v[j + 1] = x.y;
               far = fmaxf(far, fmaxf(fabsf(x.x), fabsf(x.y)));
             }
             if (__all_sync(0xffffffffu, far <= 1.0f)) {
               // tanh(x) = x P(x^2) on [-1, 1]: least squares reweighted to the smallest largest error, 2.4e-7
 #pragma unroll
-              for (int j = 0; j < 32; j += 2) {
-                const float2 x = make_float2(v[32 * c + j], v[32 * c + j + 1]), u = mul2(x, x);
+              for (int j = 0; j < kHalf; j += 2) {
+                const float2 x = make_float2(v[j], v[j + 1]), u = mul2(x, x);
                 float2 p = fma2(u, both(-0.00283947f), both(0.01611418f));
                 p = fma2(u, p, both(-0.05097286f));
                 p = fma2(u, p, both(0.13253525f));
                 p = fma2(u, p, both(-0.33324004f));
                 p = fma2(u, p, both(0.99999685f));
-                p = mul2(mul2(p, x), both(a.cap.cap));
-                v[32 * c + j] = p.x;
-                v[32 * c + j + 1] = p.y;
+                p = mul2(p, x);
+                v[j] = p.x;
+                v[j + 1] = p.y;
               }
             } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[32 * c + j] = a.cap.cap * tanh_of<false>(v[32 * c + j]);
+              for (int j = 0; j < kHalf; ++j) v[j] = tanh_of<false>(v[j]);
             }
           }
-        } else if (BIAS || !whole_sign) {
+          scale = CAP ? a.cap.cap : a.cap.scale;
+          if (BIAS) {
+            const float at = (float)(r.at - key0);
+            // a tile that lies on one side of the query: |at - j| is a line
+            const bool before = r.at >= key0 + kHalf - 1;
+            if (__all_sync(0xffffffffu, before || r.at <= key0)) {
+              const float slope = before ? r.slope : -r.slope, start = -slope * at;
 #pragma unroll
-          for (int j = 0; j < kKeys; ++j) v[j] *= a.cap.scale;
-        }
-        if (BIAS) {
-          const float at = (float)(r.at - key0);
+              for (int j = 0; j < kHalf; j += 2) {
+                const float2 x = fma2(make_float2(v[j], v[j + 1]), both(scale), fma2(both(slope), make_float2((float)j, (float)(j + 1)), both(start)));
+                v[j] = x.x;
+                v[j + 1] = x.y;
+              }
+            } else {
 #pragma unroll
-          for (int j = 0; j < kKeys; ++j) v[j] = fmaf(-r.slope, fabsf(at - (float)j), v[j]);
-        }
-        if (view == kTileSome) {
-          const int last = r.last - key0;
-          if (a.k_documents.p) {
+              for (int j = 0; j < kHalf; ++j) v[j] = fmaf(-r.slope, fabsf(at - (float)j), v[j] * scale);
+            }
+            scale = 1.0f;
+          } else if (!(scale > 0.0f)) {  // (a negative divisor: the largest score is the smallest product)
 #pragma unroll
-            for (int j = 0; j < kKeys; ++j)
-              if (j >= last || docs[j] != r.document) v[j] = -INFINITY;
-          } else {
-#pragma unroll
-            for (int j = 0; j < kKeys; ++j)
-              if (j >= last) v[j] = -INFINITY;
+            for (int j = 0; j < kHalf; ++j) v[j] *= scale;
+            scale = 1.0f;
           }
-        }
-        float m_tile = v[0];
+          if (view != kTileAll) {
+            const int last = r.last - key0;
+            if (view == kTileSome && a.k_documents.p) {
 #pragma unroll
-        for (int j = 1; j < kKeys; ++j) m_tile = fmaxf(m_tile, v[j]);
-        const float scale = !CAP && !BIAS && whole_sign ? a.cap.scale : 1.0f;
-        m_tile *= scale;
-        if (n == 0) {
-          m = m_tile;
-        } else if (__any_sync(0xffffffffu, m_tile > m + 8.0f)) {
-          const float m_new = fmaxf(m, m_tile), f = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
-          l *= f;
-          m = m_new;
-          for (int c = 0; c < DP; c += 32) {
-            float o[32];
-            tmem_ld32_start(col_o + (uint32_t)c, o);
-            tmem_ld_tie(o);
+              for (int j = 0; j < kHalf; ++j)
+                if (j >= last || docs[j] != r.document) v[j] = -INFINITY;
+            } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] *= f;
-            tmem_st32(col_o + (uint32_t)c, reinterpret_cast<const uint32_t *>(o));
+              for (int j = 0; j < kHalf; ++j)
+                if (j >= last) v[j] = -INFINITY;
+            }
           }
+          float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int j = 4; j < kHalf - 4; j += 8) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], fmaxf(v[j + c], v[j + 4 + c]));
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) top[c] = fmaxf(top[c], v[kHalf - 4 + c]);
+          m_tile = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+        }
+        // the query's largest score of the tile, from both halves
+        float *const exchange = largest + ((n & 1u) * 2 + t) * 2 * kRows + local;
+        exchange[half * kRows] = m_tile;
+        named_barrier_sync(1 + t, 256);
+        if (ok) {
+          m_tile = fmaxf(m_tile, exchange[(half ^ 1) * kRows]);
+          if (n == 0) {
+            m = m_tile;
+          } else if (__any_sync(0xffffffffu, m_tile > m + 8.0f)) {
+            const float m_new = fmaxf(m, m_tile), f = m_new == -INFINITY ? 1.0f : ex2_approx(m - m_new);
+            l *= f;
+            m = m_new;
+#pragma unroll 1
+            for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 16) {
+              uint32_t o[16];
+              tmem_ld16(col_o + (uint32_t)c, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st16(col_o + (uint32_t)c, o);
+            }
+          }
+          const float2 base = both(m == -INFINITY ? 0.0f : -m), s2 = both(scale);
+          float2 sum[2] = {both(0.0f), both(0.0f)};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t p[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 x = fma2(make_float2(v[32 * c + 2 * j], v[32 * c + 2 * j + 1]), s2, base);
+              const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+              sum[j & 1] = add2(sum[j & 1], e);
+              p[j] = pack2<T>(e.x, e.y);
+            }
+            tmem_st16(col_s + 16u * c, p);
+          }
+          const float2 all = add2(sum[0], sum[1]);
+          l += all.x + all.y;
           tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar + 8u * (B::kP + t));
+        } else {
+          *abort_flag = 1;
         }
-        const float2 base = both(m == -INFINITY ? 0.0f : -m), s2 = both(scale);
-        float2 sum = both(0.0f);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t p[32];
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 x = fma2(make_float2(v[64 * c + 2 * j], v[64 * c + 2 * j + 1]), s2, base);
-            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            sum = add2(sum, e);
-            p[j] = pack2<T>(e.x, e.y);
-          }
-          tmem_st32(col_s + 32u * c, p);
-        }
-        l += sum.x + sum.y;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar + 8u * (B::kP + t));
         ++n;
       }
-      // ---- out = O / l
+      // ---- out = O / l, half of the features each
+      float *const exchange = largest + ((n & 1u) * 2 + t) * 2 * kRows + local;
+      exchange[half * kRows] = l;
+      named_barrier_sync(1 + t, 256);
+      l += exchange[(half ^ 1) * kRows];
       if (ok) ok = mbar_wait_warp(bar + 8u * B::kDone, 0u, abort_flag);
+      bool bad = false;
       if (ok) {
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros; NaN stays)
         T *const dst = static_cast<T *>(a.out) + batch * a.o_s[0] + head * a.o_s[1] + (int64_t)row * a.o_s[2];
         const bool wide = a.o_s[3] == 1 && a.o_s[2] % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-        bool bad = false;
 #pragma unroll
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
           if (c >= a.D) break;
           float o[32];
           if (n > 0) {
@@ -411,13 +450,15 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             }
           }
         }
-        unsigned redo = __ballot_sync(0xffffffffu, bad && i < a.Sq);
-        __syncwarp();
-        while (redo) {
-          const int which = __ffs(redo) - 1;
-          redo &= redo - 1;
-          redo_rules_row<T>(a, batch, head, row0 + t * kRows + (warp & 3) * 32 + which);
-        }
+      }
+      const unsigned mine = __ballot_sync(0xffffffffu, bad && i < a.Sq);
+      if (lane == 0) redo_rows[warp] = mine;
+      named_barrier_sync(1 + t, 256);  // (both halves of a row are written before it is done again)
+      unsigned redo = half == 0 ? redo_rows[warp] | redo_rows[warp + 4] : 0u;
+      while (redo) {
+        const int which = __ffs(redo) - 1;
+        redo &= redo - 1;
+        redo_rules_row<T>(a, batch, head, row0 + t * kRows + (warp & 3) * 32 + which);
       }
     }
   }
@@ -427,7 +468,7 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
