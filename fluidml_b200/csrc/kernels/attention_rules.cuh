@@ -16,6 +16,7 @@ struct RulesArgs {
   int batch, heads, group, Sq, Sk, D, causal;
   Cap cap;
   int q_vec, k_vec, v_vec;  // rows take 16-byte accesses
+  int o_tma;                // the result leaves by tensor map (attention_rules_tc.cu)
   int *status;
 };
 

@@ -20,6 +20,7 @@
 #include "attention_rules.cuh"
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <type_traits>
 
 namespace fml {
@@ -35,7 +36,7 @@ struct TcBarriers {  // offsets of 8 bytes
 template <int DP> struct TcShape {
   static constexpr int kTile = 128 * DP * 2;  // bytes of 128 rows
   static constexpr int kBoxes = DP / 64;      // of 64 features: 128 bytes, one swizzle row
-  static constexpr size_t kBytes = 6 * kTile + 16 * kHalf * 8 + 8 * kRows * 4 + kMaxTiles + TcBarriers::kCount * 8 + 16 + 16 * 4;
+  static constexpr size_t kBytes = 6 * kTile + 16 * kHalf * 4 + 8 * kRows * 4 + kMaxTiles + TcBarriers::kCount * 8 + 16 + 16 * 4;
 };
 
 __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float *v) {
@@ -86,16 +87,24 @@ __device__ __forceinline__ uint32_t instr_desc_16(uint32_t type, int n, uint32_t
   return (1u << 4) | (type << 7) | (type << 10) | (b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 
+// x - base, cut to +-INT_MAX (where it no longer says which).
+__device__ __forceinline__ int near_difference(int64_t x, int64_t base) {
+  const int64_t d = (int64_t)((uint64_t)x - (uint64_t)base);
+  const bool wraps = (x < base) != (d < 0);  // (further apart than 64 bits hold)
+  if (wraps) return x < base ? -INT_MAX : INT_MAX;
+  return d >= INT_MAX ? INT_MAX : d <= -INT_MAX ? -INT_MAX : (int)d;
+}
+
 template <typename T, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 1)
 attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ RulesArgs a) {
+                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o, const __grid_constant__ RulesArgs a) {
   using S = TcShape<DP>;
   using B = TcBarriers;
   extern __shared__ __align__(1024) uint8_t smem[];
   // [ Q of A | Q of B | K stage 0, 1 | V stage 0, 1 | documents of a tile, per softmax warp | largest scores | views | barriers ]
   const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * S::kTile, v_s = k_s + 2 * S::kTile;
-  int64_t *const documents = reinterpret_cast<int64_t *>(smem + 6 * S::kTile);
+  int *const documents = reinterpret_cast<int *>(smem + 6 * S::kTile);
   float *const largest = reinterpret_cast<float *>(documents + 16 * kHalf);  // [parity][tile A, B][half of the keys][row]
   uint8_t *const views = reinterpret_cast<uint8_t *>(largest + 8 * kRows);   // [tile]: view of A | view of B << 2
   uint64_t *const bars = reinterpret_cast<uint64_t *>(views + kMaxTiles);
@@ -133,13 +142,37 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     for (int i = threadIdx.x; i < tiles; i += kThreads)
       views[i] = (uint8_t)(tile_view(ra, i * kKeys, kKeys) | (two ? tile_view(rb, i * kKeys, kKeys) << 2 : 0));
   } else {
-#pragma unroll 4
-    for (int i = warp; i < tiles; i += kThreads / 32) {
-      int64_t low, high;
-      tile_documents(a, batch, i * kKeys, min(i * kKeys + kKeys, a.Sk), &low, &high);
-      if (lane == 0)
-        views[i] = (uint8_t)(document_view(tile_view(ra, i * kKeys, kKeys), ra, low, high) |
-                             (two ? document_view(tile_view(rb, i * kKeys, kKeys), rb, low, high) << 2 : 0));  // (kTileLast: no documents to compare)
+    constexpr int kWarps = kThreads / 32, kAtOnce = 4;  // (tiles of a warp whose loads are in flight together)
+    for (int i0 = warp; i0 < tiles; i0 += kWarps * kAtOnce) {
+      int64_t low[kAtOnce], high[kAtOnce];
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        low[k] = INT64_MAX;
+        high[k] = INT64_MIN;
+      }
+      auto scan = [&](auto *p) {  // (one width at a time: a choice at every load would put them one after another)
+        p += batch * a.k_documents_row;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k)
+#pragma unroll
+          for (int j = 0; j < kKeys / 32; ++j) {
+            const int key = (i0 + k * kWarps) * kKeys + 32 * j + lane;
+            const int64_t x = p[min(key, a.Sk - 1) * a.k_documents.stride];
+            low[k] = min(low[k], key < a.Sk ? x : INT64_MAX);
+            high[k] = max(high[k], key < a.Sk ? x : INT64_MIN);
+          }
+      };
+      if (a.k_documents.wide) scan(static_cast<const int64_t *>(a.k_documents.p));
+      else scan(static_cast<const int32_t *>(a.k_documents.p));
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int i = i0 + k * kWarps;
+        if (i >= tiles) break;
+        const int64_t l = warp_min(low[k]), h = ~warp_min(~high[k]);
+        if (lane == 0)
+          views[i] = (uint8_t)(document_view(tile_view(ra, i * kKeys, kKeys), ra, l, h) |
+                               (two ? document_view(tile_view(rb, i * kKeys, kKeys), rb, l, h) << 2 : 0));
+      }
     }
   }
   __syncthreads();
@@ -195,11 +228,12 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     bool first_o[2] = {true, true};
     auto scores = [&](int t, uint32_t stage) {
       if (leader) {
-        for (int k = 0; k < steps; ++k) {
+        const uint64_t dq = desc_q + (uint64_t)(t * S::kTile >> 4), dk = desc_k + (uint64_t)(stage * S::kTile >> 4);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
           // 32 bytes of a swizzle row per step; four steps to a box
           const uint64_t off = (uint64_t)((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-          umma_f16_ss(tmem + kColS + 128u * t, desc_q + (uint64_t)(t * S::kTile >> 4) + off, desc_k + (uint64_t)(stage * S::kTile >> 4) + off, idesc_s,
-                      k ? 1u : 0u);
+          if (k < steps) umma_f16_ss(tmem + kColS + 128u * t, dq + off, dk + off, idesc_s, k ? 1u : 0u);
         }
         umma_commit(bar + 8u * (B::kS + t));
       }
@@ -211,9 +245,11 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       ++done[t];
       tc_fence_after();
       if (leader) {
+        const uint64_t dv = desc_v + (uint64_t)(stage * S::kTile >> 4);
+#pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)
           // (each half of the keys has its weights in its own scores' place)
-          umma_f16_ts(tmem + kColO + 128u * t, tmem + kColS + 128u * t + 64u * (k >> 2) + 8u * (k & 3), desc_v + (uint64_t)((stage * S::kTile + k * 2048) >> 4), idesc_o,
+          umma_f16_ts(tmem + kColO + 128u * t, tmem + kColS + 128u * t + 64u * (k >> 2) + 8u * (k & 3), dv + (uint64_t)(k * 2048 >> 4), idesc_o,
                       first_o[t] && k == 0 ? 0u : 1u);
       }
       __syncwarp();
@@ -265,7 +301,12 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lane_addr + kColS + 128u * t + 64u * half,
                    col_o = lane_addr + kColO + 128u * t;
     const RowRules r = row_rules(a, batch, head, row);
-    int64_t *const docs = documents + warp * kHalf;
+    // documents go by their differences from the warp's first, which fit 32 bits unless they are cut (then the keys' own are asked)
+    int *const docs = documents + warp * kHalf;
+    RowRules r0 = r;
+    r0.document = __shfl_sync(0xffffffffu, (long long)r.document, 0);
+    const int r_near = near_difference(r.document, r0.document);
+    const bool far_documents = __any_sync(0xffffffffu, r_near == INT_MAX || r_near == -INT_MAX);
     float m = -INFINITY, l = 0.0f;
     uint32_t n = 0;
     if (t == 0 || two) {
@@ -276,8 +317,10 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         const int key0 = tile * kKeys + half * kHalf;
         if (ok && view == kTileSome && a.k_documents.p) {
           __syncwarp();
-          for (int j = lane; j < kHalf; j += 32)
-            docs[j] = key0 + j < a.Sk ? document_at(a.k_documents, a.k_documents_row, batch, key0 + j) : 0;
+          for (int j = lane; j < kHalf; j += 32) {
+            const int64_t x = key0 + j < a.Sk ? document_at(a.k_documents, a.k_documents_row, batch, key0 + j) : r0.document;
+            docs[j] = near_difference(x, r0.document);
+          }
           __syncwarp();
         }
         if (ok) ok = mbar_wait_warp(bar + 8u * (B::kS + t), n & 1u, abort_flag);
@@ -325,12 +368,18 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             // a tile that lies on one side of the query: |at - j| is a line
             const bool before = r.at >= key0 + kHalf - 1;
             if (__all_sync(0xffffffffu, before || r.at <= key0)) {
+              // (stepped by eight keys in four chains: pairs of constants would cost two moves each)
               const float slope = before ? r.slope : -r.slope, start = -slope * at;
+              const float2 step = both(8.0f * slope);
+              float2 bias[4];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) bias[c] = make_float2(fmaf(slope, (float)(2 * c), start), fmaf(slope, (float)(2 * c + 1), start));
 #pragma unroll
               for (int j = 0; j < kHalf; j += 2) {
-                const float2 x = fma2(make_float2(v[j], v[j + 1]), both(scale), fma2(both(slope), make_float2((float)j, (float)(j + 1)), both(start)));
+                const float2 x = fma2(make_float2(v[j], v[j + 1]), both(scale), bias[(j >> 1) & 3]);
                 v[j] = x.x;
                 v[j + 1] = x.y;
+                bias[(j >> 1) & 3] = add2(bias[(j >> 1) & 3], step);
               }
             } else {
 #pragma unroll
@@ -346,8 +395,18 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             const int last = r.last - key0;
             if (view == kTileSome && a.k_documents.p) {
 #pragma unroll
-              for (int j = 0; j < kHalf; ++j)
-                if (j >= last || docs[j] != r.document) v[j] = -INFINITY;
+              for (int j = 0; j < kHalf; j += 4) {
+                const int4 d = *reinterpret_cast<const int4 *>(docs + j);
+                if (j >= last || d.x != r_near) v[j] = -INFINITY;
+                if (j + 1 >= last || d.y != r_near) v[j + 1] = -INFINITY;
+                if (j + 2 >= last || d.z != r_near) v[j + 2] = -INFINITY;
+                if (j + 3 >= last || d.w != r_near) v[j + 3] = -INFINITY;
+              }
+              if (far_documents) {
+#pragma unroll
+                for (int j = 0; j < kHalf; ++j)
+                  if (key0 + j < a.Sk && document_at(a.k_documents, a.k_documents_row, batch, key0 + j) != r.document) v[j] = -INFINITY;
+              }
             } else {
 #pragma unroll
               for (int j = 0; j < kHalf; ++j)
@@ -421,10 +480,10 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         tc_fence_after();
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros; NaN stays)
         T *const dst = static_cast<T *>(a.out) + batch * a.o_s[0] + head * a.o_s[1] + (int64_t)row * a.o_s[2];
-        const bool wide = a.o_s[3] == 1 && a.o_s[2] % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+        uint8_t *const staged = smem + t * S::kTile;  // (its queries are done with)
 #pragma unroll
-        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
-          if (c >= a.D) break;
+        for (int c0 = 0; c0 < DP / 2; c0 += 32) {
+          const int c = half * (DP / 2) + c0;
           float o[32];
           if (n > 0) {
             __syncwarp();
@@ -438,22 +497,38 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             bad = bad || (c + j < a.D && !(fabsf(x0) <= FLT_MAX && fabsf(x1) <= FLT_MAX));
             x[j / 2] = pack2<T>(x0, x1);
           }
-          if (i < a.Sq) {
-            if (wide) {
+          if (a.o_tma) {
 #pragma unroll
-              for (int j = 0; j < 16; j += 4)
-                if (c + 2 * j < a.D) *reinterpret_cast<uint4 *>(dst + c + 2 * j) = make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (c + j < a.D) dst[(int64_t)(c + j) * a.o_s[3]] = reinterpret_cast<const T *>(x)[j];
+            for (int j = 0; j < 16; j += 4) {
+              const int chunk = (c + 2 * j) >> 3;  // of 8 features; eight to a box's row, permuted as the map's swizzle does
+              *reinterpret_cast<uint4 *>(staged + (chunk >> 3) * 16384 + local * 128 + (((chunk & 7) ^ (local & 7)) << 4)) =
+                  make_uint4(x[j], x[j + 1], x[j + 2], x[j + 3]);
             }
+          } else if (i < a.Sq) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < a.D) dst[(int64_t)(c + j) * a.o_s[3]] = reinterpret_cast<const T *>(x)[j];
           }
         }
+        if (a.o_tma) fence_async_smem();
       }
       const unsigned mine = __ballot_sync(0xffffffffu, bad && i < a.Sq);
       if (lane == 0) redo_rows[warp] = mine;
-      named_barrier_sync(1 + t, 256);  // (both halves of a row are written before it is done again)
+      named_barrier_sync(1 + t, 256);
+      unsigned any = 0u;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) any |= redo_rows[8 * t + w];
+      if (ok && a.o_tma && (warp & 7) == 0 && leader) {
+        for (int b = 0; b < S::kBoxes; ++b)
+          if (64 * b < a.D)
+            asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+                         ::"l"(&map_o), "r"(q_s + (uint32_t)(t * S::kTile + b * 16384)), "r"(64 * b), "r"(row0 + t * kRows), "r"(head), "r"(batch)
+                         : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        if (any) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      }
+      if (any) named_barrier_sync(1 + t, 256);  // (both halves of a row are written before it is done again)
       unsigned redo = half == 0 ? redo_rows[warp] | redo_rows[warp + 4] : 0u;
       while (redo) {
         const int which = __ffs(redo) - 1;
@@ -490,7 +565,7 @@ int rules_map(CUtensorMap *map, const void *base, int dtype, int64_t d, int64_t 
   return FML_OK;
 }
 
-using TcKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const RulesArgs);
+using TcKernel = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const CUtensorMap, const RulesArgs);
 template <typename T, int DP> TcKernel tc_kernel(bool cap, bool bias) {
   return cap ? bias ? attention_rules_tc_kernel<T, DP, true, true> : attention_rules_tc_kernel<T, DP, true, false>
              : bias ? attention_rules_tc_kernel<T, DP, false, true> : attention_rules_tc_kernel<T, DP, false, false>;
@@ -508,11 +583,21 @@ bool attention_rules_tc_eligible(const RulesArgs &a, int dtype) {
   return a.Sq >= 128 && a.Sk >= 128;
 }
 
-int launch_attention_rules_tc(const RulesArgs &a, int dtype, cudaStream_t s) {
-  CUtensorMap mq, mk, mv;
+int launch_attention_rules_tc(const RulesArgs &args, int dtype, cudaStream_t s) {
+  RulesArgs a = args;
+  CUtensorMap mq, mk, mv, mo;
   int st = rules_map(&mq, a.q, dtype, a.D, a.Sq, a.q_s, a.heads, a.batch);
   if (st == FML_OK) st = rules_map(&mk, a.k, dtype, a.D, a.Sk, a.k_s, a.heads / a.group, a.batch);
   if (st == FML_OK) st = rules_map(&mv, a.v, dtype, a.D, a.Sk, a.v_s, a.heads / a.group, a.batch);
+  // the result leaves through shared memory and a tensor map where its layout allows (a thread's own row, 16 bytes at a time to
+  // 32 rows per instruction, cost 9000 clocks of a CTA)
+  a.o_tma = a.o_s[3] == 1 && aligned16(a.out);
+  for (int i = 0; i < 3; ++i) {
+    const int64_t n = i == 0 ? a.batch : i == 1 ? a.heads : a.Sq;
+    a.o_tma = a.o_tma && (n == 1 || (a.o_s[i] > 0 && a.o_s[i] < (1ll << 38) && a.o_s[i] % 8 == 0));
+  }
+  mo = mq;
+  if (st == FML_OK && a.o_tma) st = rules_map(&mo, a.out, dtype, a.D, a.Sq, a.o_s, a.heads, a.batch);
   if (st != FML_OK) return st;
   const bool cap = a.cap.cap > 0.0f, bias = a.slopes != nullptr;
   const int dp = a.D <= 64 ? 64 : 128;
@@ -529,7 +614,7 @@ int launch_attention_rules_tc(const RulesArgs &a, int dtype, cudaStream_t s) {
     set = true;
   }
   FML_CUDA(launch_kernel(kernel, dim3((unsigned)((a.Sq + 2 * kRows - 1) / (2 * kRows)), (unsigned)a.heads, (unsigned)a.batch), dim3(kThreads), smem, s,
-                         mq, mk, mv, a));
+                         mq, mk, mv, mo, a));
   return FML_OK;
 }
 
