@@ -7,8 +7,10 @@
 //   warps 0-7, 8-15  softmax of tile A, B: thread = query = lane of tensor memory, and 64 of the 128 keys: two threads share a
 //                    query, and tell each other its largest score
 //   warp 16          loads (tensor maps, 128-byte swizzle): Q once, K and V tiles into two stages each
-//   warp 17          products, in the order  S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j): while one tile's softmax runs, the tensor cores
+//   warp 17          products, in the order  S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j)  (weights apart, see TcShape: S_A(j)  PV_B(j-2)
 //                    work for the other
+//   (warps 18, 19    make up the last group of four, which gives registers to the softmax: 512 x 104 + 128 x 64 = 640 x 96, what the
+//                    launch has)
 //
 // What bounds it.  A tile of 128 x 128 is 512 clocks of tensor core for either product at head size 128 (256 at 64) and 16384
 // exponentials at 16 a clock, 1024: per pair of products as much as they take at head size 128, twice as much at 64.  A capped
@@ -16,7 +18,8 @@
 //
 // The running maximum follows only when a tile's exceeds it by more than 8 (in units of ln 2): weights then reach 2^8, which the
 // sums carry, and the context's correction, a round trip through registers, is rare.  The commit that publishes S(j) also covers
-// PV(j - 1), issued before it, so the correction needs no barrier of its own.
+// PV(j - 1), issued before it, so that the correction needs no barrier of its own (weights apart: PV(j - 2), and PV(j - 1) has one,
+// whose phase is then either that product's or just over).
 #include "attention_rules.cuh"
 #include <algorithm>
 #include <cfloat>
@@ -26,17 +29,22 @@
 namespace fml {
 namespace {
 
-constexpr int kThreads = 576, kRows = 128, kKeys = 128, kHalf = 64, kMaxTiles = 2048;
-constexpr uint32_t kColS = 0, kColO = 256;  // two of 128 columns each
+constexpr int kThreads = 640, kRows = 128, kKeys = 128, kHalf = 64, kMaxTiles = 2048;
+constexpr uint32_t kColS = 0, kColO = 256;  // columns of tensor memory
 
 struct TcBarriers {  // offsets of 8 bytes
-  enum { kQ = 0, kKFull = 2, kKEmpty = 4, kVFull = 6, kVEmpty = 8, kS = 10, kP = 12, kDone = 14, kDrain = 15, kCount = 16 };
+  enum { kQ = 0, kKFull = 2, kKEmpty = 6, kVFull = 10, kVEmpty = 14, kS = 18, kSFree = 20, kP = 22, kPV = 24, kDone = 26, kDrain = 27, kCount = 28 };
 };
 
 template <int DP> struct TcShape {
   static constexpr int kTile = 128 * DP * 2;  // bytes of 128 rows
   static constexpr int kBoxes = DP / 64;      // of 64 features: 128 bytes, one swizzle row
-  static constexpr size_t kBytes = 6 * kTile + 16 * kHalf * 4 + 8 * kRows * 4 + kMaxTiles + TcBarriers::kCount * 8 + 16 + 16 * 4;
+  // Head sizes up to 64 leave room in tensor memory for weights beside the scores: the next tile's scores are then computed as
+  // soon as the softmax has read these.
+  static constexpr bool kApart = DP == 64;
+  static constexpr uint32_t kStepO = kApart ? 64 : 128, kColP = kApart ? 384 : kColS, kStepP = kApart ? 64 : 128, kHalfP = kApart ? 32 : 64;
+  static constexpr int kStages = kApart ? 4 : 2;
+  static constexpr size_t kBytes = (2 + 2 * kStages) * kTile + 16 * kHalf * 4 + 8 * kRows * 4 + kMaxTiles + TcBarriers::kCount * 8 + 16 + 16 * 4;
 };
 
 __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float *v) {
@@ -80,6 +88,20 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// The tiles of keys that a role works on, in order: f(tile, its views) for tiles whose views have a bit of `mask`, until f says
+// false.  By whole warps: 32 tiles are looked at together (one by one, those that a late document skips took thousands of clocks).
+template <typename F> __device__ __forceinline__ void each_tile(const uint8_t *views, int tiles, int mask, F f) {
+  for (int first = 0; first < tiles; first += 32) {
+    const int i = first + (int)(threadIdx.x & 31);
+    const int mine = i < tiles ? views[i] : 0;
+    unsigned left = __ballot_sync(0xffffffffu, (mine & mask) != 0);
+    while (left) {
+      const int j = __ffs(left) - 1;
+      left &= left - 1;
+      if (!f(first + j, __shfl_sync(0xffffffffu, mine, j))) return;
+    }
+  }
+}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Instruction descriptor of kind::f16 with fp32 sums: type 0 fp16, 1 bf16; M = 128; B along its columns (1) or along k (0).
@@ -102,9 +124,9 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   using S = TcShape<DP>;
   using B = TcBarriers;
   extern __shared__ __align__(1024) uint8_t smem[];
-  // [ Q of A | Q of B | K stage 0, 1 | V stage 0, 1 | documents of a tile, per softmax warp | largest scores | views | barriers ]
-  const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * S::kTile, v_s = k_s + 2 * S::kTile;
-  int *const documents = reinterpret_cast<int *>(smem + 6 * S::kTile);
+  // [ Q of A | Q of B | K stages | V stages | documents of a tile, per softmax warp | largest scores | views | barriers ]
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + 2 * S::kTile, v_s = k_s + S::kStages * S::kTile;
+  int *const documents = reinterpret_cast<int *>(smem + (2 + 2 * S::kStages) * S::kTile);
   float *const largest = reinterpret_cast<float *>(documents + 16 * kHalf);  // [parity][tile A, B][half of the keys][row]
   uint8_t *const views = reinterpret_cast<uint8_t *>(largest + 8 * kRows);   // [tile]: view of A | view of B << 2
   uint64_t *const bars = reinterpret_cast<uint64_t *>(views + kMaxTiles);
@@ -122,7 +144,7 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     tma_prefetch_map(&map_q);
     tma_prefetch_map(&map_k);
     tma_prefetch_map(&map_v);
-    for (int i = 0; i < B::kCount; ++i) mbar_init(bar + 8u * i, i >= B::kP && i < B::kP + 2 ? 8 : 1);
+    for (int i = 0; i < B::kCount; ++i) mbar_init(bar + 8u * i, (i >= B::kP && i < B::kP + 2) || (i >= B::kSFree && i < B::kSFree + 2) ? 8 : 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -134,67 +156,108 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
   pdl_launch_dependents();  // (only now: tensor memory)
   pdl_wait();
 
+  if (warp == 16 && leader && g_drop_loads != 1) {
+    for (int t = 0; t < (two ? 2 : 1); ++t) {
+      mbar_expect_tx(bar + 8u * (B::kQ + t), S::kTile);
+      for (int i = 0; i < S::kBoxes; ++i)
+        tma_load_4d(q_s + (uint32_t)(t * S::kTile + i * 16384), &map_q, bar + 8u * (B::kQ + t), 64 * i, row0 + t * kRows, a.q_s[1] ? head : 0,
+                    a.q_s[0] ? batch : 0);
+    }
+  }
+  __syncwarp();
   // ---- what the two tiles see of each tile of keys
-  const TileRange ra = tile_range(a, batch, row0, min(row0 + kRows, a.Sq));
-  const TileRange rb = two ? tile_range(a, batch, row0 + kRows, min(row0 + 2 * kRows, a.Sq)) : ra;
+  TileRange ra, rb;
+  const int a1 = min(row0 + kRows, a.Sq), b0 = two ? a1 : row0, b1 = two ? min(row0 + 2 * kRows, a.Sq) : a1;
+  ra.first_key = last_key_of(a, batch, row0);
+  ra.last_key = last_key_of(a, batch, a1 - 1);
+  rb.first_key = last_key_of(a, batch, b0);
+  rb.last_key = last_key_of(a, batch, b1 - 1);
   const int tiles = (max(ra.last_key, rb.last_key) + kKeys - 1) / kKeys;
+  const bool narrow = !a.q_documents.wide && !a.k_documents.wide;
   if (!a.k_documents.p) {
     for (int i = threadIdx.x; i < tiles; i += kThreads)
       views[i] = (uint8_t)(tile_view(ra, i * kKeys, kKeys) | (two ? tile_view(rb, i * kKeys, kKeys) << 2 : 0));
   } else {
-    constexpr int kWarps = kThreads / 32, kAtOnce = 4;  // (tiles of a warp whose loads are in flight together)
-    for (int i0 = warp; i0 < tiles; i0 += kWarps * kAtOnce) {
-      int64_t low[kAtOnce], high[kAtOnce];
+    // Documents in 32 bits: as they are, or as differences from the first query's.  All of a warp's loads are in flight together (its four tiles of
+    // keys, and the queries), and one width at a time: a choice at every load would put them one after another.
+    constexpr int kWarps = kThreads / 32, kAtOnce = 4, kPer = kKeys / 32;
+    const int64_t base = narrow ? 0 : document_at(a.q_documents, a.q_documents_row, batch, row0);
+    int q_low[2], q_high[2];
+    auto scan = [&](auto *qp, auto *kp) {
+      using Wide = decltype(*qp + *kp);  // (int for two narrow ones)
+      auto cut = [&](Wide x) { return sizeof(Wide) == 4 ? (int)x : near_difference(x, base); };
+      qp += batch * a.q_documents_row;
+      kp += batch * a.k_documents_row;
+      Wide x[2 * kPer];
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        low[k] = INT64_MAX;
-        high[k] = INT64_MIN;
-      }
-      auto scan = [&](auto *p) {  // (one width at a time: a choice at every load would put them one after another)
-        p += batch * a.k_documents_row;
+      for (int j = 0; j < 2 * kPer; ++j) x[j] = qp[(j < kPer ? min(row0 + 32 * j + lane, a1 - 1) : min(b0 + 32 * (j - kPer) + lane, b1 - 1)) * a.q_documents.stride];
+#pragma unroll 1
+      for (int i0 = warp; i0 < tiles || i0 == warp; i0 += kWarps * kAtOnce) {
+        Wide y[kAtOnce][kPer];
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k)
 #pragma unroll
-          for (int j = 0; j < kKeys / 32; ++j) {
-            const int key = (i0 + k * kWarps) * kKeys + 32 * j + lane;
-            const int64_t x = p[min(key, a.Sk - 1) * a.k_documents.stride];
-            low[k] = min(low[k], key < a.Sk ? x : INT64_MAX);
-            high[k] = max(high[k], key < a.Sk ? x : INT64_MIN);
-          }
-      };
-      if (a.k_documents.wide) scan(static_cast<const int64_t *>(a.k_documents.p));
-      else scan(static_cast<const int32_t *>(a.k_documents.p));
+          for (int j = 0; j < kPer; ++j) y[k][j] = a.Sk > 0 ? kp[min((i0 + k * kWarps) * kKeys + 32 * j + lane, a.Sk - 1) * a.k_documents.stride] : 0;
+        if (i0 == warp) {
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const int i = i0 + k * kWarps;
-        if (i >= tiles) break;
-        const int64_t l = warp_min(low[k]), h = ~warp_min(~high[k]);
-        if (lane == 0)
-          views[i] = (uint8_t)(document_view(tile_view(ra, i * kKeys, kKeys), ra, l, h) |
-                               (two ? document_view(tile_view(rb, i * kKeys, kKeys), rb, l, h) << 2 : 0));
+          for (int t = 0; t < 2; ++t) {
+            int low = INT_MAX, high = INT_MIN;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+              const int d = cut(x[t * kPer + j]);
+              low = min(low, d);
+              high = max(high, d);
+            }
+            q_low[t] = __reduce_min_sync(0xffffffffu, low);
+            q_high[t] = __reduce_max_sync(0xffffffffu, high);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+          const int i = i0 + k * kWarps;
+          int low = INT_MAX, high = INT_MIN;
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) {
+            const int d = cut(y[k][j]);
+            low = min(low, d);
+            high = max(high, d);
+          }
+          low = __reduce_min_sync(0xffffffffu, low);
+          high = __reduce_max_sync(0xffffffffu, high);
+          auto view_of = [&](const TileRange &r, int t) {
+            const int view = tile_view(r, i * kKeys, kKeys);
+            if (view == kTileNone || low > q_high[t] || high < q_low[t]) return (int)kTileNone;
+            // one document, and not one that the difference was cut at
+            const bool same = low == high && q_low[t] == q_high[t] && (narrow || (low != INT_MAX && low != -INT_MAX));
+            return !same ? (int)kTileSome : view == kTileAll ? (int)kTileAll : (int)kTileLast;
+          };
+          if (lane == 0 && i < tiles) views[i] = (uint8_t)(view_of(ra, 0) | (two ? view_of(rb, 1) << 2 : 0));
+        }
       }
+    };
+    if (a.q_documents.wide && a.k_documents.wide) {
+      scan(static_cast<const int64_t *>(a.q_documents.p), static_cast<const int64_t *>(a.k_documents.p));
+    } else if (a.k_documents.wide) {
+      scan(static_cast<const int32_t *>(a.q_documents.p), static_cast<const int64_t *>(a.k_documents.p));
+    } else if (a.q_documents.wide) {
+      scan(static_cast<const int64_t *>(a.q_documents.p), static_cast<const int32_t *>(a.k_documents.p));
+    } else {
+      scan(static_cast<const int32_t *>(a.q_documents.p), static_cast<const int32_t *>(a.k_documents.p));
     }
   }
   __syncthreads();
 
   bool ok = true;
+  if (warp >= 16) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 16) {
     // ------------------------------------------------------------ loads
     if (g_drop_loads != 1) {
-      if (leader) {
-        for (int t = 0; t < (two ? 2 : 1); ++t) {
-          mbar_expect_tx(bar + 8u * (B::kQ + t), S::kTile);
-          for (int i = 0; i < S::kBoxes; ++i)
-            tma_load_4d(q_s + (uint32_t)(t * S::kTile + i * 16384), &map_q, bar + 8u * (B::kQ + t), 64 * i, row0 + t * kRows, a.q_s[1] ? head : 0,
-                        a.q_s[0] ? batch : 0);
-        }
-      }
       int n = 0, n_k = 0;
-      for (int i = 0; i < tiles && ok; ++i) {
-        if (!views[i]) continue;
-        const uint32_t s = (uint32_t)n & 1u, free_parity = ((uint32_t)(n >> 1) & 1u) ^ 1u;
+      each_tile(views, tiles, 15, [&](int i, int) {
+        const uint32_t s = (uint32_t)n % S::kStages, free_parity = ((uint32_t)(n / S::kStages) & 1u) ^ 1u;
         ok = mbar_wait_warp(bar + 8u * (B::kKEmpty + s), free_parity, abort_flag);
-        if (!ok) break;
+        if (!ok) return false;
         if (leader) {
           mbar_expect_tx(bar + 8u * (B::kKFull + s), S::kTile);
           for (int b = 0; b < S::kBoxes; ++b)
@@ -202,19 +265,22 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
         ++n_k;
         ok = mbar_wait_warp(bar + 8u * (B::kVEmpty + s), free_parity, abort_flag);
-        if (!ok) break;
+        if (!ok) return false;
         if (leader) {
           mbar_expect_tx(bar + 8u * (B::kVFull + s), S::kTile);
           for (int b = 0; b < S::kBoxes; ++b)
             tma_load_4d(v_s + s * S::kTile + b * 16384, &map_v, bar + 8u * (B::kVFull + s), 64 * b, i * kKeys, a.v_s[1] ? kv : 0, a.v_s[0] ? batch : 0);
         }
         ++n;
-      }
+        return true;
+      });
       if (!ok) {  // bounded wait for the loads in flight
         volatile int never = 0;
         for (int t = 0; t < (two ? 2 : 1); ++t) mbar_wait_warp(bar + 8u * (B::kQ + t), 0u, &never);
-        for (int j = max(0, n_k - 2); j < n_k; ++j) mbar_wait_warp(bar + 8u * (B::kKFull + (j & 1)), (uint32_t)(j >> 1) & 1u, &never);
-        for (int j = max(0, n - 2); j < n; ++j) mbar_wait_warp(bar + 8u * (B::kVFull + (j & 1)), (uint32_t)(j >> 1) & 1u, &never);
+        for (int j = max(0, n_k - S::kStages); j < n_k; ++j)
+          mbar_wait_warp(bar + 8u * (B::kKFull + j % S::kStages), (uint32_t)(j / S::kStages) & 1u, &never);
+        for (int j = max(0, n - S::kStages); j < n; ++j)
+          mbar_wait_warp(bar + 8u * (B::kVFull + j % S::kStages), (uint32_t)(j / S::kStages) & 1u, &never);
       }
     }
   } else if (warp == 17) {
@@ -223,10 +289,14 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t idesc_s = instr_desc_16(type, kKeys, 0u), idesc_o = instr_desc_16(type, a.D, 1u);
     const uint64_t desc_q = smem_desc(q_s, 16u, 1024u), desc_k = smem_desc(k_s, 16u, 1024u), desc_v = smem_desc(v_s, 16384u, 1024u);
     const int steps = a.D / 16;
-    uint32_t n = 0, done[2] = {0u, 0u}, last_stage = 0;  // tiles of keys; weights taken per query tile; B's last tile
-    bool pending = false;                                 // B's product with V of the tile before
-    bool first_o[2] = {true, true};
+    uint32_t done[2] = {0u, 0u}, given[2] = {0u, 0u};  // of each query tile: second products, first products
     auto scores = [&](int t, uint32_t stage) {
+      if (S::kApart && given[t] > 0) {
+        ok = mbar_wait_warp(bar + 8u * (B::kSFree + t), (given[t] - 1u) & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+      }
+      ++given[t];
       if (leader) {
         const uint64_t dq = desc_q + (uint64_t)(t * S::kTile >> 4), dk = desc_k + (uint64_t)(stage * S::kTile >> 4);
 #pragma unroll
@@ -239,87 +309,103 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       }
       __syncwarp();
     };
-    auto context = [&](int t, uint32_t stage) {
-      ok = mbar_wait_warp(bar + 8u * (B::kP + t), done[t] & 1u, abort_flag);
+    // tile number n (of those that either sees); last: nobody needs its values any more
+    auto context = [&](int t, uint32_t n, bool last) {
+      const uint32_t stage = n % S::kStages;
+      ok = mbar_wait_warp(bar + 8u * (B::kVFull + stage), n / S::kStages & 1u, abort_flag) &&
+           mbar_wait_warp(bar + 8u * (B::kP + t), done[t] & 1u, abort_flag);
       if (!ok) return;
-      ++done[t];
       tc_fence_after();
       if (leader) {
         const uint64_t dv = desc_v + (uint64_t)(stage * S::kTile >> 4);
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          // (each half of the keys has its weights in its own scores' place)
-          umma_f16_ts(tmem + kColO + 128u * t, tmem + kColS + 128u * t + 64u * (k >> 2) + 8u * (k & 3), dv + (uint64_t)(k * 2048 >> 4), idesc_o,
-                      first_o[t] && k == 0 ? 0u : 1u);
+        for (int k = 0; k < kKeys / 16; ++k)  // (each half of the keys has its weights in a place of its own)
+          umma_f16_ts(tmem + kColO + S::kStepO * t, tmem + S::kColP + S::kStepP * t + S::kHalfP * (k >> 2) + 8u * (k & 3), dv + (uint64_t)(k * 2048 >> 4),
+                      idesc_o, done[t] == 0 && k == 0 ? 0u : 1u);
+        if (S::kApart) umma_commit(bar + 8u * (B::kPV + t));
+        if (last) umma_commit(bar + 8u * (B::kVEmpty + stage));
       }
       __syncwarp();
-      first_o[t] = false;
-    };
-    auto release_v = [&](uint32_t stage) {
-      if (leader) umma_commit(bar + 8u * (B::kVEmpty + stage));
-      __syncwarp();
+      ++done[t];
     };
     ok = mbar_wait_warp(bar + 8u * B::kQ, 0u, abort_flag) && (!two || mbar_wait_warp(bar + 8u * (B::kQ + 1), 0u, abort_flag));
-    for (int i = 0; i < tiles && ok; ++i) {
-      const int view = views[i];
-      if (!view) continue;
-      const uint32_t stage = n & 1u, parity = (n >> 1) & 1u;
-      ok = mbar_wait_warp(bar + 8u * (B::kKFull + stage), parity, abort_flag);
-      if (!ok) break;
+    // second products that are to come: of A at most one, of B two with weights apart, else one
+    uint32_t n = 0, wait_a = 0, wait_b[2] = {0u, 0u};
+    bool has_a = false, last_a = false;
+    int has_b = 0;
+    auto next_b = [&]() {
+      context(1, wait_b[0], true);
+      wait_b[0] = wait_b[1];
+      --has_b;
+    };
+    if (ok) each_tile(views, tiles, 15, [&](int, int view) {
+      const uint32_t stage = n % S::kStages;
+      ok = mbar_wait_warp(bar + 8u * (B::kKFull + stage), n / S::kStages & 1u, abort_flag);
+      if (!ok) return false;
       tc_fence_after();
       if (view & 3) scores(0, stage);
-      if (pending) {
-        context(1, last_stage);
-        if (!ok) break;
-        release_v(last_stage);
-        pending = false;
-      }
+      if (ok && has_b == (S::kApart ? 2 : 1)) next_b();
+      if (!ok) return false;
       if (view >> 2) scores(1, stage);
+      if (!ok) return false;
       if (leader) umma_commit(bar + 8u * (B::kKEmpty + stage));
       __syncwarp();
-      ok = mbar_wait_warp(bar + 8u * (B::kVFull + stage), parity, abort_flag);
-      if (!ok) break;
-      if (view & 3) context(0, stage);
-      if (!ok) break;
+      if (has_a) {
+        context(0, wait_a, last_a);
+        has_a = false;
+        if (!ok) return false;
+      }
+      if (view & 3) {
+        if (S::kApart) {
+          has_a = true;
+          wait_a = n;
+          last_a = !(view >> 2);
+        } else {
+          context(0, n, !(view >> 2));
+        }
+      }
       if (view >> 2) {
-        pending = true;
-        last_stage = stage;
-      } else {
-        release_v(stage);
+        if (has_b) wait_b[1] = n; else wait_b[0] = n;
+        ++has_b;
       }
       ++n;
-    }
-    if (ok && pending) context(1, last_stage);
+      return true;
+    });
+    if (ok && has_b == 2) next_b();
+    if (ok && has_a) context(0, wait_a, last_a);
+    if (ok && has_b) next_b();
     if (ok && leader) umma_commit(bar + 8u * B::kDone);
     if (!ok) *abort_flag = 1;
     if (leader) umma_drain(bar + 8u * B::kDrain);
     __syncwarp();
+  }
   } else {
     // ------------------------------------------------------------ softmax: two threads = query
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     const int t = warp >> 3, half = warp >> 2 & 1, local = (warp & 3) * 32 + lane;
     const int i = row0 + t * kRows + local, row = min(i, a.Sq - 1);
     const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), col_s = lane_addr + kColS + 128u * t + 64u * half,
-                   col_o = lane_addr + kColO + 128u * t;
+                   col_p = S::kApart ? lane_addr + S::kColP + S::kStepP * t + S::kHalfP * half : col_s, col_o = lane_addr + kColO + S::kStepO * t;
     const RowRules r = row_rules(a, batch, head, row);
-    // documents go by their differences from the warp's first, which fit 32 bits unless they are cut (then the keys' own are asked)
+    // wide documents go by their differences from the warp's first, which fit 32 bits unless they are cut (then the keys' own are
+    // asked)
     int *const docs = documents + warp * kHalf;
     RowRules r0 = r;
     r0.document = __shfl_sync(0xffffffffu, (long long)r.document, 0);
-    const int r_near = near_difference(r.document, r0.document);
-    const bool far_documents = __any_sync(0xffffffffu, r_near == INT_MAX || r_near == -INT_MAX);
+    const int r_near = narrow ? (int)r.document : near_difference(r.document, r0.document);
+    const bool far_documents = __any_sync(0xffffffffu, !narrow && (r_near == INT_MAX || r_near == -INT_MAX));
     float m = -INFINITY, l = 0.0f;
     uint32_t n = 0;
     if (t == 0 || two) {
       // (a warp that gave up goes on through the barriers, so that none is left waiting)
-      for (int tile = 0; tile < tiles; ++tile) {
-        const int view = views[tile] >> (2 * t) & 3;
-        if (view == kTileNone) continue;
+      each_tile(views, tiles, 3 << (2 * t), [&](int tile, int both_views) {
+        const int view = both_views >> (2 * t) & 3;
         const int key0 = tile * kKeys + half * kHalf;
         if (ok && view == kTileSome && a.k_documents.p) {
           __syncwarp();
           for (int j = lane; j < kHalf; j += 32) {
             const int64_t x = key0 + j < a.Sk ? document_at(a.k_documents, a.k_documents_row, batch, key0 + j) : r0.document;
-            docs[j] = near_difference(x, r0.document);
+            docs[j] = narrow ? (int)x : near_difference(x, r0.document);
           }
           __syncwarp();
         }
@@ -332,6 +418,11 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           tmem_ld32_start(col_s + 32u, v + 32);
           tmem_ld_tie(v);
           tmem_ld_tie(v + 32);
+          if (S::kApart) {  // the next scores may come
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar + 8u * (B::kSFree + t));
+          }
           // scores in units of ln 2 (without cap and bias they stay products, scaled on the way into the exponential)
           if (CAP) {
             const float2 f = both(a.cap.scale);
@@ -427,7 +518,10 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         float *const exchange = largest + ((n & 1u) * 2 + t) * 2 * kRows + local;
         exchange[half * kRows] = m_tile;
         named_barrier_sync(1 + t, 256);
+        // (with weights apart the last product may still read the weights, and add to the context)
+        if (S::kApart && n > 0 && ok) ok = mbar_wait_warp(bar + 8u * (B::kPV + t), (n - 1u) & 1u, abort_flag);
         if (ok) {
+          if (S::kApart) tc_fence_after();
           m_tile = fmaxf(m_tile, exchange[(half ^ 1) * kRows]);
           if (n == 0) {
             m = m_tile;
@@ -456,7 +550,7 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               sum[j & 1] = add2(sum[j & 1], e);
               p[j] = pack2<T>(e.x, e.y);
             }
-            tmem_st16(col_s + 16u * c, p);
+            tmem_st16(col_p + 16u * c, p);
           }
           const float2 all = add2(sum[0], sum[1]);
           l += all.x + all.y;
@@ -468,7 +562,8 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           *abort_flag = 1;
         }
         ++n;
-      }
+        return true;
+      });
       // ---- out = O / l, half of the features each
       float *const exchange = largest + ((n & 1u) * 2 + t) * 2 * kRows + local;
       exchange[half * kRows] = l;
@@ -478,7 +573,7 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
       bool bad = false;
       if (ok) {
         tc_fence_after();
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros; NaN stays)
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (no key seen: zeros; a NaN of keys not seen is done again below)
         T *const dst = static_cast<T *>(a.out) + batch * a.o_s[0] + head * a.o_s[1] + (int64_t)row * a.o_s[2];
         uint8_t *const staged = smem + t * S::kTile;  // (its queries are done with)
 #pragma unroll
@@ -489,14 +584,20 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             __syncwarp();
             tmem_ld32_start(col_o + (uint32_t)c, o);
             tmem_ld_tie(o);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = 0.0f;
           }
-          uint32_t x[16];
+          uint32_t x[16] = {};
+          float2 check = both(0.0f);  // 0, or NaN from an infinity or NaN on
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float x0 = l == 0.0f ? 0.0f : o[j] * inv, x1 = l == 0.0f ? 0.0f : o[j + 1] * inv;
-            bad = bad || (c + j < a.D && !(fabsf(x0) <= FLT_MAX && fabsf(x1) <= FLT_MAX));
-            x[j / 2] = pack2<T>(x0, x1);
+            const float2 y = mul2(make_float2(o[j], o[j + 1]), both(inv));
+            if (j % 16 == 0 && c + j >= a.D) break;  // (columns that the products do not write)
+            check = fma2(y, both(0.0f), check);
+            x[j / 2] = pack2<T>(y.x, y.y);
           }
+          bad = bad || !(check.x + check.y == 0.0f);
           if (a.o_tma) {
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
