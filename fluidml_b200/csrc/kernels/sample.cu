@@ -6,7 +6,8 @@
 //   1  largest logit
 //   2  counts in bins linear in (largest - logit) / temperature: the logits of a vocabulary spread over all of them, where the
 //      leading bits of their encoding would put most into a dozen and serialise the atomics
-//   3  top-k: the bin that holds the k-th token, as a range of keys (integers in the order of the logits), is binned by key
+//   3  top-k: where the bins up to the k-th token hold few tokens (1024), these go to one CTA, which sorts them, cuts and draws.
+//      Else the bin that holds the k-th token, as a range of keys (integers in the order of the logits), is binned by key
 //      until a bin is one key; of equal logits the lowest indexes are kept
 //   4  top-p: the counts bound every bin's weight, which leaves a few bins for the cut; one pass sums the weights of all
 //      tokens and of those above these bins exactly and bins the rest by key, as in 3, with weights in place of counts
@@ -26,7 +27,8 @@ namespace fml {
 namespace {
 
 using u64 = unsigned long long;
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 1024, kMaxCluster = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 1024, kPer = kBins / kThreads, kMaxCluster = 8;
+constexpr int kList = 1024;  // candidates that one CTA sorts
 constexpr double kOne = 17592186044416.0;  // 2^44: the weight of the largest logit
 constexpr float kSpan = 32.0f;             // the bins reach e^-32, below which every weight is a unit
 
@@ -43,21 +45,30 @@ struct SampleArgs {
 };
 
 struct Shared {
-  u64 hist[kBins], merged[kBins];
+  u64 hist[kBins], merged[kBins];  // (one of them also the list of candidates)
   uint32_t counts[kBins];
-  u64 part[kWarps];
+  double part[2 * kWarps];         // u64 or double
+  u64 sums[2][kMaxCluster];        // of every CTA
   u64 exchange[2][kMaxCluster];
   u64 found[4];
-  double top;
+  int listed;
 };
 
-// Integers in the order of the logits; both zeros are one.
-__device__ __forceinline__ uint32_t key_of(float z) {
+// Integers in the order of the logits, without the bits that the type does not have; both zeros are one.
+template <typename T> struct Key;
+template <> struct Key<float> { static constexpr int kDrop = 0; };
+template <> struct Key<__half> { static constexpr int kDrop = 13; };
+template <> struct Key<__nv_bfloat16> { static constexpr int kDrop = 16; };
+template <typename T> __device__ __forceinline__ uint32_t key_of(float z) {
   const uint32_t u = __float_as_uint(z + 0.0f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return (u & 0x80000000u ? ~u : u | 0x80000000u) >> Key<T>::kDrop;
 }
-__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-constexpr uint32_t kNone = 0x007fffffu;  // key of -infinity: nothing to draw
+template <typename T> __device__ __forceinline__ float value_of(uint32_t k) {
+  k <<= Key<T>::kDrop;
+  // (a negative number's dropped bits are ones in its key)
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~(k | ((1u << Key<T>::kDrop) - 1u)));
+}
+template <typename T> constexpr uint32_t kNone = 0x007fffffu >> Key<T>::kDrop;  // key of -infinity: nothing to draw
 
 // 2^x for -1100 < x <= 0: the fraction's Taylor series (terms ln(2)^n / n!) to the 11th power, 6e-15 on half a unit.
 __device__ __forceinline__ double exp2_64(double x) {
@@ -117,109 +128,158 @@ template <typename T> struct Sampler {
       for (int j = 0; j < V; ++j) f(to_f32(x[j]), base + i + j);
     }
   }
+  __device__ __forceinline__ u64 *part() { return reinterpret_cast<u64 *>(sh->part); }
   __device__ __forceinline__ u64 warp_sum(u64 v) const {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
   }
-  // Every CTA's `mine` (of its first thread) to all CTAs: exchange[phase][rank]; ends with a cluster barrier.
+  // Sum over the CTA.
+  __device__ u64 block_sum(u64 v) {
+    v = warp_sum(v);
+    __syncthreads();
+    if (lane == 0) part()[warp] = v;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) all += part()[w];
+    return all;
+  }
+  // Every CTA's `mine` (of its first threads) to all CTAs: exchange[phase][rank]; ends with a cluster barrier.
   __device__ __forceinline__ const u64 *to_all(u64 mine) {
     phase ^= 1;
     if (threadIdx.x < ranks) *cluster.map_shared_rank(&sh->exchange[phase][rank], threadIdx.x) = mine;
     cluster.sync();
     return sh->exchange[phase];
   }
-  // Sum over the cluster of the threads' values (MAX: the largest).
-  template <bool MAX> __device__ u64 reduce(u64 v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
-      v = MAX ? max(v, w) : v + w;
-    }
-    __syncthreads();
-    if (lane == 0) sh->part[warp] = v;
+  __device__ uint32_t largest(uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (lane == 0) part()[warp] = v;
     __syncthreads();
     u64 all = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) all = MAX ? max(all, sh->part[w]) : all + sh->part[w];
+    for (int w = 0; w < kWarps; ++w) all = max(all, part()[w]);
     const u64 *x = to_all(all);
     all = 0;
-    for (int i = 0; i < ranks; ++i) all = MAX ? max(all, x[i]) : all + x[i];
-    return all;
+    for (int i = 0; i < ranks; ++i) all = max(all, x[i]);
+    return (uint32_t)all;
   }
   __device__ void clear() {
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh->hist[i] = 0;
     __syncthreads();
   }
-  // hist of all CTAs, added up, into every CTA's merged.
-  __device__ void merge() {
+  // hist of all CTAs, added up, into every CTA's merged; the CTAs' two sums into every CTA's sums.  Each CTA adds up its share of
+  // the bins.
+  __device__ void merge(u64 s0 = 0, u64 s1 = 0) {
+    if (threadIdx.x < ranks) {
+      *cluster.map_shared_rank(&sh->sums[0][rank], threadIdx.x) = s0;
+      *cluster.map_shared_rank(&sh->sums[1][rank], threadIdx.x) = s1;
+    }
     cluster.sync();
     const int share = kBins / ranks;
     for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += kThreads) {
       u64 sum = 0;
-      for (int c = 0; c < ranks; ++c) sum += *cluster.map_shared_rank(&sh->hist[i], c);
-      for (int c = 0; c < ranks; ++c) *cluster.map_shared_rank(&sh->merged[i], c) = sum;
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < ranks) sum += *cluster.map_shared_rank(&sh->hist[i], c);
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c)
+        if (c < ranks) *cluster.map_shared_rank(&sh->merged[i], c) = sum;
     }
     cluster.sync();
   }
-  // The first bin b of values(b) whose running sum, from `above` on, has reached(sum): found[0] = b, found[1] = the sum before it,
-  // the last bin if none has.  Two neighbouring bins per thread.
-  template <typename U, typename G, typename R> __device__ void first_bin(U above, G values, R reached, int *bin, U *before) {
-    const U a = values(2 * threadIdx.x), b = values(2 * threadIdx.x + 1);
-    U run = a + b;
+  __device__ __forceinline__ u64 sum_of(int which) const {
+    u64 s = 0;
+    for (int c = 0; c < ranks; ++c) s += sh->sums[which][c];
+    return s;
+  }
+  // v: a thread's total -> what the threads before it have (N totals at once); all: the CTA's.
+  template <typename U, int N> __device__ __forceinline__ void before(const U (&v)[N], U (&start)[N], U (&all)[N]) {
+    U run[N];
+    U *p = reinterpret_cast<U *>(sh->part);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const U up = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += up;
+    for (int n = 0; n < N; ++n) {
+      run[n] = v[n];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const U up = __shfl_up_sync(0xffffffffu, run[n], o);
+        if (lane >= o) run[n] += up;
+      }
     }
-    U *part = reinterpret_cast<U *>(sh->part);
-    U *found = reinterpret_cast<U *>(sh->found);
     __syncthreads();
-    if (lane == 31) part[warp] = run;
-    if (threadIdx.x == 0) *reinterpret_cast<volatile int *>(sh->found + 2) = kBins;
+    if (lane == 31)
+#pragma unroll
+      for (int n = 0; n < N; ++n) p[n * kWarps + warp] = run[n];
     __syncthreads();
-    U start = above;
-    for (int w = 0; w < warp; ++w) start += part[w];
-    start += run - a - b;
-    // (sums of non-negative numbers: once reached, always; only the first says so and its predecessor does not)
-    int *at = reinterpret_cast<int *>(sh->found + 2);
-    const bool r0 = reached(start + a), r1 = reached(start + a + b);
-    if (r0) atomicMin(at, 2 * (int)threadIdx.x);
-    else if (r1) atomicMin(at, 2 * (int)threadIdx.x + 1);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      U s = 0, t = 0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) s = t;
+        t += p[n * kWarps + w];
+      }
+      start[n] = s + run[n] - v[n];
+      all[n] = t;
+    }
+  }
+  // The first bin whose running sum, from `above` on, has reached(sum), and the sum before it; the last bin if none has.
+  template <typename R> __device__ void first_bin(u64 above, R reached, int *bin, u64 *sum_before) {
+    u64 v[kPer], own[1] = {0}, start[1], all[1];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) own[0] += v[i] = sh->merged[kPer * threadIdx.x + i];
+    if (threadIdx.x == 0) sh->found[0] = kBins - 1;
+    before<u64, 1>(own, start, all);
+    u64 run = above + start[0];
+    if (threadIdx.x == kThreads - 1 && !reached(run + own[0])) sh->found[1] = run + own[0] - v[kPer - 1];
+    if (!reached(run) && reached(run + own[0])) {  // (sums of non-negative numbers: one thread; its first bin that reaches)
+      int i = 0;
+      while (i < kPer - 1 && !reached(run + v[i])) run += v[i++];
+      sh->found[0] = kPer * threadIdx.x + i;
+      sh->found[1] = run;
+    } else if (threadIdx.x == 0 && reached(above)) {
+      sh->found[0] = 0;
+      sh->found[1] = above;
+    }
     __syncthreads();
-    const int got = min(*at, kBins - 1);
-    if (got == 2 * (int)threadIdx.x) found[0] = start;
-    if (got == 2 * (int)threadIdx.x + 1) found[0] = start + a;
-    __syncthreads();
-    *bin = got;
-    *before = found[0];
+    *bin = (int)sh->found[0];
+    *sum_before = sh->found[1];
     __syncthreads();
   }
-  // The keys of bins [b1, b2]: bin_of is monotone, so they are an interval, whose ends two searches find.
-  __device__ __forceinline__ void keys_of(const Row &r, int b1, int b2, uint32_t *lo, uint32_t *hi) const {
-    uint32_t l = kNone + 1, h = key_of(r.topf);  // smallest key of a bin up to b2
+  // The keys of bins [b1, b2]: bin_of is monotone, so they are an interval.  A warp asks 32 keys at a time for either end.
+  __device__ void keys_of(const Row &r, int b1, int b2, uint32_t *lo, uint32_t *hi) const {
+    const uint32_t top = key_of<T>(r.topf);
+    uint32_t l = kNone<T> + 1, h = top;  // the smallest key of a bin up to b2 is in [l, h]
     while (l < h) {
-      const uint32_t m = l + (h - l) / 2;
-      if (bin_of(r, value_of(m)) <= b2) h = m; else l = m + 1;
+      const uint32_t step = (h - l) / 33 + 1, m = min(l + (lane + 1) * step - 1, h);
+      const unsigned yes = __ballot_sync(0xffffffffu, bin_of(r, value_of<T>(m)) <= b2);
+      const int k = yes ? __ffs(yes) - 1 : 32;  // the first that is
+      const uint32_t was = l;
+      if (k > 0) l = min(was + (uint32_t)k * step, h);
+      if (k < 32) h = min(was + (uint32_t)(k + 1) * step - 1, h);
     }
     *lo = l;
-    l = *lo; h = key_of(r.topf);  // largest key of a bin from b1 on
+    h = top;  // the largest key of a bin from b1 on is in [l, h]
     while (l < h) {
-      const uint32_t m = l + (h - l + 1) / 2;
-      if (bin_of(r, value_of(m)) >= b1) l = m; else h = m - 1;
+      const uint32_t step = (h - l) / 33 + 1, m = min(l + (lane + 1) * step, h);
+      const unsigned yes = __ballot_sync(0xffffffffu, bin_of(r, value_of<T>(m)) >= b1);
+      const int k = __popc(yes);  // the first k are
+      const uint32_t was = l;
+      if (k > 0) l = min(was + (uint32_t)k * step, h);
+      if (k < 32) h = min(was + (uint32_t)(k + 1) * step - 1, h);
     }
     *hi = l;
   }
   // Narrows the range of keys [lo, hi], above which lies `above` of the measure, to the one key at which the running sum has
   // reached(sum).  first: the histogram of the range is merged already (by (hi - key) >> shift_of).
   template <typename M, typename R>
-  __device__ void narrow(uint32_t lo, uint32_t hi, u64 above, bool first, M measure, R reached, uint32_t *key, u64 *before, u64 *ties) {
+  __device__ void narrow(uint32_t lo, uint32_t hi, u64 above, bool first, M measure, R reached, uint32_t *key, u64 *sum_before, u64 *ties) {
     for (;;) {
       const int shift = shift_of(lo, hi);
       if (!first) {
         clear();
         each([&](float z, int i) {
-          const uint32_t k = key_of(z);
+          const uint32_t k = key_of<T>(z);
           if (k >= lo && k <= hi) {
             const u64 m = measure(z, k, i);
             if (m) atomicAdd(&sh->hist[(hi - k) >> shift], m);
@@ -229,11 +289,11 @@ template <typename T> struct Sampler {
       }
       first = false;
       int b;
-      first_bin<u64>(above, [&](int i) { return sh->merged[i]; }, reached, &b, &above);
+      first_bin(above, reached, &b, &above);
       const u64 inside = sh->merged[b];
       hi = hi - min((uint32_t)b << shift, hi - lo);
       if (shift == 0) {
-        *key = hi; *before = above; *ties = inside;
+        *key = hi; *sum_before = above; *ties = inside;
         return;
       }
       lo = max(lo, hi - min(hi, (1u << shift) - 1u));
@@ -244,15 +304,16 @@ template <typename T> struct Sampler {
   // The first index, in the vocabulary's order, at which the running sum of measure(z, key, index) has reached(sum); -1: none.
   template <typename M, typename R> __device__ int locate(M measure, R reached, u64 *total) {
     u64 mine = 0;
-    each([&](float z, int i) { mine += measure(z, key_of(z), i); });
+    each([&](float z, int i) { mine += measure(z, key_of<T>(z), i); });
     mine = warp_sum(mine);
     __syncthreads();
-    if (lane == 0) sh->part[warp] = mine;
+    if (lane == 0) part()[warp] = mine;
+    if (threadIdx.x == 0) sh->found[3] = ~0ull;
     __syncthreads();
     u64 start = 0, all = 0;
     for (int w = 0; w < kWarps; ++w) {
       if (w == warp) start = all;
-      all += sh->part[w];
+      all += part()[w];
     }
     const u64 *x = to_all(all);
     u64 sum = 0;
@@ -261,8 +322,6 @@ template <typename T> struct Sampler {
       sum += x[c];
     }
     *total = sum;
-    if (threadIdx.x == 0) sh->found[3] = ~0ull;
-    cluster.sync();
     if (!reached(start, sum) && reached(start + mine, sum)) {  // (one warp of the cluster)
       bool done = false;
       for (int i = warp * seg + lane * V; i < (warp + 1) * seg && !done; i += 32 * V) {
@@ -272,7 +331,7 @@ template <typename T> struct Sampler {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const float z = to_f32(v[j]);
-          m[j] = measure(z, key_of(z), base + i + j);
+          m[j] = measure(z, key_of<T>(z), base + i + j);
           own += m[j];
         }
         u64 run = own;
@@ -299,7 +358,86 @@ template <typename T> struct Sampler {
     const u64 got = sh->found[3];
     return got == ~0ull ? -1 : (int)got;
   }
+  // Sorts n <= kList numbers of the CTA, the rest of the next power of two filled up with the largest number.
+  __device__ void sort(u64 *list, int n) {
+    int size = 32;
+    while (size < n) size <<= 1;
+    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = ~0ull;
+    __syncthreads();
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j; j >>= 1) {
+        for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const u64 x = list[a], y = list[b];
+          if ((x > y) == ((a & k) == 0)) { list[a] = y; list[b] = x; }
+        }
+        __syncthreads();
+      }
+  }
 };
+
+// Top-k of at most kList candidates, gathered in one CTA: sorted, cut, and drawn there.
+template <typename T>
+__device__ int draw_listed(Sampler<T> &s, const Row &r, int n, int k, float p, float u, double *probability) {
+  u64 *const list = s.sh->hist, *const weights = s.sh->merged;
+  s.sort(list, n);  // by falling key, then index
+  n = min(n, k);
+  // a thread has kPer neighbours of the order
+  u64 w[kPer], own[1] = {0}, start[1], all[1];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = kPer * threadIdx.x + i;
+    w[i] = at < n ? weight_of(r, value_of<T>(~(uint32_t)(list[at] >> 32))) : 0ull;
+    own[0] += w[i];
+  }
+  s.template before<u64, 1>(own, start, all);
+  const double want = (double)fmaxf(p, 0.0f) * (double)all[0];
+  u64 run = start[0];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = kPer * threadIdx.x + i;
+    const u64 sum_before = run;
+    run += w[i];
+    const bool kept = at < n && (!(p < 1.0f) || at == 0 || (double)sum_before < want) &&
+                      exponent_of(r, value_of<T>(~(uint32_t)(list[at] >> 32))) >= r.least;
+    if (!kept) w[i] = 0;
+  }
+  __syncthreads();
+  // back to the vocabulary's order: index above, place below
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = kPer * threadIdx.x + i;
+    if (at < n) {
+      weights[at] = w[i];
+      list[at] = (list[at] & 0xffffffffull) << 32 | (u64)at;
+    }
+  }
+  __syncthreads();
+  s.sort(list, n);
+  own[0] = 0;
+  int index[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = kPer * threadIdx.x + i;
+    index[i] = at < n ? (int)(list[at] >> 32) : -1;
+    w[i] = at < n ? weights[list[at] & 0xffffffffull] : 0ull;
+    own[0] += w[i];
+  }
+  s.template before<u64, 1>(own, start, all);
+  const double target = (double)u * (double)all[0];
+  if (threadIdx.x == 0) s.sh->found[0] = ~0ull;
+  __syncthreads();
+  run = start[0];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (!((double)run > target) && (double)(run + w[i]) > target) s.sh->found[0] = (u64)index[i];
+    run += w[i];
+  }
+  __syncthreads();
+  const int token = s.sh->found[0] == ~0ull ? -1 : (int)s.sh->found[0];
+  *probability = (double)all[0];
+  return token;
+}
 
 template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
@@ -311,12 +449,18 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
   s.base = s.rank * a.slice; s.seg = a.slice / kWarps; s.phase = 0;
   const int64_t row = blockIdx.x / s.ranks;
   pdl_prologue();
+  float temperature = a.temperature ? a.temperature[row * a.temperature_s] : 1.0f;
+  float p = a.top_p ? a.top_p[row * a.top_p_s] : 1.0f;
+  const float m = a.min_p ? a.min_p[row * a.min_p_s] : 0.0f;
+  const int64_t k = a.top_k.p ? index_at(a.top_k, row) : 0;
+  float u = a.uniform[row * a.uniform_s];
   // ---- 1: the slice into shared memory, -infinity behind its end and for NaN
   constexpr int V = Sampler<T>::V;
   T *const data = reinterpret_cast<T *>(raw);
   const T *const src = static_cast<const T *>(a.logits) + row * a.row_stride;
   const T lowest = from_f32<T>(-INFINITY);
   float top = -INFINITY;
+#pragma unroll 4
   for (int i = threadIdx.x * V; i < a.slice; i += kThreads * V) {
     alignas(16) T x[V];
     if (a.vec && s.base + i + V <= a.vocab) {
@@ -333,22 +477,19 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
     }
     *reinterpret_cast<uint4 *>(data + i) = *reinterpret_cast<const uint4 *>(x);
   }
-  const uint32_t top_key = (uint32_t)s.template reduce<true>(key_of(top));  // (its barriers publish the slice too)
-  float temperature = a.temperature ? a.temperature[row * a.temperature_s] : 1.0f;
+  const uint32_t top_key = s.largest(key_of<T>(top));  // (its barriers publish the slice too)
   if (temperature > 0.0f) temperature = fmaxf(temperature, 1e-30f);  // (the bins' scale stays finite)
   int token = -1;
   double probability = 0.0;
-  if (top_key > kNone) {
+  if (top_key > kNone<T>) {
     Row r;
-    r.topf = value_of(top_key);
+    r.topf = value_of<T>(top_key);
     r.top = (double)r.topf;
     r.rate = 1.4426950408889634 / (double)temperature;
     r.scale = 2.0f * (float)kBins / kSpan / temperature;
-    r.cut_key = kNone + 1; r.cut_index = a.vocab;
-    float p = a.top_p ? a.top_p[row * a.top_p_s] : 1.0f;
-    const float m = a.min_p ? a.min_p[row * a.min_p_s] : 0.0f;
+    r.cut_key = kNone<T> + 1; r.cut_index = a.vocab;
     r.least = m > 0.0f ? log2((double)fminf(m, 1.0f)) : -INFINITY;
-    int64_t k = a.top_k.p ? index_at(a.top_k, row) : 0;
+    u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     if (!(temperature > 0.0f)) {
       // the largest logit, lowest index
       u64 total;
@@ -359,6 +500,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
       // ---- 2: counts by distance from the largest
       if (by_k || by_p) {
         uint32_t *h = reinterpret_cast<uint32_t *>(shared.hist);
+        if (threadIdx.x == 0) shared.listed = 0;
         s.clear();
         s.each([&](float z, int) {
           if (z > -INFINITY) atomicAdd(&h[2 * bin_of(r, z)], 1u);
@@ -372,16 +514,38 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         const u64 want = (u64)k;
         int b;
         u64 above;
-        s.template first_bin<u64>(0ull, [&](int i) { return (u64)shared.counts[i]; }, [&](u64 c) { return c >= want; }, &b, &above);
+        s.first_bin(0ull, [&](u64 c) { return c >= want; }, &b, &above);
+        if (above + shared.counts[b] <= (u64)kList && above + shared.counts[b] >= want) {
+          // few enough candidates for one CTA's shared memory: the rest happens there
+          u64 *const list = s.cluster.map_shared_rank(shared.hist, 0);
+          int *const listed = s.cluster.map_shared_rank(&shared.listed, 0);
+          s.each([&](float z, int i) {
+            if (z > -INFINITY && bin_of(r, z) <= b) list[atomicAdd(listed, 1)] = (u64)(uint32_t)~key_of<T>(z) << 32 | (uint32_t)i;
+          });
+          s.cluster.sync();
+          if (s.rank != 0) return;
+          double total;
+          token = draw_listed(s, r, (int)above + (int)shared.counts[b], (int)want, p, u, &total);
+          if (threadIdx.x == 0) {
+            if (token >= 0) {
+              const float z = to_f32(src[(int64_t)token * a.col_stride]);
+              probability = exp2_64(fmax(exponent_of(r, z), -1074.0)) * kOne / total;
+            }
+            if (a.tokens_wide) static_cast<int64_t *>(a.tokens)[row * a.tokens_s] = token;
+            else static_cast<int32_t *>(a.tokens)[row * a.tokens_s] = token;
+            if (a.probabilities) a.probabilities[row * a.probabilities_s] = (float)probability;
+          }
+          return;
+        }
         if (above + shared.counts[b] > want) {  // the cut is inside the bin
           uint32_t lo, hi, key;
-          u64 before, ties;
+          u64 sum_before, ties;
           s.keys_of(r, b, b, &lo, &hi);
-          s.narrow(lo, hi, above, false, [](float, uint32_t, int) { return 1ull; }, [&](u64 c) { return c >= want; }, &key, &before, &ties);
+          s.narrow(lo, hi, above, false, [](float, uint32_t, int) { return 1ull; }, [&](u64 c) { return c >= want; }, &key, &sum_before, &ties);
           r.cut_key = key;
-          if (before + ties > want) {
+          if (sum_before + ties > want) {
             u64 total;
-            r.cut_index = s.locate([&](float, uint32_t x, int) { return (u64)(x == key); }, [&](u64 c, u64) { return c >= want - before; }, &total);
+            r.cut_index = s.locate([&](float, uint32_t x, int) { return (u64)(x == key); }, [&](u64 c, u64) { return c >= want - sum_before; }, &total);
           }
         } else if (above + shared.counts[b] == want) {  // behind it
           uint32_t lo, hi;
@@ -397,48 +561,63 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
       // ---- 4: top-p
       if (by_p) {
         const double share = p > 0.0f ? (double)p : 0.0;  // (0: the first token alone)
-        // a bin's weights, in units of the largest: exp(-x) for x between its ends, with more than fp32's errors to spare
-        const double width = (double)kSpan / kBins;
-        auto most = [&](int i) { return (double)shared.counts[i] * (exp2_64(-i * width * 1.4426950408889634 * (1 - 1e-5)) * 1.0001 + 1e-13); };
-        auto least = [&](int i) {
-          return i == kBins - 1 ? 0.0 : (double)shared.counts[i] * fmax(0.0, exp2_64(-(i + 1) * width * 1.4426950408889634 * (1 + 1e-5)) * 0.9999 - 1e-13);
-        };
-        int b1, b2, last;
-        double x, most_all, least_all;
-        s.template first_bin<double>(0.0, most, [](double) { return false; }, &last, &x);
-        most_all = x + most(last);
-        s.template first_bin<double>(0.0, least, [](double) { return false; }, &last, &x);
-        least_all = x + least(last);
-        s.template first_bin<double>(0.0, most, [&](double c) { return c >= share * least_all * (1 - 1e-9); }, &b1, &x);
-        s.template first_bin<double>(0.0, least, [&](double c) { return c >= share * most_all * (1 + 1e-9); }, &b2, &x);
-        b2 = max(b1, b2);
+        // A bin's weights, in units of the largest, are exp(-x) for x between its ends: sums of the most and of the least they can
+        // be, with more than fp32's errors to spare.
+        const float width = kSpan / kBins * 1.4426950408889634f;
+        double own[2] = {0.0, 0.0}, start[2], all2[2], most[kPer], least[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int i = kPer * threadIdx.x + j;
+          const double count = (double)shared.counts[i];
+          most[j] = count * ((double)exp2f(-(float)i * width * (1.0f - 1e-5f)) * 1.0001 + 1e-13);
+          least[j] = i == kBins - 1 ? 0.0 : count * fmax(0.0, (double)exp2f(-(float)(i + 1) * width * (1.0f + 1e-5f)) * 0.9999 - 1e-13);
+          own[0] += most[j];
+          own[1] += least[j];
+        }
+        if (threadIdx.x == 0) reinterpret_cast<int *>(shared.found)[0] = reinterpret_cast<int *>(shared.found)[1] = kBins - 1;
+        s.template before<double, 2>(own, start, all2);
+        int *const ends = reinterpret_cast<int *>(shared.found);
+        // the cut is no earlier than the first bin that the most can reach it in, and no later than the first that the least must
+        const double early = share * all2[1] * (1 - 1e-9), late = share * all2[0] * (1 + 1e-9);
+#pragma unroll
+        for (int j = kPer - 1; j >= 0; --j) {
+          double c0 = start[0], c1 = start[1];
+          for (int i = 0; i <= j; ++i) { c0 += most[i]; c1 += least[i]; }
+          if (c0 >= early) atomicMin(&ends[0], kPer * (int)threadIdx.x + j);
+          if (c1 >= late) atomicMin(&ends[1], kPer * (int)threadIdx.x + j);
+        }
+        __syncthreads();
+        const int b1 = ends[0], b2 = max(b1, ends[1]);
+        __syncthreads();
         uint32_t lo, hi;
         s.keys_of(r, b1, b2, &lo, &hi);
         const int shift = Sampler<T>::shift_of(lo, hi);
         u64 all = 0, over = 0;
         s.clear();
         s.each([&](float z, int i) {
-          const uint32_t key = key_of(z);
-          if (key > kNone && kept_by_cut(r, key, i)) {
+          const uint32_t key = key_of<T>(z);
+          if (key > kNone<T> && kept_by_cut(r, key, i)) {
             const u64 w = weight_of(r, z);
             all += w;
             if (key > hi) over += w;
             else if (key >= lo && w) atomicAdd(&shared.hist[(hi - key) >> shift], w);
           }
         });
-        s.merge();
-        all = s.template reduce<false>(all);
-        over = s.template reduce<false>(over);
+        all = s.block_sum(all);
+        over = s.block_sum(over);
+        s.merge(all, over);
+        all = s.sum_of(0);
+        over = s.sum_of(1);
         const double want = share * (double)all;
         uint32_t key;
-        u64 before, ties;
+        u64 sum_before, ties;
         s.narrow(lo, hi, over, true, [&](float z, uint32_t x, int i) { return kept_by_cut(r, x, i) ? weight_of(r, z) : 0ull; },
-                 [&](u64 c) { return (double)c >= want && c > 0; }, &key, &before, &ties);
-        const u64 w = weight_of(r, value_of(key));
+                 [&](u64 c) { return (double)c >= want && c > 0; }, &key, &sum_before, &ties);
+        const u64 w = weight_of(r, value_of<T>(key));
         // of the tied tokens the first n: those before which less than `want` lies
-        u64 n = w ? (u64)fmax(ceil((want - (double)before) / (double)w), 1.0) : 1;
-        while (n > 1 && !((double)(before + (n - 1) * w) < want)) --n;
-        while (w && (double)(before + n * w) < want && n * w < ties) ++n;
+        u64 n = w ? (u64)fmax(ceil((want - (double)sum_before) / (double)w), 1.0) : 1;
+        while (n > 1 && !((double)(sum_before + (n - 1) * w) < want)) --n;
+        while (w && (double)(sum_before + n * w) < want && n * w < ties) ++n;
         int index = r.cut_index;
         if (w && n * w < ties) {
           u64 total;
@@ -450,12 +629,10 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         r.cut_index = index;
       }
       // ---- 5: the draw
-      float u = a.uniform[row * a.uniform_s];
-      u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
       u64 total;
       token = s.locate(
           [&](float z, uint32_t key, int i) {
-            return key > kNone && kept_by_cut(r, key, i) && exponent_of(r, z) >= r.least ? weight_of(r, z) : 0ull;
+            return key > kNone<T> && kept_by_cut(r, key, i) && exponent_of(r, z) >= r.least ? weight_of(r, z) : 0ull;
           },
           [&](u64 c, u64 sum) { return (double)c > (double)u * (double)sum; }, &total);
       if (token >= s.base && token < s.base + a.slice) {
