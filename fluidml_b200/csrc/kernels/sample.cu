@@ -20,6 +20,7 @@
 #include "serving_common.cuh"
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 namespace cg = cooperative_groups;
 
@@ -54,25 +55,43 @@ struct Shared {
   int listed;
 };
 
-// Integers in the order of the logits, without the bits that the type does not have; both zeros are one.
-template <typename T> struct Key;
-template <> struct Key<float> { static constexpr int kDrop = 0; };
-template <> struct Key<__half> { static constexpr int kDrop = 13; };
-template <> struct Key<__nv_bfloat16> { static constexpr int kDrop = 16; };
-template <typename T> __device__ __forceinline__ uint32_t key_of(float z) {
-  const uint32_t u = __float_as_uint(z + 0.0f);
-  return (u & 0x80000000u ? ~u : u | 0x80000000u) >> Key<T>::kDrop;
+// Integers in the order of the logits, as wide as the type; both zeros are one.  Shared memory holds these: cuts compare them.
+template <typename T> struct Key {  // 16-bit types
+  using Int = uint16_t;
+  static constexpr uint32_t kInfinity = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u, kNone = 0xffffu ^ kInfinity;  // of +, - infinity
+  __device__ __forceinline__ static uint32_t of(uint32_t u) {
+    return u == 0x8000u ? 0x8000u : u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+  }
+  __device__ __forceinline__ static float value(uint32_t k) {
+    const unsigned short u = (unsigned short)(k & 0x8000u ? k ^ 0x8000u : ~k);
+    return to_f32(*reinterpret_cast<const T *>(&u));
+  }
+  // two at a time
+  __device__ __forceinline__ static uint32_t of_pair(uint32_t u) {
+    u = zeros_alike(u);
+    return u ^ (0x80008000u | (u >> 15 & 0x00010001u) * 0x7fffu);
+  }
+  __device__ __forceinline__ static uint32_t zeros_alike(uint32_t u);  // -0 -> 0: adds 0
+};
+template <> __device__ __forceinline__ uint32_t Key<__half>::zeros_alike(uint32_t u) {
+  const __half2 y = __hadd2(*reinterpret_cast<const __half2 *>(&u), __half2half2(__ushort_as_half(0)));
+  return *reinterpret_cast<const uint32_t *>(&y);
 }
-template <typename T> __device__ __forceinline__ float value_of(uint32_t k) {
-  k <<= Key<T>::kDrop;
-  // (a negative number's dropped bits are ones in its key)
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~(k | ((1u << Key<T>::kDrop) - 1u)));
+template <> __device__ __forceinline__ uint32_t Key<__nv_bfloat16>::zeros_alike(uint32_t u) {
+  const __nv_bfloat162 y = __hadd2(*reinterpret_cast<const __nv_bfloat162 *>(&u), __bfloat162bfloat162(__ushort_as_bfloat16(0)));
+  return *reinterpret_cast<const uint32_t *>(&y);
 }
-template <typename T> constexpr uint32_t kNone = 0x007fffffu >> Key<T>::kDrop;  // key of -infinity: nothing to draw
+template <> struct Key<float> {
+  using Int = uint32_t;
+  static constexpr uint32_t kInfinity = 0xff800000u, kNone = 0x007fffffu;
+  // (on the bits as they were loaded: of a float's, the compiler makes setting the sign a negation, which loses a NaN's bits)
+  __device__ __forceinline__ static uint32_t of(uint32_t u) { return u == 0x80000000u ? u : u & 0x80000000u ? ~u : u | 0x80000000u; }
+  __device__ __forceinline__ static float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+};
 
-// 2^x for -1100 < x <= 0: the fraction's Taylor series (terms ln(2)^n / n!) to the 11th power, 6e-15 on half a unit.
-__device__ __forceinline__ double exp2_64(double x) {
-  const double n = rint(x), f = (x - n) * 0.6931471805599453;
+// The fraction's part of 2^x for the rest f of x, |f| <= 1 / 2: Taylor's series of e^(f ln 2) to the 11th power, 6e-15.
+__device__ __forceinline__ double exp2_rest(double f) {
+  f *= 0.6931471805599453;
   double p = 1.0 / 39916800.0;
   p = fma(p, f, 1.0 / 3628800.0);
   p = fma(p, f, 1.0 / 362880.0);
@@ -84,8 +103,11 @@ __device__ __forceinline__ double exp2_64(double x) {
   p = fma(p, f, 1.0 / 6.0);
   p = fma(p, f, 0.5);
   p = fma(p, f, 1.0);
-  p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
+  return fma(p, f, 1.0);
+}
+__device__ __forceinline__ double exp2_64(double x) {  // -1100 < x <= 0
+  const double n = rint(x);
+  return ldexp(exp2_rest(x - n), (int)n);
 }
 
 struct Row {
@@ -99,14 +121,17 @@ struct Row {
 __device__ __forceinline__ double exponent_of(const Row &r, float z) { return z == r.topf ? 0.0 : ((double)z - r.top) * r.rate; }
 __device__ __forceinline__ u64 weight_of(const Row &r, float z) {
   const double t = exponent_of(r, z);
-  if (t < -45.0) return t > -1075.0 ? 1ull : 0ull;  // (a weight that 64 bits hold; NaN, of an infinite rate: none)
-  if (!(t >= -45.0)) return 0ull;
-  const u64 w = (u64)__double2ull_rn(exp2_64(t) * kOne);
+  if (!(t >= -45.0)) return t > -1075.0 ? 1ull : 0ull;  // (a weight that 64 bits hold; NaN, of an infinite rate: none)
+  // adding 1.5 x 2^52 leaves the nearest integer in the low bits, adding 2^52 the rounded weight
+  const double shifted = t + 6755399441055744.0;
+  const double p = exp2_rest(t - (shifted - 6755399441055744.0));
+  const double scaled = __hiloint2double(__double2hiint(p) + ((__double2loint(shifted) + 44) << 20), __double2loint(p));
+  const u64 w = (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;
   return w ? w : 1ull;
 }
 __device__ __forceinline__ int bin_of(const Row &r, float z) {
-  // (halves: the difference of two finite logits may not be finite; NaN goes last)
-  return z >= r.topf ? 0 : (int)fminf((0.5f * r.topf - 0.5f * z) * r.scale, (float)(kBins - 1));
+  // (halves: the difference of two finite logits may not be finite; that of two infinite ones is NaN, whose integer is 0)
+  return min((int)(fmaf(z, -0.5f, 0.5f * r.topf) * r.scale), kBins - 1);
 }
 __device__ __forceinline__ bool kept_by_cut(const Row &r, uint32_t key, int index) {
   return key > r.cut_key || (key == r.cut_key && index <= r.cut_index);
@@ -114,19 +139,24 @@ __device__ __forceinline__ bool kept_by_cut(const Row &r, uint32_t key, int inde
 
 template <typename T> struct Sampler {
   static constexpr int V = 16 / sizeof(T);  // logits per access
-  const T *data;
+  using Int = typename Key<T>::Int;
+  const Int *data;
   Shared *sh;
   cg::cluster_group cluster;
   int rank, ranks, base, seg, warp, lane, phase;
+  uint32_t top_key;
 
-  // f(logit, index in the vocabulary) over the warp's part, in order by lane; the part is whole accesses
+  // f(key, index in the vocabulary) over the warp's part, in order by lane; the part is whole accesses
   template <typename F> __device__ __forceinline__ void each(F f) const {
     for (int i = warp * seg + lane * V; i < (warp + 1) * seg; i += 32 * V) {
       const uint4 raw = *reinterpret_cast<const uint4 *>(data + i);
-      const T *x = reinterpret_cast<const T *>(&raw);
 #pragma unroll
-      for (int j = 0; j < V; ++j) f(to_f32(x[j]), base + i + j);
+      for (int j = 0; j < V; ++j) f(key_in(raw, j), base + i + j);
     }
+  }
+  __device__ __forceinline__ static uint32_t key_in(const uint4 &raw, int j) {
+    const uint32_t w = sizeof(T) == 4 ? 0u : j < 2 ? raw.x : j < 4 ? raw.y : j < 6 ? raw.z : raw.w;
+    return sizeof(T) == 4 ? (j == 0 ? raw.x : j == 1 ? raw.y : j == 2 ? raw.z : raw.w) : j & 1 ? w >> 16 : w & 0xffffu;
   }
   __device__ __forceinline__ u64 *part() { return reinterpret_cast<u64 *>(sh->part); }
   __device__ __forceinline__ u64 warp_sum(u64 v) const {
@@ -248,11 +278,11 @@ template <typename T> struct Sampler {
   }
   // The keys of bins [b1, b2]: bin_of is monotone, so they are an interval.  A warp asks 32 keys at a time for either end.
   __device__ void keys_of(const Row &r, int b1, int b2, uint32_t *lo, uint32_t *hi) const {
-    const uint32_t top = key_of<T>(r.topf);
-    uint32_t l = kNone<T> + 1, h = top;  // the smallest key of a bin up to b2 is in [l, h]
+    const uint32_t top = top_key;
+    uint32_t l = Key<T>::kNone + 1, h = top;  // the smallest key of a bin up to b2 is in [l, h]
     while (l < h) {
       const uint32_t step = (h - l) / 33 + 1, m = min(l + (lane + 1) * step - 1, h);
-      const unsigned yes = __ballot_sync(0xffffffffu, bin_of(r, value_of<T>(m)) <= b2);
+      const unsigned yes = __ballot_sync(0xffffffffu, bin_of(r, Key<T>::value(m)) <= b2);
       const int k = yes ? __ffs(yes) - 1 : 32;  // the first that is
       const uint32_t was = l;
       if (k > 0) l = min(was + (uint32_t)k * step, h);
@@ -262,7 +292,7 @@ template <typename T> struct Sampler {
     h = top;  // the largest key of a bin from b1 on is in [l, h]
     while (l < h) {
       const uint32_t step = (h - l) / 33 + 1, m = min(l + (lane + 1) * step, h);
-      const unsigned yes = __ballot_sync(0xffffffffu, bin_of(r, value_of<T>(m)) >= b1);
+      const unsigned yes = __ballot_sync(0xffffffffu, bin_of(r, Key<T>::value(m)) >= b1);
       const int k = __popc(yes);  // the first k are
       const uint32_t was = l;
       if (k > 0) l = min(was + (uint32_t)k * step, h);
@@ -278,10 +308,9 @@ template <typename T> struct Sampler {
       const int shift = shift_of(lo, hi);
       if (!first) {
         clear();
-        each([&](float z, int i) {
-          const uint32_t k = key_of<T>(z);
+        each([&](uint32_t k, int i) {
           if (k >= lo && k <= hi) {
-            const u64 m = measure(z, k, i);
+            const u64 m = measure(k, i);
             if (m) atomicAdd(&sh->hist[(hi - k) >> shift], m);
           }
         });
@@ -301,10 +330,10 @@ template <typename T> struct Sampler {
   }
   __device__ __forceinline__ static int shift_of(uint32_t lo, uint32_t hi) { return max(0, 22 - __clz((int)((hi - lo) | 1u))); }
 
-  // The first index, in the vocabulary's order, at which the running sum of measure(z, key, index) has reached(sum); -1: none.
+  // The first index, in the vocabulary's order, at which the running sum of measure(key, index) has reached(sum); -1: none.
   template <typename M, typename R> __device__ int locate(M measure, R reached, u64 *total) {
     u64 mine = 0;
-    each([&](float z, int i) { mine += measure(z, key_of<T>(z), i); });
+    each([&](uint32_t k, int i) { mine += measure(k, i); });
     mine = warp_sum(mine);
     __syncthreads();
     if (lane == 0) part()[warp] = mine;
@@ -326,14 +355,9 @@ template <typename T> struct Sampler {
       bool done = false;
       for (int i = warp * seg + lane * V; i < (warp + 1) * seg && !done; i += 32 * V) {
         const uint4 raw = *reinterpret_cast<const uint4 *>(data + i);
-        const T *v = reinterpret_cast<const T *>(&raw);
         u64 m[V], own = 0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float z = to_f32(v[j]);
-          m[j] = measure(z, key_of<T>(z), base + i + j);
-          own += m[j];
-        }
+        for (int j = 0; j < V; ++j) own += m[j] = measure(key_in(raw, j), base + i + j);
         u64 run = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -387,7 +411,7 @@ __device__ int draw_listed(Sampler<T> &s, const Row &r, int n, int k, float p, f
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int at = kPer * threadIdx.x + i;
-    w[i] = at < n ? weight_of(r, value_of<T>(~(uint32_t)(list[at] >> 32))) : 0ull;
+    w[i] = at < n ? weight_of(r, Key<T>::value(~(uint32_t)(list[at] >> 32))) : 0ull;
     own[0] += w[i];
   }
   s.template before<u64, 1>(own, start, all);
@@ -399,7 +423,7 @@ __device__ int draw_listed(Sampler<T> &s, const Row &r, int n, int k, float p, f
     const u64 sum_before = run;
     run += w[i];
     const bool kept = at < n && (!(p < 1.0f) || at == 0 || (double)sum_before < want) &&
-                      exponent_of(r, value_of<T>(~(uint32_t)(list[at] >> 32))) >= r.least;
+                      exponent_of(r, Key<T>::value(~(uint32_t)(list[at] >> 32))) >= r.least;
     if (!kept) w[i] = 0;
   }
   __syncthreads();
@@ -442,7 +466,8 @@ __device__ int draw_listed(Sampler<T> &s, const Row &r, int n, int k, float p, f
 template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   __shared__ Shared shared;
-  Sampler<T> s{reinterpret_cast<const T *>(raw), &shared, cg::this_cluster()};
+  using Int = typename Key<T>::Int;
+  Sampler<T> s{reinterpret_cast<const Int *>(raw), &shared, cg::this_cluster()};
   s.rank = (int)s.cluster.block_rank();
   s.ranks = (int)s.cluster.num_blocks();
   s.warp = threadIdx.x >> 5; s.lane = threadIdx.x & 31;
@@ -454,46 +479,73 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
   const float m = a.min_p ? a.min_p[row * a.min_p_s] : 0.0f;
   const int64_t k = a.top_k.p ? index_at(a.top_k, row) : 0;
   float u = a.uniform[row * a.uniform_s];
-  // ---- 1: the slice into shared memory, -infinity behind its end and for NaN
+  // ---- 1: the slice's keys into shared memory, -infinity behind its end and for NaN
   constexpr int V = Sampler<T>::V;
-  T *const data = reinterpret_cast<T *>(raw);
+  Int *const data = reinterpret_cast<Int *>(raw);
   const T *const src = static_cast<const T *>(a.logits) + row * a.row_stride;
-  const T lowest = from_f32<T>(-INFINITY);
-  float top = -INFINITY;
+  uint32_t top = 0, bottom = 0xffffffffu;  // (16-bit types: of pairs)
 #pragma unroll 4
   for (int i = threadIdx.x * V; i < a.slice; i += kThreads * V) {
-    alignas(16) T x[V];
+    uint4 k;
+    uint32_t *const w = reinterpret_cast<uint32_t *>(&k);
     if (a.vec && s.base + i + V <= a.vocab) {
-      *reinterpret_cast<uint4 *>(x) = __ldg(reinterpret_cast<const uint4 *>(src + s.base + i));
+      const uint4 x = __ldg(reinterpret_cast<const uint4 *>(src + s.base + i));
+      const uint32_t *const y = reinterpret_cast<const uint32_t *>(&x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) w[j] = Key<T>::of_pair(y[j]);
+        else w[j] = Key<T>::of(y[j]);
+      }
     } else {
+      uint32_t y[V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = s.base + i + j < a.vocab ? src[(int64_t)(s.base + i + j) * a.col_stride] : lowest;
+      for (int j = 0; j < V; ++j) y[j] = s.base + i + j < a.vocab ? Key<T>::of(reinterpret_cast<const Int *>(src)[(int64_t)(s.base + i + j) * a.col_stride]) : Key<T>::kNone;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = sizeof(T) == 4 ? y[j] : y[2 * j % V] | y[(2 * j + 1) % V] << 16;
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float z = to_f32(x[j]);
-      if (z != z) x[j] = lowest;
-      top = fmaxf(top, z);  // (leaves NaN out)
+    for (int j = 0; j < 4; ++j) {
+      top = sizeof(T) == 2 ? __vmaxu2(top, w[j]) : max(top, w[j]);
+      bottom = sizeof(T) == 2 ? __vminu2(bottom, w[j]) : min(bottom, w[j]);
     }
-    *reinterpret_cast<uint4 *>(data + i) = *reinterpret_cast<const uint4 *>(x);
+    *reinterpret_cast<uint4 *>(data + i) = k;
   }
-  const uint32_t top_key = s.largest(key_of<T>(top));  // (its barriers publish the slice too)
+  if (sizeof(T) == 2) {
+    top = max(top >> 16, top & 0xffffu);
+    bottom = min(bottom >> 16, bottom & 0xffffu);
+  }
+  if (top > Key<T>::kInfinity || bottom < Key<T>::kNone) {  // rare: NaN lies beyond the infinities
+    top = 0;
+    for (int i = threadIdx.x * V; i < a.slice; i += kThreads * V) {
+      uint4 k = *reinterpret_cast<const uint4 *>(data + i);
+      uint32_t *const w = reinterpret_cast<uint32_t *>(&k);
+      for (int j = 0; j < V; ++j) {
+        const uint32_t key = Sampler<T>::key_in(k, j);
+        if (key <= Key<T>::kInfinity && key >= Key<T>::kNone) top = max(top, key);
+        else if (sizeof(T) == 4) w[j] = Key<T>::kNone;
+        else w[j >> 1] = j & 1 ? (w[j >> 1] & 0xffffu) | Key<T>::kNone << 16 : (w[j >> 1] & 0xffff0000u) | Key<T>::kNone;
+      }
+      *reinterpret_cast<uint4 *>(data + i) = k;
+    }
+  }
+  const uint32_t top_key = s.largest(top);  // (its barriers publish the slice too)
+  s.top_key = top_key;
   if (temperature > 0.0f) temperature = fmaxf(temperature, 1e-30f);  // (the bins' scale stays finite)
   int token = -1;
   double probability = 0.0;
-  if (top_key > kNone<T>) {
+  if (top_key > Key<T>::kNone) {
     Row r;
-    r.topf = value_of<T>(top_key);
+    r.topf = Key<T>::value(top_key);
     r.top = (double)r.topf;
     r.rate = 1.4426950408889634 / (double)temperature;
     r.scale = 2.0f * (float)kBins / kSpan / temperature;
-    r.cut_key = kNone<T> + 1; r.cut_index = a.vocab;
+    r.cut_key = Key<T>::kNone + 1; r.cut_index = a.vocab;
     r.least = m > 0.0f ? log2((double)fminf(m, 1.0f)) : -INFINITY;
     u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     if (!(temperature > 0.0f)) {
       // the largest logit, lowest index
       u64 total;
-      token = s.locate([&](float, uint32_t key, int) { return (u64)(key == top_key); }, [](u64 c, u64) { return c >= 1; }, &total);
+      token = s.locate([&](uint32_t key, int) { return (u64)(key == top_key); }, [](u64 c, u64) { return c >= 1; }, &total);
       probability = 1.0;
     } else {
       const bool by_k = k > 0 && k < a.vocab, by_p = p < 1.0f;
@@ -502,8 +554,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         uint32_t *h = reinterpret_cast<uint32_t *>(shared.hist);
         if (threadIdx.x == 0) shared.listed = 0;
         s.clear();
-        s.each([&](float z, int) {
-          if (z > -INFINITY) atomicAdd(&h[2 * bin_of(r, z)], 1u);
+        s.each([&](uint32_t key, int) {
+          if (key > Key<T>::kNone) atomicAdd(&h[2 * bin_of(r, Key<T>::value(key))], 1u);
         });
         s.merge();  // (64-bit words whose upper halves are zero)
         for (int i = threadIdx.x; i < kBins; i += kThreads) shared.counts[i] = (uint32_t)shared.merged[i];
@@ -519,8 +571,10 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
           // few enough candidates for one CTA's shared memory: the rest happens there
           u64 *const list = s.cluster.map_shared_rank(shared.hist, 0);
           int *const listed = s.cluster.map_shared_rank(&shared.listed, 0);
-          s.each([&](float z, int i) {
-            if (z > -INFINITY && bin_of(r, z) <= b) list[atomicAdd(listed, 1)] = (u64)(uint32_t)~key_of<T>(z) << 32 | (uint32_t)i;
+          uint32_t lo, hi;
+          s.keys_of(r, 0, b, &lo, &hi);
+          s.each([&](uint32_t key, int i) {
+            if (key >= lo) list[atomicAdd(listed, 1)] = (u64)(uint32_t)~key << 32 | (uint32_t)i;
           });
           s.cluster.sync();
           if (s.rank != 0) return;
@@ -528,7 +582,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
           token = draw_listed(s, r, (int)above + (int)shared.counts[b], (int)want, p, u, &total);
           if (threadIdx.x == 0) {
             if (token >= 0) {
-              const float z = to_f32(src[(int64_t)token * a.col_stride]);
+              const float z = to_f32(src[(int64_t)token * a.col_stride]);  // (perhaps another CTA's)
               probability = exp2_64(fmax(exponent_of(r, z), -1074.0)) * kOne / total;
             }
             if (a.tokens_wide) static_cast<int64_t *>(a.tokens)[row * a.tokens_s] = token;
@@ -541,11 +595,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
           uint32_t lo, hi, key;
           u64 sum_before, ties;
           s.keys_of(r, b, b, &lo, &hi);
-          s.narrow(lo, hi, above, false, [](float, uint32_t, int) { return 1ull; }, [&](u64 c) { return c >= want; }, &key, &sum_before, &ties);
+          s.narrow(lo, hi, above, false, [](uint32_t, int) { return 1ull; }, [&](u64 c) { return c >= want; }, &key, &sum_before, &ties);
           r.cut_key = key;
           if (sum_before + ties > want) {
             u64 total;
-            r.cut_index = s.locate([&](float, uint32_t x, int) { return (u64)(x == key); }, [&](u64 c, u64) { return c >= want - sum_before; }, &total);
+            r.cut_index = s.locate([&](uint32_t x, int) { return (u64)(x == key); }, [&](u64 c, u64) { return c >= want - sum_before; }, &total);
           }
         } else if (above + shared.counts[b] == want) {  // behind it
           uint32_t lo, hi;
@@ -594,10 +648,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         const int shift = Sampler<T>::shift_of(lo, hi);
         u64 all = 0, over = 0;
         s.clear();
-        s.each([&](float z, int i) {
-          const uint32_t key = key_of<T>(z);
-          if (key > kNone<T> && kept_by_cut(r, key, i)) {
-            const u64 w = weight_of(r, z);
+        s.each([&](uint32_t key, int i) {
+          if (key > Key<T>::kNone && kept_by_cut(r, key, i)) {
+            const u64 w = weight_of(r, Key<T>::value(key));
             all += w;
             if (key > hi) over += w;
             else if (key >= lo && w) atomicAdd(&shared.hist[(hi - key) >> shift], w);
@@ -611,9 +664,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         const double want = share * (double)all;
         uint32_t key;
         u64 sum_before, ties;
-        s.narrow(lo, hi, over, true, [&](float z, uint32_t x, int i) { return kept_by_cut(r, x, i) ? weight_of(r, z) : 0ull; },
+        s.narrow(lo, hi, over, true, [&](uint32_t x, int i) { return kept_by_cut(r, x, i) ? weight_of(r, Key<T>::value(x)) : 0ull; },
                  [&](u64 c) { return (double)c >= want && c > 0; }, &key, &sum_before, &ties);
-        const u64 w = weight_of(r, value_of<T>(key));
+        const u64 w = weight_of(r, Key<T>::value(key));
         // of the tied tokens the first n: those before which less than `want` lies
         u64 n = w ? (u64)fmax(ceil((want - (double)sum_before) / (double)w), 1.0) : 1;
         while (n > 1 && !((double)(sum_before + (n - 1) * w) < want)) --n;
@@ -621,7 +674,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         int index = r.cut_index;
         if (w && n * w < ties) {
           u64 total;
-          index = s.locate([&](float, uint32_t x, int i) { return (u64)(x == key && kept_by_cut(r, x, i)); }, [&](u64 c, u64) { return c >= n; }, &total);
+          index = s.locate([&](uint32_t x, int i) { return (u64)(x == key && kept_by_cut(r, x, i)); }, [&](u64 c, u64) { return c >= n; }, &total);
         } else if (key != r.cut_key) {
           index = a.vocab;
         }
@@ -631,12 +684,17 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
       // ---- 5: the draw
       u64 total;
       token = s.locate(
-          [&](float z, uint32_t key, int i) {
-            return key > kNone<T> && kept_by_cut(r, key, i) && exponent_of(r, z) >= r.least ? weight_of(r, z) : 0ull;
+          [&](uint32_t key, int i) {
+            if (key <= Key<T>::kNone || !kept_by_cut(r, key, i)) return 0ull;
+            const float z = Key<T>::value(key);
+            return exponent_of(r, z) >= r.least ? weight_of(r, z) : 0ull;
           },
           [&](u64 c, u64 sum) { return (double)c > (double)u * (double)sum; }, &total);
       if (token >= s.base && token < s.base + a.slice) {
-        const float z = to_f32(data[token - s.base]);
+        const uint4 k = *reinterpret_cast<const uint4 *>(data + (token - s.base) / V * V);
+        const uint32_t *const w = reinterpret_cast<const uint32_t *>(&k);
+        const int j = (token - s.base) % V;
+        const float z = Key<T>::value(sizeof(T) == 4 ? w[j] : j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
         probability = exp2_64(fmax(exponent_of(r, z), -1074.0)) * kOne / (double)total;
       }
     }
