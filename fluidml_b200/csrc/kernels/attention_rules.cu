@@ -1,7 +1,7 @@
 // Attention over a prompt by rules (fml_attention_rules): capped scores, a bias by distance, documents, a prefix, grouped heads.
 //
 // Here: argument checks, the choice of the kernel, and the kernel on warp-wide matrix instructions, which takes fp32 and every
-// layout: a CTA has 64 queries of a head, four warps of 16, and keys pass in tiles through two stages of shared memory.  Large
+// layout: a CTA has 64 (fp32: 128) queries of a head, 16 to a warp, and keys pass in tiles through two stages of shared memory.  Large
 // 16-bit problems run on the fifth-generation tensor cores (attention_rules_tc.cu).
 //
 // A tile of keys that no query of the CTA sees is not loaded: causal and prefix leave the tiles up to a last one, documents are
@@ -13,19 +13,22 @@
 namespace fml {
 namespace {
 
-constexpr int kThreads = 128, kRows = 64, kMaxTiles = 4096;
+constexpr int kMaxTiles = 4096;
 
 template <typename T, int DP> struct Shape {
-  using F = Flash<T, DP>;
+  using F = Flash<T, DP, true>;
+  // fp32 is bound by the instructions that split its operands: twice the warps share what is loaded
+  static constexpr int kThreads = sizeof(T) == 4 ? 256 : 128, kRows = kThreads / 2;
   static constexpr int kKeys = sizeof(T) == 2 ? 64 : DP == 64 ? 64 : 32, kGroups = kKeys / 8;
   static constexpr int kTileK = kKeys * F::kPitch, kTileV = kKeys * F::kPitchV, kStage = kTileK + kTileV, kQ = kRows * F::kPitch;
   static constexpr size_t kBytes = kQ + 2 * kStage + kMaxTiles;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) attention_rules_kernel(const __grid_constant__ RulesArgs a) {
+__global__ void __launch_bounds__(Shape<T, DP>::kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) attention_rules_kernel(const __grid_constant__ RulesArgs a) {
   using S = Shape<T, DP>;
   using F = typename S::F;
+  constexpr int kThreads = S::kThreads, kRows = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *const visible = smem + S::kQ + 2 * S::kStage;  // [tile]: TileView
   const uint32_t q_tile = smem_u32(smem), data = q_tile + S::kQ;
@@ -101,16 +104,7 @@ __global__ void __launch_bounds__(kThreads) attention_rules_kernel(const __grid_
     const bool open = view_of(tile) == kTileAll;
     const int key_base = tile * S::kKeys;
     flash_step<F, DP, S::kGroups>(run, qf, q_tile, 16 * warp, k_tile, k_tile + S::kTileK, 0, [&](float (&s)[S::kGroups][4]) {
-#pragma unroll
-      for (int n = 0; n < S::kGroups; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] *= a.cap.scale;
-      if (a.cap.cap > 0.0f) {
-#pragma unroll
-        for (int n = 0; n < S::kGroups; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] = a.cap.cap * tanh_of<sizeof(T) == 4>(s[n][i]);
-      }
+      cap_scores<sizeof(T) == 4>(a.cap, s);
       if (a.slopes) {
 #pragma unroll
         for (int n = 0; n < S::kGroups; ++n)
@@ -172,7 +166,7 @@ template <typename T, int DP> int launch_mma(const RulesArgs &a, cudaStream_t s)
     FML_CUDA(cudaFuncSetAttribute(attention_rules_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kBytes));
     attr_set[dev & 63] = true;
   }
-  FML_LAUNCH((attention_rules_kernel<T, DP>), dim3((unsigned)((a.Sq + kRows - 1) / kRows), (unsigned)a.heads, (unsigned)a.batch), kThreads,
+  FML_LAUNCH((attention_rules_kernel<T, DP>), dim3((unsigned)((a.Sq + S::kRows - 1) / S::kRows), (unsigned)a.heads, (unsigned)a.batch), S::kThreads,
              S::kBytes, s, a);
   return FML_OK;
 }

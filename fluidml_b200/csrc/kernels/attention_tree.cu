@@ -14,7 +14,7 @@
 namespace fml {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kJoinThreads = 128;
 
 struct TreeArgs {
   const void *q, *k, *v;
@@ -107,37 +107,39 @@ __device__ __noinline__ void redo_row(const TreeArgs &a, int r, const Request &x
   if (lane == 0) { stats[0] = m; stats[1] = l; }
 }
 
-// WR x 4 / WR warps: WR of 16 rows each, the others take different keys of a tile.
+// Warps: WR of 16 rows each, times those that take different keys of a tile.  Tiles of up to 16 rows: four warps, queries in
+// registers, three stages of 64 keys.  More rows: eight warps, which leaves each half of the registers, so the queries are read
+// from shared memory again and again, and two stages.
 template <typename T, int DP, int WR> struct Shape {
-  using F = Flash<T, DP>;
-  static constexpr int kWarpsK = 4 / WR, kRows = 16 * WR;
-  // keys of a tile: 32 KiB of keys and values for head size 128, in three stages for two CTAs per SM
-  static constexpr int kKeys = sizeof(T) == 2 ? 64 : DP == 64 ? 64 : 32;
+  static constexpr bool kHeld = WR == 1;
+  using F = Flash<T, DP, kHeld>;
+  static constexpr int kWarps = WR == 1 ? 4 : 8, kThreads = 32 * kWarps, kWarpsK = kWarps / WR, kRows = 16 * WR;
+  static constexpr int kKeys = sizeof(T) == 2 ? 64 : DP == 64 ? 64 : 32;  // 32 KiB of keys and values for head size 128
   static constexpr int kWarpKeys = kKeys / kWarpsK, kGroups = kWarpKeys / 8;
   static constexpr int kTileK = kKeys * F::kPitch, kTileV = kKeys * F::kPitchV, kStage = kTileK + kTileV;
-  static constexpr int kQ = kRows * F::kPitch, kMerge = 64 * (DP + 4) * 4;
-  // 16-bit queries move on to registers: their tile is where the third stage will be.  fp32 ones stay, and of more than 16 rows
-  // leave room for two stages only.
-  static constexpr bool kQInStage = sizeof(T) == 2;
-  static constexpr int kStagesUsed = kQInStage || WR == 1 ? 3 : 2;
+  static constexpr int kQ = kRows * F::kPitch, kMerge = kWarps * 16 * (DP + 4) * 4;
+  // held queries move on to registers: their tile is where the third stage will be
+  static constexpr bool kQInStage = kHeld && sizeof(T) == 2;
+  static constexpr int kStagesUsed = kHeld ? 3 : 2;
   static constexpr int kData = kStagesUsed * kStage > kMerge ? kStagesUsed * kStage : kMerge;
   static constexpr int kOffsets = (kStagesUsed + 1) * kKeys * 8;
-  static constexpr size_t kBytes = (kQInStage ? 0 : kQ) + kData + kOffsets + 64 * 2 * 4 + 64 * 4 + 64;
+  static constexpr size_t kBytes = (kQInStage ? 0 : kQ) + kData + kOffsets + kWarps * 16 * 2 * 4 + 64 * 4 + 64;
   static constexpr int kPartial = kRows * (DP + 2);  // floats of a partial result
   static_assert((kQ <= kStage || !kQInStage) && 2 * (kBytes + 1024) <= 228 * 1024, "two CTAs per SM");
 };
 
 template <typename T, int DP, int WR>
-__global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_constant__ TreeArgs a) {
+__global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_kernel(const __grid_constant__ TreeArgs a) {
   using S = Shape<T, DP, WR>;
+  constexpr int kThreads = S::kThreads;
   using F = typename S::F;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *const data_ptr = smem + (S::kQInStage ? 0 : S::kQ);
   long long *const places = reinterpret_cast<long long *>(data_ptr + S::kData);   // [stage + 1][key]: page << 32 | position, -1 none
-  float *const stats = reinterpret_cast<float *>(places + (S::kStagesUsed + 1) * S::kKeys);  // [64][2]: m, l of a warp's rows
-  int *const redo = reinterpret_cast<int *>(stats + 128);                           // [64]
+  float *const stats = reinterpret_cast<float *>(places + (S::kStagesUsed + 1) * S::kKeys);  // [warp][16][2]: m, l of a warp's rows
+  int *const redo = reinterpret_cast<int *>(stats + S::kWarps * 32);                  // [64]
   int *const missing = redo + 64;                                                    // [stage + 1]: a key of the tile has no page
-  long long *const scan = reinterpret_cast<long long *>(stats);                      // [4] (before the first tile)
+  long long *const scan = reinterpret_cast<long long *>(stats);                      // [warp] (before the first tile)
   __shared__ long long sh_first;
   __shared__ int sh_request;
   const uint32_t data = smem_u32(data_ptr);
@@ -152,7 +154,9 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) scan[warp] = total;
   __syncthreads();
-  total = scan[0] + scan[1] + scan[2] + scan[3];
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < S::kWarps; ++w) total += scan[w];
   const long long share = (total + gridDim.x - 1) / gridDim.x;
   long long unit = min(total, share * blockIdx.x);
   const long long end = min(total, unit + share);
@@ -176,7 +180,8 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
       if (blockIdx.x == 0) a.first[r] = before;
       if (unit >= before && unit < before + own) { sh_request = r; sh_first = before; }
     }
-    passed += scan[0] + scan[1] + scan[2] + scan[3];
+#pragma unroll
+    for (int w = 0; w < S::kWarps; ++w) passed += scan[w];
     __syncthreads();
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.first[a.requests] = total;
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
     const int rt = (int)(in / key_tiles % row_tiles), kv = (int)(in / key_tiles / row_tiles), row_base = rt * S::kRows;
 
     // ---- queries of the row tile (row = token * group + head of the group), features beyond D zero
-    uint8_t *const q_ptr = S::kQInStage ? data_ptr + (tile0 + 2) % S::kStagesUsed * S::kStage : smem;
+    uint8_t *const q_ptr = S::kQInStage ? data_ptr + (tile0 + 2) % 3 * S::kStage : smem;
     const uint32_t q_tile = smem_u32(q_ptr);
     __syncthreads();
     for (int i = threadIdx.x; i < S::kRows * F::kChunks; i += kThreads) {
@@ -213,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
     if (threadIdx.x <= S::kStagesUsed) missing[threadIdx.x] = 0;
     __syncthreads();
 
-    // ---- the pipeline: places of tile i + 3, copies of tile i + 2, products of tile i
+    // ---- the pipeline of three (two) stages: places of tile i + 3 (i + 2), copies of tile i + 2 (i + 1), products of tile i
     auto find = [&](int tile) {
       const int slot = tile % (S::kStagesUsed + 1);
       for (int i = threadIdx.x; i < S::kKeys; i += kThreads) {
@@ -279,16 +284,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
       const int key_base = tile * S::kKeys + wk * S::kWarpKeys;
       const bool open = tile * S::kKeys + S::kKeys <= x.context && !holes;  // every key is seen by every row
       flash_step<F, DP, S::kGroups>(run, q, q_tile, 16 * wr, k_tile, k_tile + S::kTileK, wk * S::kWarpKeys, [&](float (&s)[S::kGroups][4]) {
-#pragma unroll
-        for (int n = 0; n < S::kGroups; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] *= a.cap.scale;
-        if (a.cap.cap > 0.0f) {
-#pragma unroll
-          for (int n = 0; n < S::kGroups; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = a.cap.cap * tanh_of<sizeof(T) == 4>(s[n][i]);
-        }
+        cap_scores<sizeof(T) == 4>(a.cap, s);
         if (open) {
           if (a.slopes) {
 #pragma unroll
@@ -324,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
     for (int h = 0; h < 2; ++h) {
       run.l[h] += __shfl_xor_sync(0xffffffffu, run.l[h], 1);
       run.l[h] += __shfl_xor_sync(0xffffffffu, run.l[h], 2);
-      const int row = warp * 16 + g + 8 * h;  // = (wk * WR + wr) * 16 + ...
+      const int row = warp * 16 + g + 8 * h;  // = (wk * WR + wr) * 16 + g + 8 h
       if (t == 0) { stats[2 * row] = run.m[h]; stats[2 * row + 1] = run.l[h]; }
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n)
@@ -360,7 +356,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
       if (d == 0 && !whole) { part[row * (DP + 2) + DP] = m; part[row * (DP + 2) + DP + 1] = l; }
     }
     __syncthreads();
-    for (int row = warp; row < n_rows; row += 4) {
+    for (int row = warp; row < n_rows; row += S::kWarps) {
       if (!redo[row]) continue;
       const int gr = row_base + row;
       float *ctx = merge + row * (DP + 4);
@@ -376,13 +372,13 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
 
 // Rows whose keys several CTAs had: their parts in the order of the keys.  One warp per row (token, head).
 template <typename T, int DP, int WR>
-__global__ void __launch_bounds__(kThreads) attention_tree_join_kernel(const __grid_constant__ TreeArgs a, int ctas) {
+__global__ void __launch_bounds__(kJoinThreads) attention_tree_join_kernel(const __grid_constant__ TreeArgs a, int ctas) {
   using S = Shape<T, DP, WR>;
   pdl_prologue();
   const int lane = threadIdx.x & 31;
-  const int64_t rows = a.tokens * a.heads, step = (int64_t)gridDim.x * (kThreads / 32);
+  const int64_t rows = a.tokens * a.heads, step = (int64_t)gridDim.x * (kJoinThreads / 32);
   const long long total = a.first[a.requests], share = (total + ctas - 1) / ctas;
-  for (int64_t row = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); row < rows; row += step) {
+  for (int64_t row = (int64_t)blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5); row < rows; row += step) {
     const int token = (int)(row / a.heads), head = (int)(row % a.heads), kv = head / a.group;
     // the request that the token belongs to (none: the row stays as it is).  Ranges may be anything, so all are asked.
     for (int r0 = 0; r0 < a.requests; r0 += 32) {
@@ -426,7 +422,7 @@ __global__ void __launch_bounds__(kThreads) attention_tree_join_kernel(const __g
   }
 }
 
-// CTAs: two per SM, what three stages leave room for.
+// CTAs: two per SM, what shared memory leaves room for.
 constexpr int kCtas = 2 * kSms;
 
 // Rows of a tile by the average a request has: a wider tile reads the keys once for more rows, a narrower one has more warps
@@ -445,8 +441,8 @@ template <typename T, int DP, int WR> int launch(const TreeArgs &a, cudaStream_t
     FML_CUDA(cudaFuncSetAttribute(attention_tree_kernel<T, DP, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kBytes));
     attr_set[dev & 63] = true;
   }
-  FML_LAUNCH((attention_tree_kernel<T, DP, WR>), kCtas, kThreads, S::kBytes, s, a);
-  FML_LAUNCH((attention_tree_join_kernel<T, DP, WR>), grid_for(a.tokens * a.heads, kThreads / 32, 4 * kSms), kThreads, 0, s, a, kCtas);
+  FML_LAUNCH((attention_tree_kernel<T, DP, WR>), kCtas, S::kThreads, S::kBytes, s, a);
+  FML_LAUNCH((attention_tree_join_kernel<T, DP, WR>), grid_for(a.tokens * a.heads, kJoinThreads / 32, 4 * kSms), kJoinThreads, 0, s, a, kCtas);
   return FML_OK;
 }
 template <typename T, int DP> int launch(const TreeArgs &a, int warps, cudaStream_t s) {

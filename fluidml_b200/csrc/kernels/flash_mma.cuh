@@ -57,18 +57,21 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 
 // Tiles in shared memory and products with them.  DP: the head size the tiles are laid out for (features from the real one on
 // are zeros).  at(row, chunk): byte offset of 16 bytes of a row of a K (or Q) tile; at_v: of a V tile.
-template <typename T, int DP> struct Flash {
+// HELD (16-bit types): the queries stay in registers; else they are read again for every tile, which leaves room for twice the
+// warps.
+template <typename T, int DP, bool HELD> struct Flash {
   static constexpr int kChunk = 8, kChunks = DP / 8, kPitch = DP * 2, kPitchV = DP * 2;
-  struct Q { uint32_t r[DP / 16][4]; };
+  struct Q { uint32_t r[HELD ? DP / 16 : 1][4]; };
   // the 16-byte chunks of a row are permuted by its index: a matrix load of 8 rows meets 8 different bank groups
   __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((chunk ^ (row & 7)) << 4)); }
   __device__ __forceinline__ static uint32_t at_v(int row, int chunk) { return at(row, chunk); }
   __device__ __forceinline__ static void load_q(Q &q, uint32_t tile, int row0) {
     const int lane = threadIdx.x & 31;
+    if (HELD)
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) ldmatrix4(tile + at(row0 + (lane & 15), 2 * k + (lane >> 4)), q.r[k]);
+      for (int k = 0; k < DP / 16; ++k) ldmatrix4(tile + at(row0 + (lane & 15), 2 * k + (lane >> 4)), q.r[HELD ? k : 0]);
   }
-  template <int NT> __device__ __forceinline__ static void scores(float (&s)[NT][4], const Q &q, uint32_t, int, uint32_t tile, int key0) {
+  template <int NT> __device__ __forceinline__ static void scores(float (&s)[NT][4], const Q &q, uint32_t q_tile, int row0, uint32_t tile, int key0) {
     static_assert(NT % 2 == 0, "two groups of eight keys per matrix load");
     const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -77,17 +80,25 @@ template <typename T, int DP> struct Flash {
       for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
+      uint32_t a[4];
+      if (!HELD) ldmatrix4(q_tile + at(row0 + (lane & 15), 2 * k + (lane >> 4)), a);
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
         uint32_t b[4];
         ldmatrix4(tile + at(key0 + n * 8 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)), b);
-        mma16<T>(s[n], q.r[k], b[0], b[1]);
-        mma16<T>(s[n + 1], q.r[k], b[2], b[3]);
+        mma16<T>(s[n], HELD ? q.r[HELD ? k : 0] : a, b[0], b[1]);
+        mma16<T>(s[n + 1], HELD ? q.r[HELD ? k : 0] : a, b[2], b[3]);
       }
     }
   }
-  template <int NT> __device__ __forceinline__ static void context(float (&o)[DP / 8][4], const float (&p)[NT][4], uint32_t tile, int key0) {
+  // o = o * keep + p v
+  template <int NT>
+  __device__ __forceinline__ static void context(float (&o)[DP / 8][4], const float (&keep)[2], const float (&p)[NT][4], uint32_t tile, int key0) {
     const int lane = threadIdx.x & 31;
+    if (__any_sync(0xffffffffu, keep[0] != 1.0f || keep[1] != 1.0f)) {  // (most tiles leave the maximum as it is)
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) { o[n][0] *= keep[0]; o[n][1] *= keep[0]; o[n][2] *= keep[1]; o[n][3] *= keep[1]; }
+    }
 #pragma unroll
     for (int k = 0; k < NT / 2; ++k) {
       const uint32_t a[4] = {pack2<T>(p[2 * k][0], p[2 * k][1]), pack2<T>(p[2 * k][2], p[2 * k][3]), pack2<T>(p[2 * k + 1][0], p[2 * k + 1][1]),
@@ -103,7 +114,7 @@ template <typename T, int DP> struct Flash {
   }
 };
 
-template <int DP> struct Flash<float, DP> {
+template <int DP, bool HELD> struct Flash<float, DP, HELD> {
   // rows are padded so that the loads below meet every bank once: K by pairs of features, V by single ones
   static constexpr int kChunk = 4, kChunks = DP / 4, kPitch = (DP + 8) * 4, kPitchV = (DP + 4) * 4;
   struct Q {};  // (hi and lo of 16 x DP queries would fill the registers: read again for every tile)
@@ -149,24 +160,37 @@ template <int DP> struct Flash<float, DP> {
       }
     }
   }
-  template <int NT> __device__ __forceinline__ static void context(float (&o)[DP / 8][4], const float (&p)[NT][4], uint32_t tile, int key0) {
+  // o = o * keep + p v.  A tile's (half a tile's) products are summed apart and added in one rounded step: the tensor cores cut
+  // what they add to an accumulator, and one accumulator over all keys was off by six times as much.
+  template <int NT>
+  __device__ __forceinline__ static void context(float (&o)[DP / 8][4], const float (&keep)[2], const float (&p)[NT][4], uint32_t tile, int key0) {
+    constexpr int kPart = NT < 4 ? NT : 4;
     const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
     const uint32_t va = tile + (uint32_t)((key0 + 2 * t) * kPitchV + g * 4);
 #pragma unroll
-    for (int k = 0; k < NT; ++k) {
-      uint32_t hi[4], lo[4];
-      split_tf32(p[k][0], hi[0], lo[0]);
-      split_tf32(p[k][2], hi[1], lo[1]);
-      split_tf32(p[k][1], hi[2], lo[2]);
-      split_tf32(p[k][3], hi[3], lo[3]);
+    for (int k0 = 0; k0 < NT; k0 += kPart) {
+      uint32_t hi[kPart][4], lo[kPart][4];
+#pragma unroll
+      for (int k = 0; k < kPart; ++k) {
+        split_tf32(p[k0 + k][0], hi[k][0], lo[k][0]);
+        split_tf32(p[k0 + k][2], hi[k][1], lo[k][1]);
+        split_tf32(p[k0 + k][1], hi[k][2], lo[k][2]);
+        split_tf32(p[k0 + k][3], hi[k][3], lo[k][3]);
+      }
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n) {
-        uint32_t bh[2], bl[2];
-        split_tf32(one(va + k * 8 * kPitchV + n * 32), bh[0], bl[0]);
-        split_tf32(one(va + k * 8 * kPitchV + n * 32 + kPitchV), bh[1], bl[1]);
-        mma8_tf32(o[n], lo, bh[0], bh[1]);
-        mma8_tf32(o[n], hi, bl[0], bl[1]);
-        mma8_tf32(o[n], hi, bh[0], bh[1]);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kPart; ++k) {
+          uint32_t bh[2], bl[2];
+          split_tf32(one(va + (k0 + k) * 8 * kPitchV + n * 32), bh[0], bl[0]);
+          split_tf32(one(va + (k0 + k) * 8 * kPitchV + n * 32 + kPitchV), bh[1], bl[1]);
+          mma8_tf32(sum, lo[k], bh[0], bh[1]);
+          mma8_tf32(sum, hi[k], bl[0], bl[1]);
+          mma8_tf32(sum, hi[k], bh[0], bh[1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = k0 == 0 ? fmaf(o[n][i], keep[i >> 1], sum[i]) : o[n][i] + sum[i];
       }
     }
   }
@@ -192,6 +216,7 @@ __device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &
   float s[NT][4];
   F::template scores<NT>(s, q, q_tile, row0, k_tile, key0);
   shape(s);
+  float keeps[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     float m = r.m[h];
@@ -200,7 +225,7 @@ __device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const float base = m == -INFINITY ? 0.0f : m;  // (no key so far: every p below is 2^-infinity)
-    const float keep = ex2_approx(r.m[h] - base);
+    const float keep = r.m[h] == m ? 1.0f : ex2_approx(r.m[h] - base);
     r.m[h] = m;
     float sum = 0.0f;
 #pragma unroll
@@ -210,10 +235,9 @@ __device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &
       sum += s[n][2 * h] + s[n][2 * h + 1];
     }
     r.l[h] = r.l[h] * keep + sum;  // (this thread's keys: the four lanes of a row are added up at the end)
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n) { r.o[n][2 * h] *= keep; r.o[n][2 * h + 1] *= keep; }
+    keeps[h] = keep;
   }
-  F::template context<NT>(r.o, s, v_tile, key0);
+  F::template context<NT>(r.o, keeps, s, v_tile, key0);
 }
 
 // cap * tanh(s / cap) in units of ln 2, s = x * inv_divisor.
@@ -231,6 +255,41 @@ template <bool EXACT> __device__ __forceinline__ float tanh_of(float x) {
   if (EXACT) return tanhf(x);
   // 1 - 2 / (e^2x + 1): 1e-7 of the whole, where 16-bit weights carry 2^-9 and more
   return 1.0f - __fdividef(2.0f, ex2_approx(x * (2.0f * kLog2e)) + 1.0f);
+}
+// Products -> scores in units of ln 2, bias and mask apart.
+template <bool EXACT, int NT> __device__ __forceinline__ void cap_scores(const Cap &cap, float (&s)[NT][4]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] *= cap.scale;
+  if (!(cap.cap > 0.0f)) return;
+  float far = 0.0f;
+  if (!EXACT) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) far = fmaxf(far, fabsf(s[n][i]));
+  }
+  if (!EXACT && __all_sync(0xffffffffu, far <= 1.0f)) {
+    // tanh(x) = x P(x^2) on [-1, 1]: least squares reweighted to the smallest largest error, 2.4e-7
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = s[n][i], u = x * x;
+        float p = fmaf(u, -0.00283947f, 0.01611418f);
+        p = fmaf(u, p, -0.05097286f);
+        p = fmaf(u, p, 0.13253525f);
+        p = fmaf(u, p, -0.33324004f);
+        p = fmaf(u, p, 0.99999685f);
+        s[n][i] = p * (x * cap.cap);
+      }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = cap.cap * tanh_of<EXACT>(s[n][i]);
+  }
 }
 
 }  // namespace fml
