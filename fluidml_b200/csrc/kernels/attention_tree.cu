@@ -26,7 +26,8 @@ struct TreeArgs {
   int64_t k_page, k_pos, k_head, v_page, v_pos, v_head;
   int64_t table_r, table_c, context_s, start_s, tree_s, slopes_s;
   int64_t pages, tokens;
-  int requests, columns, page, heads, kv_heads, group, D;
+  int requests, columns, page, heads, kv_heads, group, D, q_vec;
+  int alike;  // pages and positions of K and V lie alike: places are element offsets, else page << 32 | position
   Cap cap;
   float *partial;       // [CTA][2][rows of a tile][DP + 2]
   long long *first;     // [requests + 1]: first unit of a request, then all units
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
   using F = typename S::F;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *const data_ptr = smem + (S::kQInStage ? 0 : S::kQ);
-  long long *const places = reinterpret_cast<long long *>(data_ptr + S::kData);   // [stage + 1][key]: page << 32 | position, -1 none
+  long long *const places = reinterpret_cast<long long *>(data_ptr + S::kData);   // [stage + 1][key]: see a.alike; -1 none
   float *const stats = reinterpret_cast<float *>(places + (S::kStagesUsed + 1) * S::kKeys);  // [warp][16][2]: m, l of a warp's rows
   int *const redo = reinterpret_cast<int *>(stats + S::kWarps * 32);                  // [64]
   int *const missing = redo + 64;                                                    // [stage + 1]: a key of the tile has no page
@@ -147,41 +148,49 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
   const int wr = warp % WR, wk = warp / WR;
   pdl_prologue();
 
-  // ---- this CTA's part of the line
-  long long total = 0;
-  for (int r = threadIdx.x; r < a.requests; r += kThreads) total += units_of<S::kRows, S::kKeys>(a, request_of(a, r, blockIdx.x == 0));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) scan[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < S::kWarps; ++w) total += scan[w];
-  const long long share = (total + gridDim.x - 1) / gridDim.x;
-  long long unit = min(total, share * blockIdx.x);
-  const long long end = min(total, unit + share);
-  if (threadIdx.x == 0) sh_request = -1;
-  __syncthreads();
-  long long passed = 0;  // units of the requests before this round of kThreads
-  for (int r0 = 0; r0 < a.requests; r0 += kThreads) {
+  // ---- this CTA's part of the line: all units are counted (requests in rounds of kThreads), then the part's first is looked for
+  // (in the last round's counts first: few requests are read once)
+  long long passed = 0, own = 0, before = 0;
+  int r0 = 0;
+  auto count = [&](bool report) {  // units of request r0 + thread, of those before it, and of all up to this round's end
     const int r = r0 + threadIdx.x;
-    const long long own = r < a.requests ? units_of<S::kRows, S::kKeys>(a, request_of(a, r, false)) : 0;
+    own = r < a.requests ? units_of<S::kRows, S::kKeys>(a, request_of(a, r, report)) : 0;
     long long run = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long up = __shfl_up_sync(0xffffffffu, run, o);
       if (lane >= o) run += up;
     }
+    __syncthreads();
     if (lane == 31) scan[warp] = run;
     __syncthreads();
-    long long before = passed + run - own;
-    for (int w = 0; w < warp; ++w) before += scan[w];
-    if (r < a.requests) {
-      if (blockIdx.x == 0) a.first[r] = before;
-      if (unit >= before && unit < before + own) { sh_request = r; sh_first = before; }
-    }
+    before = passed + run - own;
 #pragma unroll
-    for (int w = 0; w < S::kWarps; ++w) passed += scan[w];
+    for (int w = 0; w < S::kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      passed += scan[w];
+    }
+  };
+  if (threadIdx.x == 0) sh_request = -1;
+  for (;; r0 += kThreads) {
+    count(blockIdx.x == 0);
+    if (blockIdx.x == 0 && r0 + threadIdx.x < a.requests) a.first[r0 + threadIdx.x] = before;
+    if (r0 + kThreads >= a.requests) break;
+  }
+  const long long total = passed, share = (total + gridDim.x - 1) / gridDim.x;
+  long long unit = min(total, share * blockIdx.x);
+  const long long end = min(total, unit + share);
+  auto look = [&]() {
+    if (unit >= before && unit < before + own) { sh_request = r0 + threadIdx.x; sh_first = before; }
+  };
+  look();
+  __syncthreads();
+  if (a.requests > kThreads) {
+    passed = 0;
+    for (r0 = 0; r0 + kThreads < a.requests; r0 += kThreads) {
+      count(false);
+      look();
+    }
     __syncthreads();
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.first[a.requests] = total;
@@ -205,14 +214,20 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
     __syncthreads();
     for (int i = threadIdx.x; i < S::kRows * F::kChunks; i += kThreads) {
       const int row = i / F::kChunks, c = i % F::kChunks, gr = row_base + row;
-      alignas(16) T e[F::kChunk];
       const T *src = static_cast<const T *>(a.q) + (int64_t)(x.start + gr / a.group) * a.q_t + (int64_t)(kv * a.group + gr % a.group) * a.q_h;
+      uint4 e = make_uint4(0u, 0u, 0u, 0u);
+      if (a.q_vec) {
+        if (gr < rows && c * F::kChunk < a.D) e = *reinterpret_cast<const uint4 *>(src + c * F::kChunk);
+      } else {
+        alignas(16) T x[F::kChunk];
 #pragma unroll
-      for (int b = 0; b < F::kChunk; ++b) {
-        const int d = c * F::kChunk + b;
-        e[b] = gr < rows && d < a.D ? src[d * a.q_d] : from_f32<T>(0.0f);
+        for (int b = 0; b < F::kChunk; ++b) {
+          const int d = c * F::kChunk + b;
+          x[b] = gr < rows && d < a.D ? src[d * a.q_d] : from_f32<T>(0.0f);
+        }
+        memcpy(&e, x, 16);
       }
-      *reinterpret_cast<uint4 *>(q_ptr + F::at(row, c)) = *reinterpret_cast<const uint4 *>(e);
+      *reinterpret_cast<uint4 *>(q_ptr + F::at(row, c)) = e;
     }
     if (threadIdx.x < 64) redo[threadIdx.x] = 0;
     if (threadIdx.x <= S::kStagesUsed) missing[threadIdx.x] = 0;
@@ -225,26 +240,35 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
         const int key = tile * S::kKeys + i;
         long long w = -1;
         if (key < keys) {
-          const int64_t page = page_of(a, r, key);
-          if (page >= 0) w = page << 32 | (key % a.page);
+          const int64_t page = page_of(a, r, key), pos = key % a.page;
+          if (page >= 0) w = a.alike ? page * a.k_page + pos * a.k_pos : page << 32 | pos;
           else { missing[slot] = 1; atomicOr(a.status, kStatusIndexRange); }
         }
         places[slot * S::kKeys + i] = w;
       }
     };
     auto fetch = [&](int tile) {
+      // a thread has one chunk of rows kThreads / kChunks apart
+      static_assert(kThreads % F::kChunks == 0, "");
       const uint32_t dst = data + (uint32_t)(tile % S::kStagesUsed) * S::kStage;
-      const long long *place = places + tile % (S::kStagesUsed + 1) * S::kKeys;
+      const int c = threadIdx.x % F::kChunks;
+      const long long *place = places + tile % (S::kStagesUsed + 1) * S::kKeys + threadIdx.x / F::kChunks;
+      const bool inside = c * F::kChunk < a.D;
+      const T *const k = static_cast<const T *>(a.k) + kv * a.k_head + (inside ? c * F::kChunk : 0);
+      const T *const v = static_cast<const T *>(a.v) + kv * a.v_head + (inside ? c * F::kChunk : 0);
 #pragma unroll
       for (int i = 0; i < S::kKeys * F::kChunks / kThreads; ++i) {
-        const int e = threadIdx.x + i * kThreads, row = e / F::kChunks, c = e % F::kChunks;
-        const long long w = place[row];
-        const bool valid = w >= 0 && c * F::kChunk < a.D;
-        const int64_t page = valid ? w >> 32 : 0, pos = valid ? w & 0xffffffff : 0;
-        const T *k = static_cast<const T *>(a.k) + page * a.k_page + pos * a.k_pos + kv * a.k_head + (valid ? c * F::kChunk : 0);
-        const T *v = static_cast<const T *>(a.v) + page * a.v_page + pos * a.v_pos + kv * a.v_head + (valid ? c * F::kChunk : 0);
-        cp_async16(dst + F::at(row, c), k, valid);
-        cp_async16(dst + S::kTileK + F::at_v(row, c), v, valid);
+        const int row = threadIdx.x / F::kChunks + i * (kThreads / F::kChunks);
+        const long long w = place[i * (kThreads / F::kChunks)];
+        const bool valid = inside && w >= 0;
+        int64_t kw = valid ? w : 0, vw = kw;
+        if (!a.alike) {
+          const int64_t page = kw >> 32, pos = kw & 0xffffffff;
+          kw = page * a.k_page + pos * a.k_pos;
+          vw = page * a.v_page + pos * a.v_pos;
+        }
+        cp_async16(dst + F::at(row, c), k + kw, valid);
+        cp_async16(dst + S::kTileK + F::at_v(row, c), v + vw, valid);
       }
     };
     for (int i = tile0; i < min(tile1, tile0 + S::kStagesUsed); ++i) find(i);
@@ -283,6 +307,7 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
       const uint32_t k_tile = data + (uint32_t)(tile % S::kStagesUsed) * S::kStage;
       const int key_base = tile * S::kKeys + wk * S::kWarpKeys;
       const bool open = tile * S::kKeys + S::kKeys <= x.context && !holes;  // every key is seen by every row
+      if (row_base + 16 * wr < rows)  // (a request's last tile may leave warps without rows)
       flash_step<F, DP, S::kGroups>(run, q, q_tile, 16 * wr, k_tile, k_tile + S::kTileK, wk * S::kWarpKeys, [&](float (&s)[S::kGroups][4]) {
         cap_scores<sizeof(T) == 4>(a.cap, s);
         if (open) {
@@ -399,18 +424,34 @@ __global__ void __launch_bounds__(kJoinThreads) attention_tree_join_kernel(const
         if (c0 == c1) continue;
         auto part = [&](int c) { return a.partial + ((int64_t)c * 2 + (c == c0 ? 1 : 0)) * S::kPartial + at * (DP + 2); };
         // (c0's stretch begins inside it unless it begins at its very first unit, which is a slot 1 as well: its tile0 is 0)
+        // 32 parts' maxima and sums at a time, one to a lane; then their contexts, whose loads do not wait for one another
         float m = -INFINITY, l = 0.0f, o[DP / 32];
-        for (int c = c0; c <= c1; ++c) m = fmaxf(m, part(c)[DP]);
-        const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) o[i] = 0.0f;
-        for (int c = c0; c <= c1; ++c) {
-          const float *p = part(c);
-          const float w = p[DP + 1] * ex2_approx(p[DP] - base);
-          l += w;
-          if (p[DP + 1] != 0.0f) {
+        for (int c = c0; c <= c1; c += 32) {
+          const int n = min(32, c1 - c + 1);
+          const float pm = lane < n ? part(c + lane)[DP] : -INFINITY, pl = lane < n ? part(c + lane)[DP + 1] : 0.0f;
+          float top = pm;
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) if (lane + 32 * i < a.D) o[i] += w * p[lane + 32 * i];
+          for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          top = fmaxf(top, m);
+          const float base = top == -INFINITY ? 0.0f : top, keep = ex2_approx(m - base), w = pl == 0.0f ? 0.0f : pl * ex2_approx(pm - base);
+          float sum = w;
+#pragma unroll
+          for (int k = 16; k; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+          m = top;
+          l = l * keep + sum;
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i) o[i] *= keep;
+#pragma unroll 4
+          for (int k = 0; k < n; ++k) {
+            const float *p = part(c + k);
+            const float f = __shfl_sync(0xffffffffu, w, k);
+            float v[DP / 32];
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) v[i] = lane + 32 * i < a.D ? p[lane + 32 * i] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) o[i] += f == 0.0f ? 0.0f : f * v[i];
           }
         }
         T *out = static_cast<T *>(a.out) + (int64_t)token * a.o_t + (int64_t)head * a.o_h;
@@ -513,9 +554,11 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   a.tree = tree ? static_cast<const int64_t *>(tree->data) : nullptr;
   a.slopes = slopes ? static_cast<const float *>(slopes->data) : nullptr;
   a.q_t = q->stride[0]; a.q_h = q->stride[1]; a.q_d = q->stride[2];
+  a.q_vec = a.q_d == 1 && aligned16(q->data) && (tokens == 1 || a.q_t % per16 == 0) && (heads == 1 || a.q_h % per16 == 0);
   a.o_t = out->stride[0]; a.o_h = out->stride[1]; a.o_d = out->stride[2];
   a.k_page = k_cache->stride[0]; a.k_pos = k_cache->stride[1]; a.k_head = k_cache->stride[2];
   a.v_page = v_cache->stride[0]; a.v_pos = v_cache->stride[1]; a.v_head = v_cache->stride[2];
+  a.alike = a.k_page == a.v_page && a.k_pos == a.v_pos && a.k_page >= 0 && a.k_pos >= 0;
   a.table_r = block_table->stride[0]; a.table_c = block_table->stride[1];
   a.context_s = context->stride[0]; a.start_s = query_start->stride[0];
   a.tree_s = tree ? tree->stride[0] : 0; a.slopes_s = slopes ? slopes->stride[0] : 0;
