@@ -26,8 +26,8 @@ struct TreeArgs {
   int64_t k_page, k_pos, k_head, v_page, v_pos, v_head;
   int64_t table_r, table_c, context_s, start_s, tree_s, slopes_s;
   int64_t pages, tokens;
-  int requests, columns, page, heads, kv_heads, group, D, q_vec;
-  int alike;  // pages and positions of K and V lie alike: places are element offsets, else page << 32 | position
+  int requests, columns, page, heads, kv_heads, group, D, q_vec, page_shift;  // page_shift: -1 when the page size is no power of two
+  int alike;  // pages and positions of K and V lie alike: places are byte offsets, else page << 32 | position
   Cap cap;
   float *partial;       // [CTA][2][rows of a tile][DP + 2]
   long long *first;     // [requests + 1]: first unit of a request, then all units
@@ -240,35 +240,40 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
         const int key = tile * S::kKeys + i;
         long long w = -1;
         if (key < keys) {
-          const int64_t page = page_of(a, r, key), pos = key % a.page;
-          if (page >= 0) w = a.alike ? page * a.k_page + pos * a.k_pos : page << 32 | pos;
+          const int at = a.page_shift >= 0 ? key >> a.page_shift : key / a.page, pos = key - at * a.page;
+          int64_t page = a.table[r * a.table_r + at * a.table_c];
+          if (page >= a.pages) page = -1;
+          if (page >= 0) w = a.alike ? (page * a.k_page + pos * a.k_pos) * (int)sizeof(T) : page << 32 | pos;
           else { missing[slot] = 1; atomicOr(a.status, kStatusIndexRange); }
         }
         places[slot * S::kKeys + i] = w;
       }
     };
     auto fetch = [&](int tile) {
-      // a thread has one chunk of rows kThreads / kChunks apart
-      static_assert(kThreads % F::kChunks == 0, "");
+      // Eight threads copy 128 bytes of a row at a time: a row's address is formed once for all of its parts.
+      constexpr int kParts = F::kChunks / 8, kStep = kThreads / 8;
+      static_assert(F::kChunks % 8 == 0 && S::kKeys % kStep == 0, "");
       const uint32_t dst = data + (uint32_t)(tile % S::kStagesUsed) * S::kStage;
-      const int c = threadIdx.x % F::kChunks;
-      const long long *place = places + tile % (S::kStagesUsed + 1) * S::kKeys + threadIdx.x / F::kChunks;
-      const bool inside = c * F::kChunk < a.D;
-      const T *const k = static_cast<const T *>(a.k) + kv * a.k_head + (inside ? c * F::kChunk : 0);
-      const T *const v = static_cast<const T *>(a.v) + kv * a.v_head + (inside ? c * F::kChunk : 0);
+      const int c = threadIdx.x % 8, row0 = threadIdx.x / 8;
+      const long long *place = places + tile % (S::kStagesUsed + 1) * S::kKeys + row0;
+      const char *const k = static_cast<const char *>(a.k) + 16 * c + kv * a.k_head * (int)sizeof(T);
+      const char *const v = static_cast<const char *>(a.v) + 16 * c + kv * a.v_head * (int)sizeof(T);
 #pragma unroll
-      for (int i = 0; i < S::kKeys * F::kChunks / kThreads; ++i) {
-        const int row = threadIdx.x / F::kChunks + i * (kThreads / F::kChunks);
-        const long long w = place[i * (kThreads / F::kChunks)];
-        const bool valid = inside && w >= 0;
-        int64_t kw = valid ? w : 0, vw = kw;
+      for (int i = 0; i < S::kKeys / kStep; ++i) {
+        const long long w = place[i * kStep];
+        int64_t kw = w >= 0 ? w : 0, vw = kw;
         if (!a.alike) {
           const int64_t page = kw >> 32, pos = kw & 0xffffffff;
-          kw = page * a.k_page + pos * a.k_pos;
-          vw = page * a.v_page + pos * a.v_pos;
+          kw = (page * a.k_page + pos * a.k_pos) * (int)sizeof(T);
+          vw = (page * a.v_page + pos * a.v_pos) * (int)sizeof(T);
         }
-        cp_async16(dst + F::at(row, c), k + kw, valid);
-        cp_async16(dst + S::kTileK + F::at_v(row, c), v + vw, valid);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+          const bool valid = w >= 0 && (8 * part + c) * F::kChunk < a.D;
+          const int64_t off = valid ? 128 * part : -16 * c;  // (an address within the row for what is not read)
+          cp_async16(dst + F::at(row0 + i * kStep, 8 * part + c), k + kw + off, valid);
+          cp_async16(dst + S::kTileK + F::at_v(row0 + i * kStep, 8 * part + c), v + vw + off, valid);
+        }
       }
     };
     for (int i = tile0; i < min(tile1, tile0 + S::kStagesUsed); ++i) find(i);
@@ -564,6 +569,9 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   a.tree_s = tree ? tree->stride[0] : 0; a.slopes_s = slopes ? slopes->stride[0] : 0;
   a.pages = pages; a.tokens = tokens;
   a.requests = (int)requests; a.columns = (int)columns; a.page = (int)page;
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (page == (1ll << i)) a.page_shift = i;
   a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.group = (int)(heads / kv_heads); a.D = (int)d;
   a.cap = Cap::make(rules->divisor, rules->cap);
   a.first = static_cast<long long *>(workspace);

@@ -1,7 +1,7 @@
 // Attention on warp-wide matrix instructions, shared by attention_rules.cu and attention_tree.cu: a warp owns 16 rows, whose
 // queries, running maximum, sum and context stay in its registers, and takes keys and values from tiles in shared memory.
 //
-//   s = q k^T;  m' = max(m, s);  p = 2^(s - m');  l = l 2^(m - m') + sum p;  o = o 2^(m - m') + p v
+//   s = q k^T;  p = 2^(s - m);  l = l + sum p;  o = o + p v;  l and o times 2^(m - m') where m moves to m'
 //
 // 16-bit types: m16n8k16 with fp32 sums; p is rounded to the type (half a step of a weight, as the values carry), its sum is
 // not.  fp32: every operand is split into two TF32 numbers, hi + lo to 2^-22, and three products of four are kept.
@@ -60,10 +60,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 // HELD (16-bit types): the queries stay in registers; else they are read again for every tile, which leaves room for twice the
 // warps.
 template <typename T, int DP, bool HELD> struct Flash {
-  static constexpr int kChunk = 8, kChunks = DP / 8, kPitch = DP * 2, kPitchV = DP * 2;
+  static constexpr int kChunk = 8, kChunks = DP / 8, kPitch = DP * 2 + 16, kPitchV = kPitch;
   struct Q { uint32_t r[HELD ? DP / 16 : 1][4]; };
-  // the 16-byte chunks of a row are permuted by its index: a matrix load of 8 rows meets 8 different bank groups
-  __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + ((chunk ^ (row & 7)) << 4)); }
+  // rows are 16 bytes longer than their features: a matrix load of 8 rows meets 8 different bank groups
+  __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + (chunk << 4)); }
   __device__ __forceinline__ static uint32_t at_v(int row, int chunk) { return at(row, chunk); }
   __device__ __forceinline__ static void load_q(Q &q, uint32_t tile, int row0) {
     const int lane = threadIdx.x & 31;
@@ -198,7 +198,7 @@ template <int DP, bool HELD> struct Flash<float, DP, HELD> {
 
 // The two rows of a thread: lane / 4 and lane / 4 + 8 of the warp's 16.
 template <int DP> struct Running {
-  float o[DP / 8][4], m[2], l[2];  // m, and the scores, in units of ln 2; m is -infinity before the first visible key
+  float o[DP / 8][4], m[2], l[2];  // m (what p refers to), and the scores, in units of ln 2; -infinity before the first visible key
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n)
@@ -219,14 +219,18 @@ __device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &
   float keeps[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float m = r.m[h];
+    float m = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n) m = fmaxf(m, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+    for (int n = 1; n < NT; ++n) m = fmaxf(m, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const float base = m == -INFINITY ? 0.0f : m;  // (no key so far: every p below is 2^-infinity)
-    const float keep = r.m[h] == m ? 1.0f : ex2_approx(r.m[h] - base);
-    r.m[h] = m;
+    // the reference moves only for a score that exceeds it by more than 8: weights reach 2^8, and the context is seldom rescaled
+    float keep = 1.0f;
+    if (m > (r.m[h] == -INFINITY ? -3.402823466e38f : r.m[h] + 8.0f)) {
+      keep = ex2_approx(r.m[h] - m);
+      r.m[h] = m;
+    }
+    const float base = r.m[h] == -INFINITY ? 0.0f : r.m[h];  // (no key so far: every p below is 2^-infinity)
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
