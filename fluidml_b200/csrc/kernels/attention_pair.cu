@@ -21,6 +21,7 @@
 // this block's V): O is one accumulator.  O is rescaled, by a round trip through registers, only when a
 // block's maximum exceeds the reference m of a row by more than 4 in log2 or V's scale moves by more than 3:
 // the largest P of a row is then within 2^-3 .. 2^7, and what its pair leaves out is below 2^-22 of it.
+#include "attention_rules.cuh"
 #include "gemm_common.cuh"
 #include "pair_common.cuh"
 #include <algorithm>
@@ -34,7 +35,9 @@ constexpr int kRawStage = 2 * kKeys * kD * 4;    // K and V of a block, fp32: 32
 constexpr int kSplit = kKeys * kD * 4;           // hi and lo of K or V: 16 KiB
 constexpr int kHalfSplit = kSplit / 2;           // offset of lo
 constexpr uint32_t kColS = 0, kColO = 128, kColQ = 192;  // tensor memory: two score buffers (P over S), O, Q
-enum { kNoMask = 0, kKeyMask = 1, kFullMask = 2, kCausal = 3 };
+enum { kNoMask = 0, kKeyMask = 1, kFullMask = 2, kCausal = 3, kRules = 4 };
+constexpr int kMaxBlocks = 2048;  // of keys, with rules
+struct NoRules {};
 
 struct AttnPairArgs {
   int Sq, Sk, nb0;
@@ -42,14 +45,16 @@ struct AttnPairArgs {
   const float *mask;
   int64_t m_s[4], o_s[4];
   float *out;
-  float inv_divisor;
+  float inv_divisor, cap;
   int *status;
 };
 
-template <int MASK>
+// With rules (fml_attention_rules): the blocks of keys that some query of the tile sees are listed first, heads share keys and
+// values in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.
+template <int MASK, typename Rules>
 __global__ void __launch_bounds__(kThreads, 2)
 attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_v, const AttnPairArgs a) {
+                      const __grid_constant__ CUtensorMap map_v, const AttnPairArgs a, const __grid_constant__ Rules rules) {
   extern __shared__ __align__(1024) uint8_t smem[];
   // [ raw stage 0 | raw stage 1 | split K | split V | mask | barriers ]
   const uint32_t raw0 = smem_u32(smem), split_k = raw0 + 2 * kRawStage, split_v = split_k + kSplit;
@@ -66,7 +71,8 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const bool leader = elect_one();
-  const int q0 = blockIdx.x * kBM, h = blockIdx.y % a.nb0, b = blockIdx.y / a.nb0;
+  const int q0 = (MASK == kRules ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x) * kBM, h = blockIdx.y % a.nb0, b = blockIdx.y / a.nb0;
+  uint16_t *const list = reinterpret_cast<uint16_t *>(tmem_slot + 4);  // (rules) [block that is seen]: its index | TileView << 12
   int n_blocks = (a.Sk + kKeys - 1) / kKeys;
   if (MASK == kCausal) n_blocks = min(n_blocks, (q0 + kBM + kKeys - 1) / kKeys);  // keys beyond the tile's last row
 
@@ -94,6 +100,37 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
   // Only now may the next kernel start (tensor memory: see gemm_tc.cu).
   pdl_launch_dependents();
   pdl_wait();
+  int kv = h;
+  if constexpr (MASK == kRules) {
+    kv = h / rules.group;
+    const TileRange range = tile_range(rules, b, q0, min(q0 + kBM, a.Sq));
+    const int blocks = (range.last_key + kKeys - 1) / kKeys;
+    for (int i = warp; i < blocks; i += kThreads / 32) {
+      int view = tile_view(range, i * kKeys, kKeys);
+      if (rules.k_documents.p) {
+        int64_t low, high;
+        tile_documents(rules, b, i * kKeys, min(i * kKeys + kKeys, a.Sk), &low, &high);
+        view = document_view(view, range, low, high);
+      }
+      if (lane == 0) list[i] = (uint16_t)view;
+    }
+    __syncthreads();
+    if (warp == 0) {  // (a block's place is not behind its index, and 32 are read before they are written)
+      int n = 0;
+      for (int i0 = 0; i0 < blocks; i0 += 32) {
+        const int view = i0 + lane < blocks ? list[i0 + lane] : (int)kTileNone;
+        const unsigned seen = __ballot_sync(0xffffffffu, view != kTileNone);
+        __syncwarp();
+        if (view != kTileNone) list[n + __popc(seen & ((1u << lane) - 1u))] = (uint16_t)(i0 + lane | view << 12);
+        n += __popc(seen);
+        __syncwarp();
+      }
+      if (lane == 0) tmem_slot[2] = (uint32_t)n;
+    }
+    __syncthreads();
+    n_blocks = (int)tmem_slot[2];
+  }
+  auto block = [&](int j) { return MASK == kRules ? list[j] & 0xfff : j; };
 
   bool ok = true;
   if (warp == 0) {
@@ -114,8 +151,8 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           const uint32_t dst = raw0 + s * kRawStage, bar = bar_raw_full + 8u * s;
           mbar_expect_tx(bar, kRawStage);
           for (int i = 0; i < 2; ++i) {
-            tma_load_4d(dst + (uint32_t)i * (kKeys * 128), &map_k, bar, 32 * i, j * kKeys, a.k_h ? h : 0, a.k_b ? b : 0);
-            tma_load_4d(dst + (uint32_t)(2 + i) * (kKeys * 128), &map_v, bar, 32 * i, j * kKeys, a.v_h ? h : 0, a.v_b ? b : 0);
+            tma_load_4d(dst + (uint32_t)i * (kKeys * 128), &map_k, bar, 32 * i, block(j) * kKeys, a.k_h ? kv : 0, a.k_b ? b : 0);
+            tma_load_4d(dst + (uint32_t)(2 + i) * (kKeys * 128), &map_v, bar, 32 * i, block(j) * kKeys, a.v_h ? kv : 0, a.v_b ? b : 0);
           }
         }
         ++issued;
@@ -213,9 +250,13 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_q_ready);
     }
-    constexpr float kLog2e = 1.4426950408889634f;
     float m_ref = 0.0f, l = 0.0f;
     int ev_ref = 0, ev_min = 0;
+    RowRules rr;
+    if constexpr (MASK == kRules) {
+      rr = row_rules(rules, b, h, row_in);
+      rr.slope *= 1.0f / kLog2e;  // (scores are in natural units here)
+    }
     for (int j = 0; j < n_blocks && ok; ++j) {
       const uint32_t buf = (uint32_t)j & 1u;
       ok = mbar_wait_warp(bar_s + 8u * buf, (uint32_t)(j >> 1) & 1u, abort_flag);
@@ -223,12 +264,37 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       tc_fence_after();
       const int ev = exp_s[2 * buf + 1];
       const float f = a.inv_divisor * pow2(max(-126, min(126, -(e_q + exp_s[2 * buf]))));
-      const int key0 = j * kKeys;
+      const int key0 = block(j) * kKeys;
       float v[64];
       tmem_ld32(lane_addr + kColS + buf * 64u, v);
       tmem_ld32(lane_addr + kColS + buf * 64u + 32u, v + 32);
       float m_blk = -FLT_MAX;  // (finite, for blocks without a visible key)
-      if (MASK == kKeyMask) {
+      if constexpr (MASK == kRules) {
+        const int view = list[j] >> 12, last = rr.last - key0;
+        if (a.cap > 0.0f) {
+          const float g = f / a.cap;
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = a.cap * tanhf(v[i] * g);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] *= f;
+        }
+        if (rules.slopes) {
+          const float at = (float)(rr.at - key0);
+#pragma unroll
+          for (int i = 0; i < 64; ++i) v[i] = fmaf(-rr.slope, fabsf(at - (float)i), v[i]);
+        }
+        if (view != kTileAll) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= last) v[i] = -INFINITY;
+          if (view == kTileSome && rules.k_documents.p) {
+#pragma unroll
+            for (int i = 0; i < 64; ++i)
+              if (document_at(rules.k_documents, rules.k_documents_row, b, min(key0 + i, a.Sk - 1)) != rr.document) v[i] = -INFINITY;
+          }
+        }
+      } else if (MASK == kKeyMask) {
         const float *mk = mask_s + buf * kKeys;  // keys beyond the last one hold -infinity
 #pragma unroll
         for (int i = 0; i < 64; ++i) v[i] = fmaf(v[i], f, mk[i]);
@@ -295,10 +361,11 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (ok && lane == 0) mbar_arrive(bar_p_ready + 8u * buf);  // (two barriers: the softmax may be a block ahead of PV)
     }
     // ---- out = O / l
-    if (ok) ok = mbar_wait_warp(bar_pv, (uint32_t)(n_blocks - 1) & 1u, abort_flag);
+    if (ok && (MASK != kRules || n_blocks > 0)) ok = mbar_wait_warp(bar_pv, (uint32_t)(n_blocks - 1) & 1u, abort_flag);
     if (ok) {
       tc_fence_after();
-      const float inv = pow2(-ev_ref) / l;
+      const float inv = MASK == kRules && l == 0.0f ? 0.0f : pow2(-ev_ref) / l;
+      bool bad = false;
       float *dst = a.out + (int64_t)b * a.o_s[0] + (int64_t)h * a.o_s[1] + (int64_t)row_in * a.o_s[2];
       const bool vec = a.o_s[3] == 1 && (a.o_s[2] & 3) == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll
@@ -306,6 +373,16 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         float o[32];
         __syncwarp();
         tmem_ld32(lane_addr + kColO + (uint32_t)c, o);
+        if constexpr (MASK == kRules) {
+          if (n_blocks == 0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          }
+          float check = 0.0f;  // 0, or NaN from an infinity or NaN on
+#pragma unroll
+          for (int i = 0; i < 32; ++i) check = fmaf(o[i] * inv, 0.0f, check);
+          bad = bad || !(check == 0.0f);
+        }
         if (grow >= a.Sq) {
         } else if (vec) {
 #pragma unroll
@@ -314,6 +391,15 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) dst[(int64_t)(c + i) * a.o_s[3]] = o[i] * inv;
+        }
+      }
+      if constexpr (MASK == kRules) {
+        unsigned redo = __ballot_sync(0xffffffffu, bad && grow < a.Sq);
+        __syncwarp();
+        while (redo) {
+          const int which = __ffs(redo) - 1;
+          redo &= redo - 1;
+          redo_rules_row<float>(rules, b, h, q0 + q * 32 + which);
         }
       }
     }
@@ -429,7 +515,7 @@ int launch_attention_pair(int64_t nb1, int64_t nb0, int64_t Sq, int64_t Sk, cons
   AttnPairArgs a;
   a.Sq = (int)Sq; a.Sk = (int)Sk; a.nb0 = (int)nb0;
   for (int i = 0; i < 4; ++i) { a.m_s[i] = mask ? m_s[i] : 0; a.o_s[i] = o_s[i]; }
-  a.mask = mask; a.out = out; a.inv_divisor = 1.0f / divisor;
+  a.mask = mask; a.out = out; a.inv_divisor = 1.0f / divisor; a.cap = 0.0f;
   a.q_h = q_s[1] != 0; a.q_b = q_s[0] != 0; a.k_h = k_s[1] != 0; a.k_b = k_s[0] != 0; a.v_h = v_s[1] != 0; a.v_b = v_s[0] != 0;
   a.status = device_status_word();
   FML_REQUIRE(a.status, FML_CUDA_ERROR, "fml_attention: no device status word");
@@ -439,9 +525,9 @@ int launch_attention_pair(int64_t nb1, int64_t nb0, int64_t Sq, int64_t Sk, cons
   if (st == FML_OK) st = attention_map(&mv, v, Sk, v_s[2], nb0, v_s[1], nb1, v_s[0], kKeys);
   if (st != FML_OK) return st;
   const size_t smem = 2 * kRawStage + 2 * kSplit + 2 * kKeys * 4 + 4 * 4 + 8 * 4 + 15 * 8 + 16;
-  using KernelFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const AttnPairArgs);
-  static const KernelFn kernels[4] = {attention_pair_kernel<kNoMask>, attention_pair_kernel<kKeyMask>, attention_pair_kernel<kFullMask>,
-                                      attention_pair_kernel<kCausal>};
+  using KernelFn = void (*)(const CUtensorMap, const CUtensorMap, const CUtensorMap, const AttnPairArgs, const NoRules);
+  static const KernelFn kernels[4] = {attention_pair_kernel<kNoMask, NoRules>, attention_pair_kernel<kKeyMask, NoRules>,
+                                      attention_pair_kernel<kFullMask, NoRules>, attention_pair_kernel<kCausal, NoRules>};
   static bool attr_set[64] = {false};
   int dev = 0;
   FML_CUDA(cudaGetDevice(&dev));
@@ -451,7 +537,47 @@ int launch_attention_pair(int64_t nb1, int64_t nb0, int64_t Sq, int64_t Sk, cons
   }
   const int kind = causal ? kCausal : !mask ? kNoMask : m_s[2] == 0 ? kKeyMask : kFullMask;
   const dim3 grid((unsigned)((Sq + kBM - 1) / kBM), (unsigned)(nb0 * nb1));
-  FML_CUDA(launch_kernel(kernels[kind], grid, dim3(kThreads), smem, s, mq, mk, mv, a));
+  FML_CUDA(launch_kernel(kernels[kind], grid, dim3(kThreads), smem, s, mq, mk, mv, a, NoRules()));
+  return FML_OK;
+}
+
+// fml_attention_rules in fp32, head size 64, operands that tensor maps take.
+bool attention_rules_pair_eligible(const RulesArgs &r) {
+  if (r.D != kD || !r.q_vec || !r.k_vec || !r.v_vec || r.Sk < 1 || r.Sk > kMaxBlocks * kKeys || (int64_t)r.heads * r.batch > 65535) return false;
+  for (const int64_t *s : {r.q_s, r.k_s, r.v_s})
+    for (int i = 0; i < 3; ++i)
+      if (s[i] < 0 || s[i] >= (1ll << 37) || s[i] % 4 != 0 || (i == 2 && s[i] == 0)) return false;
+  return true;
+}
+
+int launch_attention_rules_pair(const RulesArgs &r, float divisor, float cap, cudaStream_t s) {
+  AttnPairArgs a;
+  memset(&a, 0, sizeof(a));
+  a.Sq = r.Sq; a.Sk = r.Sk; a.nb0 = r.heads;
+  for (int i = 0; i < 4; ++i) a.o_s[i] = r.o_s[i];
+  a.out = static_cast<float *>(r.out); a.inv_divisor = 1.0f / divisor; a.cap = cap;
+  const int64_t kv_heads = r.heads / r.group;
+  // (a dim of one row, head or batch takes any stride: the map is told none)
+  auto stride = [](int64_t s, int64_t n) { return n > 1 ? s : 0; };
+  const int64_t q_h = stride(r.q_s[1], r.heads), q_b = stride(r.q_s[0], r.batch), k_h = stride(r.k_s[1], kv_heads), k_b = stride(r.k_s[0], r.batch),
+                v_h = stride(r.v_s[1], kv_heads), v_b = stride(r.v_s[0], r.batch);
+  a.q_h = q_h != 0; a.q_b = q_b != 0; a.k_h = k_h != 0; a.k_b = k_b != 0; a.v_h = v_h != 0; a.v_b = v_b != 0;
+  a.status = r.status;
+  CUtensorMap mq, mk, mv;
+  int st = attention_map(&mq, static_cast<const float *>(r.q), r.Sq, r.Sq > 1 ? r.q_s[2] : kD, r.heads, q_h, r.batch, q_b, kBM);
+  if (st == FML_OK) st = attention_map(&mk, static_cast<const float *>(r.k), r.Sk, r.Sk > 1 ? r.k_s[2] : kD, kv_heads, k_h, r.batch, k_b, kKeys);
+  if (st == FML_OK) st = attention_map(&mv, static_cast<const float *>(r.v), r.Sk, r.Sk > 1 ? r.v_s[2] : kD, kv_heads, v_h, r.batch, v_b, kKeys);
+  if (st != FML_OK) return st;
+  const size_t smem = 2 * kRawStage + 2 * kSplit + 2 * kKeys * 4 + 4 * 4 + 8 * 4 + 15 * 8 + 16 + kMaxBlocks * 2;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  FML_CUDA(cudaGetDevice(&dev));
+  if (!attr_set[dev & 63]) {
+    FML_CUDA(cudaFuncSetAttribute(attention_pair_kernel<kRules, RulesArgs>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    attr_set[dev & 63] = true;
+  }
+  const dim3 grid((unsigned)((r.Sq + kBM - 1) / kBM), (unsigned)(r.heads * r.batch));
+  FML_CUDA(launch_kernel(attention_pair_kernel<kRules, RulesArgs>, grid, dim3(kThreads), smem, s, mq, mk, mv, a, r));
   return FML_OK;
 }
 

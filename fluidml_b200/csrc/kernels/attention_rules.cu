@@ -1,7 +1,7 @@
 // Attention over a prompt by rules (fml_attention_rules): capped scores, a bias by distance, documents, a prefix, grouped heads.
 //
 // Here: argument checks, the choice of the kernel, and the kernel on warp-wide matrix instructions, which takes fp32 and every
-// layout: a CTA has 64 (fp32: 128) queries of a head, 16 to a warp, and keys pass in tiles through two stages of shared memory.  Large
+// layout: a CTA has 64 queries of a head, 16 to a warp, and keys pass in tiles through two stages of shared memory.  Large
 // 16-bit problems run on the fifth-generation tensor cores (attention_rules_tc.cu).
 //
 // A tile of keys that no query of the CTA sees is not loaded: causal and prefix leave the tiles up to a last one, documents are
@@ -17,15 +17,15 @@ constexpr int kMaxTiles = 4096;
 
 template <typename T, int DP> struct Shape {
   using F = Flash<T, DP, true>;
-  // fp32 is bound by the instructions that split its operands: twice the warps share what is loaded
-  static constexpr int kThreads = sizeof(T) == 4 ? 256 : 128, kRows = kThreads / 2;
+  // (fp32 in tiles of 128 rows took as long at 4 x 16 x 512 x 64, and 23 us instead of 18 at 16 x 77)
+  static constexpr int kThreads = 128, kRows = 64;
   static constexpr int kKeys = sizeof(T) == 2 ? 64 : DP == 64 ? 64 : 32, kGroups = kKeys / 8;
   static constexpr int kTileK = kKeys * F::kPitch, kTileV = kKeys * F::kPitchV, kStage = kTileK + kTileV, kQ = kRows * F::kPitch;
   static constexpr size_t kBytes = kQ + 2 * kStage + kMaxTiles;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(Shape<T, DP>::kThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) attention_rules_kernel(const __grid_constant__ RulesArgs a) {
+__global__ void __launch_bounds__(Shape<T, DP>::kThreads) attention_rules_kernel(const __grid_constant__ RulesArgs a) {
   using S = Shape<T, DP>;
   using F = typename S::F;
   constexpr int kThreads = S::kThreads, kRows = S::kRows;
@@ -229,6 +229,7 @@ extern "C" int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, con
   a.status = device_status_word();
   FML_REQUIRE(a.status, FML_CUDA_ERROR, "fml_attention_rules: no device status word");
   if (attention_rules_tc_eligible(a, q->dtype)) return launch_attention_rules_tc(a, q->dtype, as_stream(stream));
+  if (q->dtype == FML_F32 && attention_rules_pair_eligible(a)) return launch_attention_rules_pair(a, rules->divisor, rules->cap, as_stream(stream));
   if (q->dtype == FML_F32) return launch_mma<float>(a, as_stream(stream));
   if (q->dtype == FML_F16) return launch_mma<__half>(a, as_stream(stream));
   return launch_mma<__nv_bfloat16>(a, as_stream(stream));

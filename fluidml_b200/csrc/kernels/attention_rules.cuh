@@ -23,6 +23,9 @@ struct RulesArgs {
 // attention_rules_tc.cu: whether its kernel takes these operands, and its launch.
 bool attention_rules_tc_eligible(const RulesArgs &a, int dtype);
 int launch_attention_rules_tc(const RulesArgs &a, int dtype, cudaStream_t s);
+// attention_pair.cu: the same in fp32.
+bool attention_rules_pair_eligible(const RulesArgs &r);
+int launch_attention_rules_pair(const RulesArgs &r, float divisor, float cap, cudaStream_t s);
 
 __device__ __forceinline__ int64_t document_at(const IndexView &v, int64_t row, int batch, int i) {
   const int64_t e = batch * row + i * v.stride;

@@ -16,6 +16,13 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// n / d for n d < 2^32, by a multiplication (an integer division is some twenty instructions, of about a hundred for 16 bytes).
+struct SmallDivisor {
+  uint32_t m;
+  __host__ explicit SmallDivisor(int d = 1) : m(d > 1 ? (uint32_t)(0x100000000ull / (uint32_t)d + (0x100000000ull % (uint32_t)d != 0)) : 0) {}
+  __device__ __forceinline__ int operator()(int n) const { return m ? (int)__umulhi((uint32_t)n, m) : n; }
+};
+
 struct RotaryPart {  // q, k or v: [tokens, heads, head size] in, the same or a paged cache out
   const void *in;
   void *out;
@@ -23,6 +30,7 @@ struct RotaryPart {  // q, k or v: [tokens, heads, head size] in, the same or a 
   int64_t out_t, out_h, out_d;      // out_t: of a token, or of a position in its page
   int64_t out_page;                 // of a page (paged)
   int heads, units, turned, paged;  // units of a head; of which `turned` are rotated
+  SmallDivisor by_units;
 };
 
 struct RotaryPositionsArgs {
@@ -32,6 +40,8 @@ struct RotaryPositionsArgs {
   int64_t freq_stride, tokens, capacity;  // capacity: pages * page size
   float magnitude;
   int page, half, interleaved, per_token, tokens_per_cta;  // per_token: units of a token
+  int ends[2];                                             // units of q, of q and k
+  SmallDivisor by_token, by_half;
   int *status;
 };
 
@@ -46,7 +56,7 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens_per_cta;
   const int n = (int)min((int64_t)a.tokens_per_cta, a.tokens - t0);
   for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
-    const int t = i / a.half, j = i - t * a.half;
+    const int t = a.by_half(i), j = i - t * a.half;
     // position * frequency / 2 pi with what each product rounds away (1 / 2 pi as two numbers): the fraction is good to 2^-50
     // for any position that 64 bits hold
     const double pos = (double)index_at(a.positions, t0 + t), f = (double)a.frequencies[j * a.freq_stride];
@@ -59,16 +69,20 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
   if (a.slots.p && threadIdx.x < n) {
     const int64_t slot = index_at(a.slots, t0 + threadIdx.x);
     where[threadIdx.x] = -1;
-    if (slot >= 0 && slot < a.capacity) where[threadIdx.x] = (slot / a.page) << 32 | (slot % a.page);
+    if (slot >= 0 && slot < a.capacity) {
+      const int64_t page = slot < (1ll << 31) ? (int64_t)((uint32_t)slot / (uint32_t)a.page) : slot / a.page;
+      where[threadIdx.x] = page << 32 | (slot - page * a.page);
+    }
     else if (slot >= 0) atomicOr(a.status, kStatusIndexRange);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n * a.per_token; i += kThreads) {
-    const int t = i / a.per_token;
-    int u = i - t * a.per_token, which = 0;
-    while (which < 2 && u >= a.part[which].heads * a.part[which].units) { u -= a.part[which].heads * a.part[which].units; ++which; }
+    const int t = a.by_token(i);
+    int u = i - t * a.per_token;
+    const int which = u < a.ends[0] ? 0 : u < a.ends[1] ? 1 : 2;
+    if (which) u -= a.ends[which - 1];
     const RotaryPart &p = a.part[which];
-    const int h = u / p.units;
+    const int h = p.by_units(u);
     u -= h * p.units;
     const T *src = static_cast<const T *>(p.in) + (t0 + t) * p.in_t + h * p.in_h;
     T *dst = static_cast<T *>(p.out) + h * p.out_h;
@@ -126,10 +140,18 @@ template <typename T> int launch(RotaryPositionsArgs &a, int v, int64_t head, cu
     p.units = p.turned + (int)((head - r) / v);
     per += p.heads * p.units;
     a.per_token = per;
+    if (i < 2) a.ends[i] = per;
+    p.by_units = SmallDivisor(p.units);
+    FML_REQUIRE((int64_t)per * std::max(p.units, 1) < (1ll << 32), FML_UNSUPPORTED, "fml_rotary_positions: too many features");
   }
   if (a.tokens == 0 || a.per_token == 0) return FML_OK;
   // a CTA takes as many tokens as give every thread a unit, and one when a token alone has more
   a.tokens_per_cta = std::max(1, std::min(kThreads / std::max(1, a.per_token), kThreads));
+  a.by_token = SmallDivisor(a.per_token);
+  a.by_half = SmallDivisor(a.half);
+  FML_REQUIRE((int64_t)a.per_token * a.tokens_per_cta * a.per_token < (1ll << 32) || a.tokens_per_cta == 1, FML_UNSUPPORTED,
+              "fml_rotary_positions: too many features");
+  if (a.tokens_per_cta == 1 && (int64_t)a.per_token * a.per_token >= (1ll << 32)) a.by_token.m = 1u;  // (n / per_token is 0: so is n * 1 >> 32)
   const int64_t ctas = (a.tokens + a.tokens_per_cta - 1) / a.tokens_per_cta;
   const size_t smem = (size_t)a.tokens_per_cta * a.half * sizeof(float2);
   FML_REQUIRE(ctas < (1ll << 31) && smem <= 40 * 1024, FML_UNSUPPORTED, "fml_rotary_positions: too many tokens or features");
@@ -164,7 +186,7 @@ extern "C" int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, co
   FML_REQUIRE(std::isfinite(magnitude), FML_BAD_ARG, "fml_rotary_positions: magnitude is not finite");
   FML_REQUIRE(!slots || k || v, FML_BAD_ARG, "fml_rotary_positions: slots without keys or values");
   RotaryPositionsArgs a;
-  memset(&a, 0, sizeof(a));
+  memset(static_cast<void *>(&a), 0, sizeof(a));
   a.positions = index_view(positions);
   a.slots = index_view(slots);
   a.frequencies = static_cast<const float *>(frequencies->data);
