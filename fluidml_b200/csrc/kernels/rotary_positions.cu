@@ -147,6 +147,8 @@ template <typename T> int launch(RotaryPositionsArgs &a, int v, int64_t head, cu
   if (a.tokens == 0 || a.per_token == 0) return FML_OK;
   // a CTA takes as many tokens as give every thread a unit, and one when a token alone has more
   a.tokens_per_cta = std::max(1, std::min(kThreads / std::max(1, a.per_token), kThreads));
+  // long prompts: two, so that fewer barriers wait for angles (8191 tokens of 32 + 2 x 8 heads of 128, bf16: 45 -> 42 us; four: 42)
+  if (a.tokens_per_cta == 1 && a.tokens >= 2ll * kSms * 8 && 2ll * a.per_token * a.per_token < (1ll << 32)) a.tokens_per_cta = 2;
   a.by_token = SmallDivisor(a.per_token);
   a.by_half = SmallDivisor(a.half);
   FML_REQUIRE((int64_t)a.per_token * a.tokens_per_cta * a.per_token < (1ll << 32) || a.tokens_per_cta == 1, FML_UNSUPPORTED,
