@@ -1,6 +1,7 @@
 """In-tree build of the native libraries (nvcc cross-compiles sm_100a without a GPU).
 
     libfluidml_b200_kernels.so   the CUDA kernel library behind include/fluidml_cuda.h
+    _serving.so                  the Python calls of a decoder's serving step onto that library (needs Python's headers)
     libfluidml_b200.so           the C++ host (parser, converter, planners, executor) behind
                                  include/worker/executor.h and include/fluidml_executor.h
 
@@ -13,6 +14,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -28,6 +30,7 @@ CXX = os.environ.get("FLUIDML_CXX", "/usr/bin/g++" if os.path.exists("/usr/bin/g
 
 KERNELS_SO = os.path.join(LIBDIR, "libfluidml_b200_kernels.so")
 HOST_SO = os.path.join(LIBDIR, "libfluidml_b200.so")
+SERVING_SO = os.path.join(LIBDIR, "_serving.so")
 
 NVCC_FLAGS = ["-ccbin", CXX, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-I", INCLUDE, "-I", os.path.join(CSRC, "kernels"),
@@ -112,8 +115,17 @@ def build_host(verbose: bool = False) -> str:
     return HOST_SO
 
 
+def build_serving(verbose: bool = False) -> str:
+    src = os.path.join(CSRC, "python", "serving.cpp")
+    if _newer(SERVING_SO, [src, KERNELS_SO, *glob.glob(os.path.join(INCLUDE, "*.h"))]):
+        _run([CXX, "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], src, "-o",
+              SERVING_SO, "-L", LIBDIR, "-lfluidml_b200_kernels", "-Wl,-rpath,$ORIGIN"], verbose)
+    return SERVING_SO
+
+
 def build_all(verbose: bool = False) -> None:
     build_kernels(verbose)
+    build_serving(verbose)
     build_host(verbose)
     build_cli(verbose)
 

@@ -7,6 +7,7 @@ path behind these functions.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import struct
 from typing import Optional, Sequence
@@ -436,52 +437,49 @@ class ScoreRules(ctypes.Structure):
     _fields_ = [("divisor", ctypes.c_float), ("cap", ctypes.c_float), ("causal", ctypes.c_int32)]
 
 
-_DTYPES: dict = {}  # dtype object of another library -> code
 _PACK = [struct.Struct(f"Qii{r}q{8 * (MAX_RANK - r)}x{r}q{8 * (MAX_RANK - r)}x").pack for r in range(MAX_RANK + 1)]
+_native = None
 
 
-def _arg(t):
-    """What the serving operators take: a DeviceTensor, a Tensor, None, or any object with data_ptr(), dtype, shape and stride()
-    (a torch tensor on the current device).  Returns a value ctypes passes as a pointer to the description, which the call reads
-    before it returns."""
-    if t is None:
-        return None
+def _describe(t) -> bytes:
+    """The bytes of an fml_tensor for what the serving operators take: a DeviceTensor, a Tensor, or any object with data_ptr(), dtype,
+    shape, stride() and is_cuda (a torch tensor on the current device)."""
     if isinstance(t, (DeviceTensor, Tensor)):
-        return ctypes.byref(t if isinstance(t, Tensor) else t.c())
-    # (one packed block of bytes: a ctypes structure costs several times as much, and a small call is mostly this)
-    shape = t.shape
-    code = _DTYPES.get(t.dtype)
-    if code is None or not t.is_cuda or len(shape) > MAX_RANK:
-        code = _DTYPES.setdefault(t.dtype, _SERVING_CODE.get(str(t.dtype), 0))
-        if code == 0:
-            raise FmlError(2, f"no kernel takes {t.dtype}")
-        if not t.is_cuda:
-            raise FmlError(1, f"a tensor on {t.device} was given where device memory is needed")
-        if len(shape) > MAX_RANK:
-            raise FmlError(1, f"at most {MAX_RANK} dims")
-    return _PACK[len(shape)](t.data_ptr(), code, len(shape), *shape, *t.stride())
+        return bytes(t if isinstance(t, Tensor) else t.c())
+    code = _SERVING_CODE.get(str(t.dtype), 0)
+    if code == 0:
+        raise FmlError(2, f"no kernel takes {t.dtype}")
+    if not t.is_cuda:
+        raise FmlError(1, f"a tensor on {t.device} was given where device memory is needed")
+    if len(t.shape) > MAX_RANK:
+        raise FmlError(1, f"at most {MAX_RANK} dims")
+    if type(t).__name__ == "Tensor":  # plain torch tensors are read by the extension itself from here on
+        _native.add_dtype(t.dtype, code)
+        _native.set_tensor_type(type(t))
+    return _PACK[len(t.shape)](t.data_ptr(), code, len(t.shape), *t.shape, *t.stride())
 
 
-_FUNCTIONS: dict = {}
-
-
-def _serving(name, *types):
-    """A function of the library with its argument types (set at its first use)."""
-    f = _FUNCTIONS.get(name)
-    if f is None:
-        f = _FUNCTIONS[name] = getattr(lib(), name)
-        f.argtypes = list(types)
-    return f
-
-
-_P, _F, _I = ctypes.c_void_p, ctypes.c_float, ctypes.c_int
+def _serving():
+    """The extension behind the calls below (csrc/python/serving.cpp), loaded once."""
+    global _native
+    if _native is None:
+        lib()  # the kernel library first, so that the extension resolves against it
+        path = os.path.join(os.path.dirname(_LIB_PATH), "_serving.so")
+        if not os.path.exists(path):
+            raise ImportError(f"{path} is missing: run `python -m fluidml_b200.build` (there is no fallback implementation)")
+        spec = importlib.util.spec_from_file_location("_serving", path)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.set_describe(_describe)
+        _native = module
+    return _native
 
 
 def rotary_positions(q, k, v, positions, slots, frequencies, q_out, k_out, v_out, magnitude=1.0, layout=ROTARY_HALVES, stream=None):
     """Turns q and k by their positions; with slots, k and v go into a paged cache (fml_rotary_positions)."""
-    f = _FUNCTIONS.get("fml_rotary_positions") or _serving("fml_rotary_positions", _P, _P, _P, _P, _P, _P, _F, _I, _P, _P, _P, _P)
-    check(f(_arg(q), _arg(k), _arg(v), _arg(positions), _arg(slots), _arg(frequencies), magnitude, layout, _arg(q_out), _arg(k_out),
-            _arg(v_out), stream))
+    st = (_native or _serving()).rotary_positions(q, k, v, positions, slots, frequencies, q_out, k_out, v_out, magnitude, layout, stream)
+    if st:
+        check(st)
 
 
 def rotary_frequencies(rot, scaling=ROTARY_PLAIN, base=10000.0, factor=1.0, trained_length=0.0, turns_low=1.0, turns_high=4.0):
@@ -494,35 +492,36 @@ def rotary_frequencies(rot, scaling=ROTARY_PLAIN, base=10000.0, factor=1.0, trai
 
 def attention_rules(q, k, v, out, divisor, cap=0.0, causal=False, slopes=None, prefix=None, q_documents=None, k_documents=None, stream=None):
     """Attention over a prompt with capped scores, a distance bias, documents and a prefix (fml_attention_rules)."""
-    f = _FUNCTIONS.get("fml_attention_rules") or _serving("fml_attention_rules", *[_P] * 10)
-    rules = ScoreRules(divisor, cap, 1 if causal else 0)
-    check(f(_arg(q), _arg(k), _arg(v), _arg(slopes), _arg(prefix), _arg(q_documents), _arg(k_documents), ctypes.byref(rules), _arg(out), stream))
+    st = (_native or _serving()).attention_rules(q, k, v, slopes, prefix, q_documents, k_documents, out, divisor, cap, causal, stream)
+    if st:
+        check(st)
 
 
 def attention_tree_workspace(requests, tokens, heads, kv_heads, head_size) -> int:
     """Bytes that attention_tree needs as its workspace (fml_attention_tree_workspace); host only."""
-    f = _serving("fml_attention_tree_workspace", *[ctypes.c_int64] * 5)
+    f = lib().fml_attention_tree_workspace
     f.restype = ctypes.c_size_t
-    return f(requests, tokens, heads, kv_heads, head_size)
+    return f(*[ctypes.c_int64(x) for x in (requests, tokens, heads, kv_heads, head_size)])
 
 
 def attention_tree(q, k_cache, v_cache, block_table, context, query_start, tree, out, workspace, divisor, cap=0.0, slopes=None, stream=None):
     """Attention of new tokens (a chain, or with `tree` a tree of drafts) over a paged cache (fml_attention_tree).
-    `workspace`: a DeviceBuffer, or any array of bytes on the device with data_ptr() and numel()."""
-    f = _FUNCTIONS.get("fml_attention_tree") or _serving("fml_attention_tree", *[_P] * 11, ctypes.c_size_t, _P)
-    rules = ScoreRules(divisor, cap, 1)
+    `workspace`: a DeviceBuffer, or any array of bytes on the device with data_ptr(), numel() and element_size()."""
     if isinstance(workspace, DeviceBuffer):
         place, size = workspace.ptr, workspace.nbytes
     else:
         place, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    check(f(_arg(q), _arg(k_cache), _arg(v_cache), _arg(block_table), _arg(context), _arg(query_start), _arg(tree), _arg(slopes),
-            ctypes.byref(rules), _arg(out), place, size, stream))
+    st = (_native or _serving()).attention_tree(q, k_cache, v_cache, block_table, context, query_start, tree, slopes, out, divisor, cap, place,
+                                                size, stream)
+    if st:
+        check(st)
 
 
 def sample(logits, uniform, tokens, temperature=None, top_k=None, top_p=None, min_p=None, probabilities=None, stream=None):
     """One token per row of logits from given random numbers (fml_sample)."""
-    f = _FUNCTIONS.get("fml_sample") or _serving("fml_sample", *[_P] * 9)
-    check(f(_arg(logits), _arg(uniform), _arg(temperature), _arg(top_k), _arg(top_p), _arg(min_p), _arg(tokens), _arg(probabilities), stream))
+    st = (_native or _serving()).sample(logits, uniform, temperature, top_k, top_p, min_p, tokens, probabilities, stream)
+    if st:
+        check(st)
 
 
 # ------------------------------------------------------------------ resident stage program
