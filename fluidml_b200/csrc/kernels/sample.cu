@@ -11,7 +11,8 @@
 //      until a bin is one key; of equal logits the lowest indexes are kept
 //   4  top-p: the counts bound every bin's weight, which leaves a few bins for the cut; one pass sums the weights of all
 //      tokens and of those above these bins exactly and bins the rest by key, as in 3, with weights in place of counts
-//   5  the draw: sums of the kept weights per warp, in the vocabulary's order, then the warp that holds the token walks its part
+//   5  min-p, as a key; the draw: sums of the kept weights per warp, in the vocabulary's order (those above 4's bins are known),
+//      then the warp that holds the token walks its part
 //
 // Weights are integers, 2^44 for the largest: their sums are exact in any order, so neither the atomics nor the split over warps
 // and CTAs changes a result, and a cumulative sum lies within 2^-27 of the largest weight of the real one however many tokens
@@ -52,6 +53,7 @@ struct Shared {
   u64 sums[2][kMaxCluster];        // of every CTA
   u64 exchange[2][kMaxCluster];
   u64 found[4];
+  double roots[32];
   int listed;
 };
 
@@ -89,31 +91,21 @@ template <> struct Key<float> {
   __device__ __forceinline__ static float value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 };
 
-// The fraction's part of 2^x for the rest f of x, |f| <= 1 / 2: Taylor's series of e^(f ln 2) to the 11th power, 6e-15.
-__device__ __forceinline__ double exp2_rest(double f) {
-  f *= 0.6931471805599453;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, f, 1.0 / 3628800.0);
-  p = fma(p, f, 1.0 / 362880.0);
-  p = fma(p, f, 1.0 / 40320.0);
-  p = fma(p, f, 1.0 / 5040.0);
-  p = fma(p, f, 1.0 / 720.0);
-  p = fma(p, f, 1.0 / 120.0);
-  p = fma(p, f, 1.0 / 24.0);
-  p = fma(p, f, 1.0 / 6.0);
-  p = fma(p, f, 0.5);
-  p = fma(p, f, 1.0);
-  return fma(p, f, 1.0);
-}
-__device__ __forceinline__ double exp2_64(double x) {  // -1100 < x <= 0
-  const double n = rint(x);
-  return ldexp(exp2_rest(x - n), (int)n);
+// e^x for |x| <= ln 2 / 64 by Taylor's series to the fifth power, 2.3e-15: what is left of 2^y besides a power of two and one of
+// 2^(i / 32), i = 0 .. 31, which a CTA has in a table.
+__device__ __forceinline__ double exp_small(double x) {
+  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(p, x, 1.0 / 6.0);
+  p = fma(p, x, 0.5);
+  p = fma(p, x, 1.0);
+  return fma(p, x, 1.0);
 }
 
 struct Row {
-  double top, rate;  // weight = 2^((z - top) * rate)
+  double top, rate;  // weight = 2^((z - top) * rate / 32)
+  const double *roots;  // 2^(i / 32), in shared memory
   float topf, scale;  // bins: (topf - z) / 2 * scale
-  double least;       // log2 of min-p, -infinity when off
+  double least;       // 32 log2 of min-p, -infinity when off
   uint32_t cut_key;   // kept: a key above cut_key, or equal and an index up to cut_index
   int cut_index;
 };
@@ -121,14 +113,17 @@ struct Row {
 __device__ __forceinline__ double exponent_of(const Row &r, float z) { return z == r.topf ? 0.0 : ((double)z - r.top) * r.rate; }
 __device__ __forceinline__ u64 weight_of(const Row &r, float z) {
   const double t = exponent_of(r, z);
-  if (!(t >= -45.0)) return t > -1075.0 ? 1ull : 0ull;  // (a weight that 64 bits hold; NaN, of an infinite rate: none)
+  if (!(t >= -45.0 * 32)) return t > -1075.0 * 32 ? 1ull : 0ull;  // (a weight that 64 bits hold; NaN, of an infinite rate: none)
   // adding 1.5 x 2^52 leaves the nearest integer in the low bits, adding 2^52 the rounded weight
   const double shifted = t + 6755399441055744.0;
-  const double p = exp2_rest(t - (shifted - 6755399441055744.0));
-  const double scaled = __hiloint2double(__double2hiint(p) + ((__double2loint(shifted) + 44) << 20), __double2loint(p));
+  const int i = __double2loint(shifted);
+  const double p = exp_small((t - (shifted - 6755399441055744.0)) * (0.6931471805599453 / 32)) * r.roots[i & 31];
+  const double scaled = __hiloint2double(__double2hiint(p) + (((i >> 5) + 44) << 20), __double2loint(p));
   const u64 w = (u64)__double_as_longlong(scaled + 4503599627370496.0) & 0xfffffffffffffull;
   return w ? w : 1ull;
 }
+// The weight as a number, of the largest's 1.
+__device__ __forceinline__ double share_of(const Row &r, float z) { return exp2(fmax(exponent_of(r, z), -1074.0 * 32) * (1.0 / 32)); }
 __device__ __forceinline__ int bin_of(const Row &r, float z) {
   // (halves: the difference of two finite logits may not be finite; that of two infinite ones is NaN, whose integer is 0)
   return min((int)(fmaf(z, -0.5f, 0.5f * r.topf) * r.scale), kBins - 1);
@@ -300,23 +295,47 @@ template <typename T> struct Sampler {
     }
     *hi = l;
   }
-  // Narrows the range of keys [lo, hi], above which lies `above` of the measure, to the one key at which the running sum has
-  // reached(sum).  first: the histogram of the range is merged already (by (hi - key) >> shift_of).
-  template <typename M, typename R>
-  __device__ void narrow(uint32_t lo, uint32_t hi, u64 above, bool first, M measure, R reached, uint32_t *key, u64 *sum_before, u64 *ties) {
+  // The smallest key whose weight is not below min-p: the exponent is monotone in the key.
+  __device__ uint32_t least_key(const Row &r) const {
+    uint32_t l = Key<T>::kNone + 1, h = top_key;
+    while (l < h) {
+      const uint32_t step = (h - l) / 33 + 1, m = min(l + (lane + 1) * step - 1, h);
+      const unsigned yes = __ballot_sync(0xffffffffu, exponent_of(r, Key<T>::value(m)) >= r.least);
+      const int k = yes ? __ffs(yes) - 1 : 32;
+      const uint32_t was = l;
+      if (k > 0) l = min(was + (uint32_t)k * step, h);
+      if (k < 32) h = min(was + (uint32_t)(k + 1) * step - 1, h);
+    }
+    return l;
+  }
+  // One kept key of the range into the histogram.  A bin of one key counts them (a 32-bit atomic; equal logits, of which a 16-bit
+  // type has thousands, meet there, and 64-bit ones would go round in turns); wider bins add up what they measure.
+  template <typename W> __device__ __forceinline__ void put(uint32_t hi, int shift, uint32_t key, W unit) {
+    if (shift == 0) atomicAdd(reinterpret_cast<uint32_t *>(&sh->hist[hi - key]), 1u);
+    else atomicAdd(&sh->hist[(hi - key) >> shift], unit(key));
+  }
+  // After merge(): counts times what their key measures.
+  template <typename W> __device__ void weigh(uint32_t lo, uint32_t hi, int shift, W unit) {
+    if (shift) return;
+    for (uint32_t i = threadIdx.x; i <= hi - lo; i += kThreads)
+      if (sh->merged[i]) sh->merged[i] *= unit(hi - i);
+    __syncthreads();
+  }
+  // Narrows the range of keys [lo, hi], above which lies `above` of the measure (unit(key) for kept(key, index)), to the one key at
+  // which the running sum has reached(sum).  first: the histogram of the range is merged already.
+  template <typename K, typename W, typename R>
+  __device__ void narrow(uint32_t lo, uint32_t hi, u64 above, bool first, K kept, W unit, R reached, uint32_t *key, u64 *sum_before, u64 *ties) {
     for (;;) {
       const int shift = shift_of(lo, hi);
       if (!first) {
         clear();
         each([&](uint32_t k, int i) {
-          if (k >= lo && k <= hi) {
-            const u64 m = measure(k, i);
-            if (m) atomicAdd(&sh->hist[(hi - k) >> shift], m);
-          }
+          if (k >= lo && k <= hi && kept(k, i)) put(hi, shift, k, unit);
         });
         merge();
       }
       first = false;
+      weigh(lo, hi, shift, unit);
       int b;
       first_bin(above, reached, &b, &above);
       const u64 inside = sh->merged[b];
@@ -331,10 +350,13 @@ template <typename T> struct Sampler {
   __device__ __forceinline__ static int shift_of(uint32_t lo, uint32_t hi) { return max(0, 22 - __clz((int)((hi - lo) | 1u))); }
 
   // The first index, in the vocabulary's order, at which the running sum of measure(key, index) has reached(sum); -1: none.
-  template <typename M, typename R> __device__ int locate(M measure, R reached, u64 *total) {
+  // known: what the warp has of it in keys above `below`, which are then left out of the first pass.
+  template <typename M, typename R> __device__ int locate(M measure, R reached, u64 *total, u64 known = 0, uint32_t below = 0xffffffffu) {
     u64 mine = 0;
-    each([&](uint32_t k, int i) { mine += measure(k, i); });
-    mine = warp_sum(mine);
+    each([&](uint32_t k, int i) {
+      if (k <= below) mine += measure(k, i);
+    });
+    mine = warp_sum(mine) + known;
     __syncthreads();
     if (lane == 0) part()[warp] = mine;
     if (threadIdx.x == 0) sh->found[3] = ~0ull;
@@ -528,6 +550,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
       *reinterpret_cast<uint4 *>(data + i) = k;
     }
   }
+  if (threadIdx.x < 32) shared.roots[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32));
   const uint32_t top_key = s.largest(top);  // (its barriers publish the slice too)
   s.top_key = top_key;
   if (temperature > 0.0f) temperature = fmaxf(temperature, 1e-30f);  // (the bins' scale stays finite)
@@ -537,10 +560,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
     Row r;
     r.topf = Key<T>::value(top_key);
     r.top = (double)r.topf;
-    r.rate = 1.4426950408889634 / (double)temperature;
+    r.rate = 32 * 1.4426950408889634 / (double)temperature;
+    r.roots = shared.roots;
     r.scale = 2.0f * (float)kBins / kSpan / temperature;
     r.cut_key = Key<T>::kNone + 1; r.cut_index = a.vocab;
-    r.least = m > 0.0f ? log2((double)fminf(m, 1.0f)) : -INFINITY;
+    r.least = m > 0.0f ? 32 * log2((double)fminf(m, 1.0f)) : -INFINITY;
     u = u >= 0.0f ? fminf(u, 0.99999994f) : 0.0f;
     if (!(temperature > 0.0f)) {
       // the largest logit, lowest index
@@ -583,7 +607,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
           if (threadIdx.x == 0) {
             if (token >= 0) {
               const float z = to_f32(src[(int64_t)token * a.col_stride]);  // (perhaps another CTA's)
-              probability = exp2_64(fmax(exponent_of(r, z), -1074.0)) * kOne / total;
+              probability = share_of(r, z) * kOne / total;
             }
             if (a.tokens_wide) static_cast<int64_t *>(a.tokens)[row * a.tokens_s] = token;
             else static_cast<int32_t *>(a.tokens)[row * a.tokens_s] = token;
@@ -595,7 +619,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
           uint32_t lo, hi, key;
           u64 sum_before, ties;
           s.keys_of(r, b, b, &lo, &hi);
-          s.narrow(lo, hi, above, false, [](uint32_t, int) { return 1ull; }, [&](u64 c) { return c >= want; }, &key, &sum_before, &ties);
+          s.narrow(lo, hi, above, false, [](uint32_t, int) { return true; }, [](uint32_t) { return 1ull; }, [&](u64 c) { return c >= want; }, &key,
+                   &sum_before, &ties);
           r.cut_key = key;
           if (sum_before + ties > want) {
             u64 total;
@@ -613,6 +638,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         __syncthreads();
       }
       // ---- 4: top-p
+      u64 known = 0;                  // this warp's weights of keys above `range`, all of which are kept
+      uint32_t range = 0xffffffffu;
       if (by_p) {
         const double share = p > 0.0f ? (double)p : 0.0;  // (0: the first token alone)
         // A bin's weights, in units of the largest, are exp(-x) for x between its ends: sums of the most and of the least they can
@@ -649,13 +676,15 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         u64 all = 0, over = 0;
         s.clear();
         s.each([&](uint32_t key, int i) {
-          if (key > Key<T>::kNone && kept_by_cut(r, key, i)) {
+          if (kept_by_cut(r, key, i)) {
             const u64 w = weight_of(r, Key<T>::value(key));
             all += w;
             if (key > hi) over += w;
-            else if (key >= lo && w) atomicAdd(&shared.hist[(hi - key) >> shift], w);
+            else if (key >= lo) s.put(hi, shift, key, [&](uint32_t) { return w; });
           }
         });
+        known = s.warp_sum(over);
+        range = hi;
         all = s.block_sum(all);
         over = s.block_sum(over);
         s.merge(all, over);
@@ -664,8 +693,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         const double want = share * (double)all;
         uint32_t key;
         u64 sum_before, ties;
-        s.narrow(lo, hi, over, true, [&](uint32_t x, int i) { return kept_by_cut(r, x, i) ? weight_of(r, Key<T>::value(x)) : 0ull; },
-                 [&](u64 c) { return (double)c >= want && c > 0; }, &key, &sum_before, &ties);
+        s.narrow(lo, hi, over, true, [&](uint32_t x, int i) { return kept_by_cut(r, x, i); },
+                 [&](uint32_t x) { return weight_of(r, Key<T>::value(x)); }, [&](u64 c) { return (double)c >= want && c > 0; }, &key, &sum_before, &ties);
         const u64 w = weight_of(r, Key<T>::value(key));
         // of the tied tokens the first n: those before which less than `want` lies
         u64 n = w ? (u64)fmax(ceil((want - (double)sum_before) / (double)w), 1.0) : 1;
@@ -682,20 +711,23 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         r.cut_index = index;
       }
       // ---- 5: the draw
+      if (m > 0.0f) {
+        const uint32_t least = s.least_key(r);
+        if (least > r.cut_key) {
+          r.cut_key = least;
+          r.cut_index = a.vocab;
+          if (least > range) { known = 0; range = 0xffffffffu; }  // (some keys above the range are not kept)
+        }
+      }
       u64 total;
-      token = s.locate(
-          [&](uint32_t key, int i) {
-            if (key <= Key<T>::kNone || !kept_by_cut(r, key, i)) return 0ull;
-            const float z = Key<T>::value(key);
-            return exponent_of(r, z) >= r.least ? weight_of(r, z) : 0ull;
-          },
-          [&](u64 c, u64 sum) { return (double)c > (double)u * (double)sum; }, &total);
+      token = s.locate([&](uint32_t key, int i) { return kept_by_cut(r, key, i) ? weight_of(r, Key<T>::value(key)) : 0ull; },
+                       [&](u64 c, u64 sum) { return (double)c > (double)u * (double)sum; }, &total, known, range);
       if (token >= s.base && token < s.base + a.slice) {
         const uint4 k = *reinterpret_cast<const uint4 *>(data + (token - s.base) / V * V);
         const uint32_t *const w = reinterpret_cast<const uint32_t *>(&k);
         const int j = (token - s.base) % V;
         const float z = Key<T>::value(sizeof(T) == 4 ? w[j] : j & 1 ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu);
-        probability = exp2_64(fmax(exponent_of(r, z), -1074.0)) * kOne / (double)total;
+        probability = share_of(r, z) * kOne / (double)total;
       }
     }
   }
