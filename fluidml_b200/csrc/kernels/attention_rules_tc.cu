@@ -7,7 +7,7 @@
 //   warps 0-7, 8-15  softmax of tile A, B: thread = query = lane of tensor memory, and 64 of the 128 keys: two threads share a
 //                    query, and tell each other its largest score
 //   warp 16          loads (tensor maps, 128-byte swizzle): Q once, K and V tiles into two stages each
-//   warp 17          products, in the order  S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j)  (weights apart, see TcShape: S_A(j)  PV_B(j-2)
+//   warp 17          products (weights apart, see TcShape: whichever can go next): while one tile's softmax runs, the tensor cores
 //                    work for the other
 //   (warps 18, 19    make up the last group of four, which gives registers to the softmax: 512 x 104 + 128 x 64 = 640 x 96, what the
 //                    launch has)
@@ -18,8 +18,8 @@
 //
 // The running maximum follows only when a tile's exceeds it by more than 8 (in units of ln 2): weights then reach 2^8, which the
 // sums carry, and the context's correction, a round trip through registers, is rare.  The commit that publishes S(j) also covers
-// PV(j - 1), issued before it, so that the correction needs no barrier of its own (weights apart: PV(j - 2), and PV(j - 1) has one,
-// whose phase is then either that product's or just over).
+// PV(j - 1), issued before it, so that the correction needs no barrier of its own (weights apart, S(j) may come first: the softmax
+// waits for PV(j - 1) before it writes the next weights or corrects).
 #include "attention_rules.cuh"
 #include <algorithm>
 #include <cfloat>
@@ -289,14 +289,8 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t idesc_s = instr_desc_16(type, kKeys, 0u), idesc_o = instr_desc_16(type, a.D, 1u);
     const uint64_t desc_q = smem_desc(q_s, 16u, 1024u), desc_k = smem_desc(k_s, 16u, 1024u), desc_v = smem_desc(v_s, 16384u, 1024u);
     const int steps = a.D / 16;
-    uint32_t done[2] = {0u, 0u}, given[2] = {0u, 0u};  // of each query tile: second products, first products
-    auto scores = [&](int t, uint32_t stage) {
-      if (S::kApart && given[t] > 0) {
-        ok = mbar_wait_warp(bar + 8u * (B::kSFree + t), (given[t] - 1u) & 1u, abort_flag);
-        if (!ok) return;
-        tc_fence_after();
-      }
-      ++given[t];
+    ok = mbar_wait_warp(bar + 8u * B::kQ, 0u, abort_flag) && (!two || mbar_wait_warp(bar + 8u * (B::kQ + 1), 0u, abort_flag));
+    auto issue_scores = [&](int t, uint32_t stage, bool last) {  // last: nobody needs these keys any more
       if (leader) {
         const uint64_t dq = desc_q + (uint64_t)(t * S::kTile >> 4), dk = desc_k + (uint64_t)(stage * S::kTile >> 4);
 #pragma unroll
@@ -306,74 +300,113 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
           if (k < steps) umma_f16_ss(tmem + kColS + 128u * t, dq + off, dk + off, idesc_s, k ? 1u : 0u);
         }
         umma_commit(bar + 8u * (B::kS + t));
+        if (last) umma_commit(bar + 8u * (B::kKEmpty + stage));
       }
       __syncwarp();
     };
-    // tile number n (of those that either sees); last: nobody needs its values any more
-    auto context = [&](int t, uint32_t n, bool last) {
-      const uint32_t stage = n % S::kStages;
-      ok = mbar_wait_warp(bar + 8u * (B::kVFull + stage), n / S::kStages & 1u, abort_flag) &&
-           mbar_wait_warp(bar + 8u * (B::kP + t), done[t] & 1u, abort_flag);
-      if (!ok) return;
-      tc_fence_after();
+    auto issue_context = [&](int t, uint32_t stage, bool first, bool last) {
       if (leader) {
         const uint64_t dv = desc_v + (uint64_t)(stage * S::kTile >> 4);
 #pragma unroll
         for (int k = 0; k < kKeys / 16; ++k)  // (each half of the keys has its weights in a place of its own)
           umma_f16_ts(tmem + kColO + S::kStepO * t, tmem + S::kColP + S::kStepP * t + S::kHalfP * (k >> 2) + 8u * (k & 3), dv + (uint64_t)(k * 2048 >> 4),
-                      idesc_o, done[t] == 0 && k == 0 ? 0u : 1u);
+                      idesc_o, first && k == 0 ? 0u : 1u);
         if (S::kApart) umma_commit(bar + 8u * (B::kPV + t));
         if (last) umma_commit(bar + 8u * (B::kVEmpty + stage));
       }
       __syncwarp();
-      ++done[t];
     };
-    ok = mbar_wait_warp(bar + 8u * B::kQ, 0u, abort_flag) && (!two || mbar_wait_warp(bar + 8u * (B::kQ + 1), 0u, abort_flag));
-    // second products that are to come: of A at most one, of B two with weights apart, else one
-    uint32_t n = 0, wait_a = 0, wait_b[2] = {0u, 0u};
-    bool has_a = false, last_a = false;
-    int has_b = 0;
-    auto next_b = [&]() {
-      context(1, wait_b[0], true);
-      wait_b[0] = wait_b[1];
-      --has_b;
-    };
-    if (ok) each_tile(views, tiles, 15, [&](int, int view) {
-      const uint32_t stage = n % S::kStages;
-      ok = mbar_wait_warp(bar + 8u * (B::kKFull + stage), n / S::kStages & 1u, abort_flag);
-      if (!ok) return false;
-      tc_fence_after();
-      if (view & 3) scores(0, stage);
-      if (ok && has_b == (S::kApart ? 2 : 1)) next_b();
-      if (!ok) return false;
-      if (view >> 2) scores(1, stage);
-      if (!ok) return false;
-      if (leader) umma_commit(bar + 8u * (B::kKEmpty + stage));
-      __syncwarp();
-      if (has_a) {
-        context(0, wait_a, last_a);
-        has_a = false;
-        if (!ok) return false;
-      }
-      if (view & 3) {
-        if (S::kApart) {
-          has_a = true;
-          wait_a = n;
-          last_a = !(view >> 2);
-        } else {
-          context(0, n, !(view >> 2));
+    if constexpr (S::kApart) {
+      // Whatever can go next goes next.  Of query tile t: the tile of keys whose scores (values) come next, its number among those that
+      // either query tile sees (stages and their phases go by that), and how many there have been.  Tiles below both numbers are done
+      // with; one kStages or more above the lower cannot have been loaded, and its stage's phase may be that of an earlier one.
+      struct Front { int tile; uint32_t number, count; };
+      Front s_at[2], v_at[2];
+      auto move = [&](int t, Front &f, bool begin) {  // to the next tile that t sees, `tiles` behind the last
+        if (!begin) { ++f.tile; ++f.number; ++f.count; }
+        while (f.tile < tiles) {
+          const int view = views[f.tile];
+          if (view >> (2 * t) & 3) return;
+          if (view) ++f.number;
+          ++f.tile;
         }
+      };
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s_at[t].tile = 0;
+        s_at[t].number = s_at[t].count = 0u;
+        move(t, s_at[t], true);  // (without a tile B its views are none: its number is behind the last at once)
+        v_at[t] = s_at[t];
       }
-      if (view >> 2) {
-        if (has_b) wait_b[1] = n; else wait_b[0] = n;
-        ++has_b;
+      uint32_t idle = 0;
+      const uint32_t limit = g_wait_limit;
+      while (ok && (v_at[0].tile < tiles || v_at[1].tile < tiles)) {
+        bool moved = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (v_at[t].count < s_at[t].count) {  // weights that are awaited
+            const uint32_t n = v_at[t].number, stage = n % S::kStages, count = v_at[t].count;
+            if (n < min(v_at[0].number, v_at[1].number) + S::kStages && mbar_test_warp(bar + 8u * (B::kP + t), count & 1u) && mbar_test_warp(bar + 8u * (B::kVFull + stage), n / S::kStages & 1u)) {
+              tc_fence_after();
+              const bool last = !(views[v_at[t].tile] >> (2 * (t ^ 1)) & 3) || v_at[t ^ 1].tile > v_at[t].tile;  // nobody needs these values any more
+              issue_context(t, stage, count == 0, last);
+              move(t, v_at[t], false);
+              moved = true;
+            }
+          }
+          // scores, once the softmax has read the last ones
+          const uint32_t count = s_at[t].count;
+          if (s_at[t].tile < tiles && (count == 0 || mbar_test_warp(bar + 8u * (B::kSFree + t), (count - 1u) & 1u))) {
+            const uint32_t n = s_at[t].number, stage = n % S::kStages;
+            if (n < min(s_at[0].number, s_at[1].number) + S::kStages && mbar_test_warp(bar + 8u * (B::kKFull + stage), n / S::kStages & 1u)) {
+              tc_fence_after();
+              const bool last = !(views[s_at[t].tile] >> (2 * (t ^ 1)) & 3) || s_at[t ^ 1].tile > s_at[t].tile;
+              issue_scores(t, stage, last);
+              move(t, s_at[t], false);
+              moved = true;
+            }
+          }
+        }
+        idle = moved ? 0u : idle + 1u;
+        if (idle > limit || ((idle & 255u) == 255u && __any_sync(0xffffffffu, *abort_flag))) ok = false;
       }
-      ++n;
-      return true;
-    });
-    if (ok && has_b == 2) next_b();
-    if (ok && has_a) context(0, wait_a, last_a);
-    if (ok && has_b) next_b();
+    } else {
+      // Weights over their scores: S_A(j)  PV_B(j-1)  S_B(j)  PV_A(j), one wait after another (asking what is ready, as above, took
+      // 399 us for 378 where the order is given anyway).
+      uint32_t n = 0, done[2] = {0u, 0u}, wait_b = 0;
+      bool pending = false;  // B's product with V of the tile before
+      auto context = [&](int t, uint32_t number, bool last) {
+        const uint32_t stage = number % S::kStages;
+        ok = mbar_wait_warp(bar + 8u * (B::kVFull + stage), number / S::kStages & 1u, abort_flag) &&
+             mbar_wait_warp(bar + 8u * (B::kP + t), done[t] & 1u, abort_flag);
+        if (!ok) return;
+        tc_fence_after();
+        issue_context(t, stage, done[t] == 0, last);
+        ++done[t];
+      };
+      if (ok) each_tile(views, tiles, 15, [&](int, int view) {
+        const uint32_t stage = n % S::kStages;
+        ok = mbar_wait_warp(bar + 8u * (B::kKFull + stage), n / S::kStages & 1u, abort_flag);
+        if (!ok) return false;
+        tc_fence_after();
+        if (view & 3) issue_scores(0, stage, !(view >> 2));
+        if (pending) {
+          context(1, wait_b, true);
+          pending = false;
+          if (!ok) return false;
+        }
+        if (view >> 2) issue_scores(1, stage, true);
+        if (view & 3) context(0, n, !(view >> 2));
+        if (!ok) return false;
+        if (view >> 2) {
+          pending = true;
+          wait_b = n;
+        }
+        ++n;
+        return true;
+      });
+      if (ok && pending) context(1, wait_b, true);
+    }
     if (ok && leader) umma_commit(bar + 8u * B::kDone);
     if (!ok) *abort_flag = 1;
     if (leader) umma_drain(bar + 8u * B::kDrain);

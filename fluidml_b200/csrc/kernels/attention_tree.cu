@@ -552,7 +552,8 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
               "fml_attention_tree: the output or the workspace is not memory of the current device");
   TreeArgs a;
   memset(&a, 0, sizeof(a));
-  a.q = q->data; a.k = k_cache->data; a.v = v_cache->data; a.out = out->data;
+  a.q = q->data; a.out = out->data;
+  a.k = pages ? k_cache->data : q->data; a.v = pages ? v_cache->data : q->data;  // (copies of nothing name an address all the same)
   a.table = static_cast<const int32_t *>(block_table->data);
   a.context = static_cast<const int32_t *>(context->data);
   a.query_start = static_cast<const int32_t *>(query_start->data);

@@ -9,10 +9,9 @@ namespace fml {
 
 // Bytes of an element of the types these operators take as data; 0: none of them.
 inline size_t data_size(int dtype) { return dtype == FML_F32 ? 4 : dtype == FML_F16 || dtype == FML_BF16 ? 2 : 0; }
-inline bool is_index(int dtype) { return dtype == FML_I32 || dtype == FML_I64; }
 
 // A described tensor of `rank` dims with elements of `size` bytes (0: a type that is not taken) whose extents are not
-// negative; data may be null only when it is empty.
+// negative; data may be null only when it is empty, and lies on a multiple of an element.
 inline bool described(const fml_tensor *t, int rank, size_t size) {
   if (!t || t->rank != rank || size == 0) return false;
   int64_t n = 1;
@@ -21,10 +20,10 @@ inline bool described(const fml_tensor *t, int rank, size_t size) {
     n = t->shape[i] && n > (1ll << 50) / t->shape[i] ? (1ll << 51) : n * t->shape[i];
     if (n > (1ll << 50)) return false;
   }
-  return n == 0 || t->data != nullptr;
+  return n == 0 || (t->data != nullptr && reinterpret_cast<uintptr_t>(t->data) % size == 0);
 }
 inline bool data_tensor(const fml_tensor *t, int rank) { return t && described(t, rank, data_size(t->dtype)); }
-inline bool index_tensor(const fml_tensor *t, int rank) { return t && described(t, rank, is_index(t->dtype) ? 4 : 0); }
+inline bool index_tensor(const fml_tensor *t, int rank) { return t && described(t, rank, t->dtype == FML_I64 ? 8 : t->dtype == FML_I32 ? 4 : 0); }
 inline bool float_tensor(const fml_tensor *t, int rank) { return t && described(t, rank, t->dtype == FML_F32 ? 4 : 0); }
 
 // Whether memory of the current device (or memory every device sees) is at `p`: a launch on another device's memory would
