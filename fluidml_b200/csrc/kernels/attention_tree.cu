@@ -6,7 +6,12 @@
 // share a CTA, and no CTA waits for the longest.  A CTA writes a stretch that is all of a row's keys to the output and any
 // other to the workspace (normalised context, maximum and sum), which a second kernel adds up in a fixed order.
 //
-// Keys and values come through shared memory by 16-byte asynchronous copies (rows of a page are contiguous, pages are not).
+// Keys and values come through shared memory by 16-byte asynchronous copies (rows of a page are contiguous, pages are not).  One
+// bulk copy per row instead, which a warp issues lane by lane, took 289 us for 232 on 64 requests of one token.
+//
+// Measured (bf16, head size 128): 64 requests of one token over up to 8192, 32 kv heads 802 us, 5.1 TB/s; 8 kv heads 222 us, 4.6;
+// 48 requests of up to 16 drafts, 32 heads on 8, capped 380 us, 2.2 TB/s: there the instructions of softmax and cap, and one
+// barrier per tile for two CTAs of eight warps, bound it; one token over 1000 14 us, most of it the two launches' dependent loads.
 #include "flash_mma.cuh"
 #include <algorithm>
 #include <cmath>

@@ -246,12 +246,11 @@ __device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &
 
 // cap * tanh(s / cap) in units of ln 2, s = x * inv_divisor.
 struct Cap {
-  float scale, cap, inv;  // without a cap scale = log2(e) / divisor; with one scale = 1 / (divisor cap), cap in units of ln 2
+  float scale, cap;  // without a cap scale = log2(e) / divisor; with one scale = 1 / (divisor cap), cap in units of ln 2
   __host__ static Cap make(float divisor, float cap) {
     Cap c;
     c.cap = cap > 0.0f ? cap * kLog2e : 0.0f;
     c.scale = cap > 0.0f ? 1.0f / (divisor * cap) : kLog2e / divisor;
-    c.inv = 0.0f;
     return c;
   }
 };

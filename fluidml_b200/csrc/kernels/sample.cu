@@ -14,6 +14,10 @@
 //   5  min-p, as a key; the draw: sums of the kept weights per warp, in the vocabulary's order (those above 4's bins are known),
 //      then the warp that holds the token walks its part
 //
+// Measured: 256 rows of 131072 bf16 logits, half of them with top-k, the others with top-p and min-p 225 us (a row of the former 60
+// instructions per 32 logits, of the latter 170: weights in 64 bits of every logit, for the sum that top-p is a share of); one row
+// of 50304 16 us, some ten cluster barriers and two small sorts.
+//
 // Weights are integers, 2^44 for the largest: their sums are exact in any order, so neither the atomics nor the split over warps
 // and CTAs changes a result, and a cumulative sum lies within 2^-27 of the largest weight of the real one however many tokens
 // there are (a rounded half unit each, 2^18 tokens).  The exponential is evaluated in 64 bits: its fp32 error, 2^-23 of a
