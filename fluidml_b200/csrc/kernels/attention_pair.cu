@@ -252,7 +252,7 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       if (lane == 0) mbar_arrive(bar_q_ready);
     }
     float m_ref = 0.0f, l = 0.0f;
-    int ev_ref = 0, ev_min = 0;
+    int ev_ref = 0, ev_min = 0, ek_low = 126, ev_low = 126;  // (rules) the scales of the largest keys and values
     RowRules rr;
     if constexpr (MASK == kRules) {
       rr = row_rules(rules, b, h, row_in);
@@ -272,6 +272,8 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       float m_blk = -FLT_MAX;  // (finite, for blocks without a visible key)
       if constexpr (MASK == kRules) {
         const int view = list[j] >> 12, last = rr.last - key0;
+        ek_low = min(ek_low, exp_s[2 * buf]);
+        ev_low = min(ev_low, ev);
         if (a.cap > 0.0f) {
           const float g = f / a.cap;
 #pragma unroll
@@ -367,6 +369,7 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       tc_fence_after();
       const float inv = MASK == kRules && l == 0.0f ? 0.0f : pow2(-ev_ref) / l;
       bool bad = false;
+      float largest = 0.0f;
       float *dst = a.out + (int64_t)b * a.o_s[0] + (int64_t)h * a.o_s[1] + (int64_t)row_in * a.o_s[2];
       const bool vec = a.o_s[3] == 1 && (a.o_s[2] & 3) == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll
@@ -381,7 +384,10 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           }
           float check = 0.0f;  // 0, or NaN from an infinity or NaN on
 #pragma unroll
-          for (int i = 0; i < 32; ++i) check = fmaf(o[i] * inv, 0.0f, check);
+          for (int i = 0; i < 32; ++i) {
+            check = fmaf(o[i] * inv, 0.0f, check);
+            largest = fmaxf(largest, fabsf(o[i] * inv));
+          }
           bad = bad || !(check == 0.0f);
         }
         if (grow >= a.Sq) {
@@ -395,6 +401,15 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
       }
       if constexpr (MASK == kRules) {
+        // A block's scale is that of its largest key and value, and some of them this row may not see.  Values are off by
+        // 2^-39 of the largest, in [2^14, 2^15) 2^-ev_low: nothing to a context above 2^-16 of it (an average of N values of
+        // random sign is some 2^-(log2 N) / 2).  A score is off by at most 64 |q| |k| 2^-39 / divisor: below 2^-19 where
+        // that product of the largest is below 2^20.
+        if (l > 0.0f) {
+          const bool values = ev_low < 126 && largest < pow2(max(-126, -2 - ev_low));
+          const bool keys = ek_low < 126 && 36.0f - (float)(e_q + ek_low) + log2f(fabsf(a.inv_divisor)) > 20.0f;
+          bad = bad || values || keys;
+        }
         unsigned redo = __ballot_sync(0xffffffffu, bad && grow < a.Sq);
         __syncwarp();
         while (redo) {

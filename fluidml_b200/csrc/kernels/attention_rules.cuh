@@ -106,7 +106,7 @@ __device__ __forceinline__ int document_view(int view, const TileRange &t, int64
 }
 
 // A row whose context came out as not finite: keys that it does not see may hold infinities or NaN, which weights of zero do
-// not cancel.  Done again by a warp, key by key, over those it sees (one of them may be the cause: then it stays).
+// not cancel (or, on packed pairs, values beside which its own have no bits left).  Done again by a warp, key by key, over those it sees (one of them may be the cause: then it stays).
 template <typename T> __device__ __noinline__ void redo_rules_row(const RulesArgs &a, int batch, int head, int row) {
   const int lane = threadIdx.x & 31, kv = head / a.group;
   const RowRules r = row_rules(a, batch, head, row);

@@ -111,6 +111,25 @@ def test_what_is_not_seen_adds_nothing(dtype, value):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("large", [2.0 ** 15, 2.0 ** 40, 2.0 ** 100])
+def test_large_numbers_that_are_not_seen_cost_no_bits(dtype, d, large):
+    """Keys and values of another document, and of later rows, in the tile of those that a row sees."""
+    t, s = TYPES[dtype], 200
+    large = min(large, 2.0 ** 15) if t == torch.float16 else large
+    for which in range(2):
+        q, k, v = randn(40, 1, 2, s, d, dtype=t), randn(41, 1, 1, s, d, dtype=t), randn(42, 1, 1, s, d, dtype=t)
+        docs = torch.zeros(1, s, dtype=torch.int32)
+        docs[0, 90:] = 1
+        (k, v)[which][0, 0, 70:90] *= large
+        run(q[:, :, 90:], k, v, qd=docs[:, 90:], kd=docs)                                # behind them
+        out = torch.empty(1, 2, s, d, dtype=t).cuda()
+        cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, math.sqrt(d), causal=True)
+        want, size = attention(q[0, 0, :70], k[0, 0, :70], v[0, 0, :70], visible_of(70, 70, True, None, None, None), math.sqrt(d))
+        assert close(out[0, 0, :70], want, size, t)                                      # in front of them
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_strides_and_alignment(dtype):
     t = TYPES[dtype]
     b, s, d = 2, 70, 64
