@@ -106,28 +106,21 @@ __device__ __forceinline__ int document_view(int view, const TileRange &t, int64
 }
 
 // A row whose context came out as not finite: keys that it does not see may hold infinities or NaN, which weights of zero do
-// not cancel (or, on packed pairs, values beside which its own have no bits left).  Done again by a warp, key by key, over those it sees (one of them may be the cause: then it stays).
+// not cancel (or, on packed pairs, values beside which its own have no bits left).  Done again by a warp over those it sees (one
+// of them may be the cause: then it stays).
 template <typename T> __device__ __noinline__ void redo_rules_row(const RulesArgs &a, int batch, int head, int row) {
   const int lane = threadIdx.x & 31, kv = head / a.group;
   const RowRules r = row_rules(a, batch, head, row);
   const T *q = static_cast<const T *>(a.q) + batch * a.q_s[0] + head * a.q_s[1] + (int64_t)row * a.q_s[2];
   const T *k0 = static_cast<const T *>(a.k) + batch * a.k_s[0] + kv * a.k_s[1], *v0 = static_cast<const T *>(a.v) + batch * a.v_s[0] + kv * a.v_s[1];
-  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-  for (int key = 0; key < r.last; ++key) {
-    if (a.k_documents.p && document_at(a.k_documents, a.k_documents_row, batch, key) != r.document) continue;
-    const T *k = k0 + (int64_t)key * a.k_s[2], *v = v0 + (int64_t)key * a.v_s[2];
-    float s = 0.0f;
-    for (int d = lane; d < a.D; d += 32) s = fmaf(to_f32(q[d * a.q_s[3]]), to_f32(k[d * a.k_s[3]]), s);
-#pragma unroll
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= a.cap.scale;
-    if (a.cap.cap > 0.0f) s = a.cap.cap * tanhf(s);
-    if (a.slopes) s -= r.slope * (float)abs(r.at - key);
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn, keep = ex2_approx(m - base), p = ex2_approx(s - base);
-    m = mn;
-    l = l * keep + p;
-    for (int i = 0, d = lane; d < a.D; ++i, d += 32) o[i] = o[i] * keep + p * to_f32(v[d * a.v_s[3]]);
-  }
+  float o[4], m, l;
+  context_of_seen(q, a.q_s[3], a.k_s[3], a.v_s[3], a.D, a.cap, 0, r.last, [&](int key, const T **k, const T **v, float *less) {
+    if (a.k_documents.p && document_at(a.k_documents, a.k_documents_row, batch, key) != r.document) return false;
+    *k = k0 + (int64_t)key * a.k_s[2];
+    *v = v0 + (int64_t)key * a.v_s[2];
+    if (a.slopes) *less = r.slope * (float)abs(r.at - key);
+    return true;
+  }, o, m, l);
   T *dst = static_cast<T *>(a.out) + batch * a.o_s[0] + head * a.o_s[1] + (int64_t)row * a.o_s[2];
   for (int i = 0, d = lane; d < a.D; ++i, d += 32) dst[d * a.o_s[3]] = from_f32<T>(l == 0.0f ? 0.0f : o[i] / l);
 }

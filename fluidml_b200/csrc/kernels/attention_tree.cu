@@ -90,25 +90,16 @@ __device__ __noinline__ void redo_row(const TreeArgs &a, int r, const Request &x
   const T *q = static_cast<const T *>(a.q) + (int64_t)(x.start + j) * a.q_t + (int64_t)head * a.q_h;
   const float slope = a.slopes ? a.slopes[head * a.slopes_s] * kLog2e : 0.0f;
   const int at = position_of(a, x, j);
-  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-  for (int key = key0; key < key1; ++key) {
-    if (key >= x.context && !sees(a, x, j, key)) continue;
+  float o[4], m, l;
+  context_of_seen(q, a.q_d, 1, 1, a.D, a.cap, key0, key1, [&](int key, const T **k, const T **v, float *less) {
+    if (key >= x.context && !sees(a, x, j, key)) return false;
     const int64_t page = page_of(a, r, key);
-    if (page < 0) continue;
-    const T *k = static_cast<const T *>(a.k) + page * a.k_page + (key % a.page) * a.k_pos + kv * a.k_head;
-    const T *v = static_cast<const T *>(a.v) + page * a.v_page + (key % a.page) * a.v_pos + kv * a.v_head;
-    float s = 0.0f;
-    for (int d = lane; d < a.D; d += 32) s = fmaf(to_f32(q[d * a.q_d]), to_f32(k[d]), s);
-#pragma unroll
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= a.cap.scale;
-    if (a.cap.cap > 0.0f) s = a.cap.cap * tanhf(s);
-    if (a.slopes) s -= slope * (float)abs(at - (key < x.context ? key : position_of(a, x, key - x.context)));
-    const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn, keep = ex2_approx(m - base), p = ex2_approx(s - base);
-    m = mn;
-    l = l * keep + p;
-    for (int i = 0, d = lane; d < a.D; ++i, d += 32) o[i] = o[i] * keep + p * to_f32(v[d]);
-  }
+    if (page < 0) return false;
+    *k = static_cast<const T *>(a.k) + page * a.k_page + (key % a.page) * a.k_pos + kv * a.k_head;
+    *v = static_cast<const T *>(a.v) + page * a.v_page + (key % a.page) * a.v_pos + kv * a.v_head;
+    if (a.slopes) *less = slope * (float)abs(at - (key < x.context ? key : position_of(a, x, key - x.context)));
+    return true;
+  }, o, m, l);
   for (int i = 0, d = lane; d < a.D; ++i, d += 32) ctx[d] = l == 0.0f ? 0.0f : o[i] / l;
   if (lane == 0) { stats[0] = m; stats[1] = l; }
 }

@@ -295,4 +295,67 @@ template <bool EXACT, int NT> __device__ __forceinline__ void cap_scores(const C
   }
 }
 
+// The context of one query over those of the keys [key0, key1) that it sees, by a warp which reads no others: for rows that what
+// they do not see has made infinite or NaN.  `at`: key -> whether it is seen, its rows of k and v, what its score loses.  Eight lanes to a
+// product, four products at a time; the features lane, lane + 32, ... of the context stay in o, undivided.  It stops once nothing
+// but NaN can come of it (l is NaN then): 32 causal heads of 2048 x 128 full of NaN 1.1 ms, where finite ones take 0.1 and
+// one infinity that all later rows do see takes 48.
+template <typename T, typename F>
+__device__ __forceinline__ void context_of_seen(const T *q, int64_t q_d, int64_t k_d, int64_t v_d, int D, const Cap &cap, int key0, int key1,
+                                                const F &at, float (&o)[4], float &m, float &l) {
+  const int lane = threadIdx.x & 31;
+  m = -INFINITY;
+  l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = 0.0f;
+  for (int from = key0; from < key1; from += 32) {
+    const T *k = nullptr, *v = nullptr;
+    float less = 0.0f, s = -INFINITY;
+    const bool seen = from + lane < key1 && at(from + lane, &k, &v, &less);
+    unsigned left = __ballot_sync(0xffffffffu, seen);
+    if (!left) continue;
+#pragma unroll 2
+    for (int r = 0; r < 8; ++r) {
+      const int of = 4 * r + (lane >> 3);
+      const T *row = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k), of));
+      float x = 0.0f;
+      if (left >> of & 1u)
+        for (int d = lane & 7; d < D; d += 8) x = fmaf(to_f32(q[d * q_d]), to_f32(row[d * k_d]), x);
+#pragma unroll
+      for (int w = 4; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+      const float got = __shfl_sync(0xffffffffu, x, (lane & 3) * 8);  // of key 4 r + lane % 4
+      if (lane >> 2 == r) s = got;
+    }
+    s *= cap.scale;
+    if (cap.cap > 0.0f) s = cap.cap * tanhf(s);
+    s = seen ? s - less : -INFINITY;
+    float top = s;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    top = fmaxf(top, m);
+    const float base = top == -INFINITY ? 0.0f : top, keep = ex2_approx(m - base), p = seen ? ex2_approx(s - base) : 0.0f;
+    float sum = p;
+#pragma unroll
+    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    m = top;
+    l = l * keep + sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] *= keep;
+#pragma unroll 2
+    for (; left; left &= left - 1) {
+      const int of = __ffs(left) - 1;
+      const T *row = reinterpret_cast<const T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), of));
+      const float f = __shfl_sync(0xffffffffu, p, of);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (lane + 32 * i < D) o[i] = fmaf(f, to_f32(row[(lane + 32 * i) * v_d]), o[i]);
+    }
+    bool lost = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lost = lost && (lane + 32 * i >= D || o[i] != o[i]);
+    if (__all_sync(0xffffffffu, lost)) l = NAN;
+    if (l != l) break;
+  }
+}
+
 }  // namespace fml

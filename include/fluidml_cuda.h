@@ -554,7 +554,8 @@ int fml_rotary_frequencies(const fml_rotary_spec *spec, float *frequencies, floa
 
 /* How scores become weights: s = q . k / divisor;  with cap > 0  s = cap * tanh(s / cap);  with slopes  s -= slope[head] *
  * |query position - key position|;  softmax over the visible keys.  A query that sees no key gives zeros.  Keys that a query
- * does not see add nothing to it, whatever they hold. */
+ * does not see add nothing to it, whatever they hold (a row that they, or its own, make infinite or NaN is computed again by
+ * itself, some hundred times slower). */
 typedef struct fml_score_rules {
   float divisor, cap; /* cap 0: none */
   int32_t causal;     /* fml_attention_rules only */

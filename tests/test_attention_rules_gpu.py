@@ -130,6 +130,27 @@ def test_large_numbers_that_are_not_seen_cost_no_bits(dtype, d, large):
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [64, 80, 128])
+def test_what_is_not_finite_stays_in_its_feature(dtype, d):
+    t, s, h = TYPES[dtype], 700, 12
+    q, k, v = randn(43, 1, h, s, d, dtype=t), randn(44, 1, h // 3, s, d, dtype=t), randn(45, 1, h // 3, s, d, dtype=t)
+    v[:, :, 33, 5] = math.inf
+    out = torch.empty(1, h, s, d, dtype=t).cuda()
+    slopes = torch.tensor([2.0 ** -(8 + i / 4) for i in range(h)])
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, math.sqrt(d), causal=True, slopes=slopes.cuda(), cap=30.0)
+    other = torch.arange(d) != 5
+    for j in (0, 7):
+        bias = -slopes[j].double() * (torch.arange(s)[:, None] - torch.arange(s)[None, :]).abs().double()
+        want, size = attention(q[0, j], k[0, j // 3][:], v[0, j // 3][:, other], visible_of(s, s, True, None, None, None), math.sqrt(d), 30.0, bias)
+        assert close(out[0, j][:, other], want, size, t)
+        assert (out[0, j, 33:, 5] == math.inf).all() and out[0, j, :33, 5].isfinite().all()
+    for x in (q, k, v):
+        y = [math.nan * z if z is x else z for z in (q, k, v)]
+        cabi.attention_rules(*(z.cuda() for z in y), out, math.sqrt(d), causal=True)
+        assert out.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
 def test_strides_and_alignment(dtype):
     t = TYPES[dtype]
     b, s, d = 2, 70, 64
