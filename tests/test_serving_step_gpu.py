@@ -211,3 +211,50 @@ def test_tensors_the_calls_refuse():
     with pytest.raises(TypeError):
         cabi.rotary_positions(x, None, None, torch.arange(2).cuda(), None, torch.ones(8).cuda(), x.clone(), None, None, magnitude="1")
     cabi.check_device()
+
+
+def spread(x, step=(1 << 31) + 64):
+    """A copy of x whose first dim moves by more than 2^31 elements."""
+    view = torch.empty((x.shape[0] - 1) * step + x[0].numel(), dtype=x.dtype, device="cuda").as_strided(x.shape, (step,) + x[0].contiguous().stride())
+    return view.copy_(x)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_offsets_that_pass_32_bits(dtype):
+    """The same bits as from tensors that lie together, which the other tests hold to 64 bits."""
+    t = TYPES[dtype]
+    rand = lambda seed, *s: torch.randn(s, generator=torch.Generator().manual_seed(seed)).to(t).cuda()  # noqa: E731
+    # positions and append: far tokens, far pages
+    q, k, v = rand(1, 2, 4, 64), rand(2, 2, 2, 64), rand(3, 2, 2, 64)
+    at, slots, f = torch.tensor([5, 9]).cuda(), torch.tensor([7, 1]).cuda(), torch.logspace(0, -3, 32).cuda()
+    kc, vc = rand(4, 2, 4, 2, 64), rand(5, 2, 4, 2, 64)
+    far_k, far_v, far_out, out = spread(kc), spread(vc), spread(q), torch.empty_like(q)
+    cabi.rotary_positions(q, k, v, at, slots, f, out, kc, vc)
+    cabi.rotary_positions(spread(q), k, v, at, slots, f, far_out, far_k, far_v)
+    assert torch.equal(out, far_out) and torch.equal(kc, far_k) and torch.equal(vc, far_v)
+    # the cache read again; values as far as keys, and not
+    table, context, start = (torch.tensor(x, dtype=I32).cuda() for x in ([[1, 0]], [6], [0, 2]))
+    ws = torch.empty(cabi.attention_tree_workspace(1, 2, 4, 2, 64), dtype=torch.uint8).cuda()
+    cabi.attention_tree(q, kc, vc, table, context, start, None, out, ws, 8.0)
+    for cache in (far_v, vc):
+        far_out.zero_()
+        cabi.attention_tree(q, far_k, cache, table, context, start, None, far_out, ws, 8.0)
+        assert torch.equal(out, far_out)
+    del far_k, far_v, far_out
+    # prompts of either size of kernel, batches far apart
+    for s, d in ((40, 64), (1100, 64), (1100, 128)):
+        q, k, v = rand(6, 2, 8, s, d), rand(7, 2, 4, s, d), rand(8, 2, 4, s, d)
+        out, far_out = torch.empty_like(q), spread(torch.zeros_like(q))
+        cabi.attention_rules(q, k, v, out, math.sqrt(d), causal=True)
+        cabi.attention_rules(spread(q), k, v, far_out, math.sqrt(d), causal=True)
+        assert torch.equal(out, far_out)
+        far_out.zero_()
+        cabi.attention_rules(q, spread(k), spread(v), far_out, math.sqrt(d), causal=True)
+        assert torch.equal(out, far_out)
+    # logits
+    z, u = rand(9, 2, 5000), torch.tensor([0.3, 0.8]).cuda()
+    token, far_token, p = torch.empty(2, dtype=I32).cuda(), torch.empty(2, dtype=I32).cuda(), torch.tensor([0.9, 0.9]).cuda()
+    cabi.sample(z, u, token, top_p=p)
+    cabi.sample(spread(z), u, far_token, top_p=p)
+    assert torch.equal(token, far_token)
+    cabi.check_device()
