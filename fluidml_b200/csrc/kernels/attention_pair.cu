@@ -37,6 +37,7 @@ constexpr int kHalfSplit = kSplit / 2;           // offset of lo
 constexpr uint32_t kColS = 0, kColO = 128, kColQ = 192;  // tensor memory: two score buffers (P over S), O, Q
 enum { kNoMask = 0, kKeyMask = 1, kFullMask = 2, kCausal = 3, kRules = 4 };
 constexpr int kMaxBlocks = 2048;  // of keys, with rules
+constexpr int kFold = 16;         // (rules) blocks of keys that one accumulator takes
 struct NoRules {};
 
 struct AttnPairArgs {
@@ -49,8 +50,9 @@ struct AttnPairArgs {
   int *status;
 };
 
-// With rules (fml_attention_rules; 4 x 16 heads of 512, prefix: 28 us, off by 1.2e-6 against 64 bits, four times a plain fp32
-// form's: the tensor cores cut what they add to an accumulator, and the context is one over all keys): the blocks of keys that some query of the tile sees are listed first, heads share keys and
+// With rules (fml_attention_rules; 4 x 16 heads of 512, prefix: 28 us, off by 1.2e-6 against 64 bits, three times a plain fp32
+// form's: the tensor cores cut what they add to an accumulator, 2^-24 of it by every instruction and always downwards, which is
+// why every 16 blocks the context moves to the output, in fp32, and begins anew): the blocks of keys that some query of the tile sees are listed first, heads share keys and
 // values in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.
 template <int MASK, typename Rules>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -201,7 +203,7 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           for (int k = 0; k < kKeys / 16; ++k) {
             const uint32_t p_hi = p + 8u * k, p_lo = p_hi + 32u;
             const uint64_t vh = desc_v + (uint64_t)(2 * k * (kD * 16) >> 4), vl = vh + (uint64_t)(kHalfSplit >> 4);
-            umma_f16_ts(d, p_lo, vh, idesc, (j == 1 && k == 0) ? 0u : 1u);
+            umma_f16_ts(d, p_lo, vh, idesc, ((j == 1 || (MASK == kRules && (j - 1) % kFold == 0)) && k == 0) ? 0u : 1u);
             umma_f16_ts(d, p_hi, vl, idesc, 1u);
             umma_f16_ts(d, p_hi, vh, idesc, 1u);
           }
@@ -258,11 +260,36 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       rr = row_rules(rules, b, h, row_in);
       rr.slope *= 1.0f / kLog2e;  // (scores are in natural units here)
     }
+    float m_fold = 0.0f;  // (rules) the reference of the context that the output holds
     for (int j = 0; j < n_blocks && ok; ++j) {
       const uint32_t buf = (uint32_t)j & 1u;
       ok = mbar_wait_warp(bar_s + 8u * buf, (uint32_t)(j >> 1) & 1u, abort_flag);
       if (!ok) break;
       tc_fence_after();
+      if constexpr (MASK == kRules) {
+        if (j > 0 && j % kFold == 0) {  // out = out + O, and O begins anew with this block
+          ok = mbar_wait_warp(bar_pv, (uint32_t)(j - 1) & 1u, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const float keep = j > kFold ? exp2f((m_fold - m_ref) * kLog2e) : 0.0f, scale = pow2(-ev_ref);
+          m_fold = m_ref;
+          float *dst = a.out + (int64_t)b * a.o_s[0] + (int64_t)h * a.o_s[1] + (int64_t)row_in * a.o_s[2];
+#pragma unroll 1
+          for (int c = 0; c < 64; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(lane_addr + kColO + (uint32_t)c, o);
+            if (grow < a.Sq) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                float *at = dst + (int64_t)(c + i) * a.o_s[3];
+                const float x = __uint_as_float(o[i]) * scale;
+                *at = j > kFold ? fmaf(*at, keep, x) : x;
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
       const int ev = exp_s[2 * buf + 1];
       const float f = a.inv_divisor * pow2(max(-126, min(126, -(e_q + exp_s[2 * buf]))));
       const int key0 = block(j) * kKeys;
@@ -378,6 +405,11 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         __syncwarp();
         tmem_ld32(lane_addr + kColO + (uint32_t)c, o);
         if constexpr (MASK == kRules) {
+          if (n_blocks > kFold && grow < a.Sq) {
+            const float keep = exp2f((m_fold - m_ref) * kLog2e) * pow2(ev_ref);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = fmaf(dst[(int64_t)(c + i) * a.o_s[3]], keep, o[i]);
+          }
           if (n_blocks == 0) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.0f;

@@ -195,6 +195,28 @@ def test_larger_problems_with_rows_that_see_nothing_and_infinities(dtype):
     run(q, k[:, :, :900], v[:, :, :900], causal=True, heads=(3,))  # more queries than keys
 
 
+@pytest.mark.parametrize("kind", ["plain", "bias", "documents"])
+def test_sums_over_many_keys_in_fp32(kind):
+    """Values of one sign, so that a context that is cut as it grows shows.  Small queries: scores sum |q||k| / 8 of 2 at most, so
+    they are off by 12 x 2^-23 x 2 for the tensor core's instructions, 2^-20 x 2 for the split operands and 20 x 2^-23 for the bias:
+    7.2e-6, twice in a weight.  The context: at most 16 blocks of 12 instructions lose 2^-23 each of what one accumulator holds,
+    2.3e-5, and 20 sums in fp32 2^-24 each, 1.2e-6."""
+    sq, sk, d = 130, 20000, 64
+    q, k, v = randn(46, 1, 2, sq, d) * 0.1, randn(47, 1, 1, sk, d), randn(48, 1, 1, sk, d).abs() + 1
+    slopes = torch.tensor([1e-3, 5e-4]) if kind == "bias" else None  # the largest score moves along the keys
+    qd, kd = (torch.arange(sq)[None] % 3, torch.arange(sk)[None] // 300 % 2) if kind == "documents" else (None, None)  # 2: none
+    out = torch.empty(1, 2, sq, 2 * d).cuda()[..., ::2] if kind == "documents" else torch.empty(1, 2, sq, d).cuda()
+    on = lambda x: None if x is None else x.cuda()  # noqa: E731
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, 8.0, causal=True, slopes=on(slopes), q_documents=on(qd), k_documents=on(kd))
+    cabi.check_device()
+    see = visible_of(sq, sk, True, None, None if qd is None else qd[0], None if kd is None else kd[0])
+    for h in range(2):
+        distance = ((torch.arange(sq)[:, None] + sk - sq) - torch.arange(sk)[None, :]).abs().double()
+        want, size = attention(q[0, h], k[0, 0], v[0, 0], see, 8.0, 0.0, None if slopes is None else -slopes[h].double() * distance)
+        err = (out[0, h].cpu().double() - want).abs()
+        assert (err <= (2 * 7.2e-6 + 2.3e-5 + 1.2e-6 + 1e-6) * size + 1e-7).all(), float((err / size.clamp_min(1e-30)).max())
+
+
 def test_large_scores():
     """Scores of hundreds: the running maximum moves, and weights of distant keys vanish."""
     for dtype in TYPES.values():
