@@ -195,6 +195,14 @@ def test_larger_problems_with_rows_that_see_nothing_and_infinities(dtype):
     run(q, k[:, :, :900], v[:, :, :900], causal=True, heads=(3,))  # more queries than keys
 
 
+@pytest.mark.parametrize("dtype,sk", [("f32", 131000), ("f32", 131200), ("f16", 262100), ("bf16", 262200)])
+def test_long_rows_on_either_side_of_what_a_kernel_lists(dtype, sk):
+    t = TYPES[dtype]
+    q, k, v = randn(49, 1, 1, 128, 64, dtype=t), randn(50, 1, 1, sk, 64, dtype=t), randn(51, 1, 1, sk, 64, dtype=t)
+    docs = (torch.arange(sk)[None] >= sk - 40000).to(torch.int32)
+    run(q, k, v, causal=True, qd=torch.arange(128, dtype=torch.int32)[None] % 2, kd=docs)
+
+
 @pytest.mark.parametrize("kind", ["plain", "bias", "documents"])
 def test_sums_over_many_keys_in_fp32(kind):
     """Values of one sign, so that a context that is cut as it grows shows.  Small queries: scores sum |q||k| / 8 of 2 at most, so
