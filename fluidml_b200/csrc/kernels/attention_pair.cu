@@ -50,7 +50,7 @@ struct AttnPairArgs {
   int *status;
 };
 
-// With rules (fml_attention_rules; 4 x 16 heads of 512, prefix: 28 us, off by 1.2e-6 against 64 bits, three times a plain fp32
+// With rules (fml_attention_rules; 4 x 16 heads of 512, prefix: 29 us, off by 1.2e-6 against 64 bits, three times a plain fp32
 // form's: the tensor cores cut what they add to an accumulator, 2^-24 of it by every instruction and always downwards, which is
 // why every 16 blocks the context moves to the output, in fp32, and begins anew): the blocks of keys that some query of the tile sees are listed first, heads share keys and
 // values in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.
