@@ -197,13 +197,16 @@ template <typename T> struct Sampler {
     for (int i = threadIdx.x; i < kBins; i += kThreads) sh->hist[i] = 0;
     __syncthreads();
   }
-  // hist of all CTAs, added up, into every CTA's merged; the CTAs' two sums into every CTA's sums.  Each CTA adds up its share of
-  // the bins.
-  __device__ void merge(u64 s0 = 0, u64 s1 = 0) {
+  // Two sums of every CTA into every CTA's sums, to be read behind the next merge().  Once per row: nothing keeps a CTA that is
+  // ahead from writing here again while another still reads.
+  __device__ void share_sums(u64 s0, u64 s1) {
     if (threadIdx.x < ranks) {
       *cluster.map_shared_rank(&sh->sums[0][rank], threadIdx.x) = s0;
       *cluster.map_shared_rank(&sh->sums[1][rank], threadIdx.x) = s1;
     }
+  }
+  // hist of all CTAs, added up, into every CTA's merged.  Each CTA adds up its share of the bins.
+  __device__ void merge() {
     cluster.sync();
     const int share = kBins / ranks;
     for (int i = rank * share + threadIdx.x; i < (rank + 1) * share; i += kThreads) {
@@ -691,7 +694,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
         range = hi;
         all = s.block_sum(all);
         over = s.block_sum(over);
-        s.merge(all, over);
+        s.share_sums(all, over);
+        s.merge();
         all = s.sum_of(0);
         over = s.sum_of(1);
         const double want = share * (double)all;

@@ -122,6 +122,26 @@ def test_cold_and_hot_rows():
     check(z * 1e-30, u, top_p=[0.5] * 6, top_k=[0, 0, 1000, 4000, 0, 1])
 
 
+@pytest.mark.parametrize("dtype,vocab", [("f32", 4201), ("f16", 8201), ("bf16", 8201)])
+def test_cuts_in_ranges_of_many_keys(dtype, vocab):
+    """The cut's bin holds more keys than a histogram has bins, so that the CTAs of a row narrow it in several rounds: fp32 always, 16-bit
+    types around zero, where a bin has all the small numbers.  Every CTA has to see the same sums in every round, run after run."""
+    n = 4
+    z, u = (randn(21, n, vocab) * 1.5).to(TYPES[dtype]), rand(22, n)
+    w = torch.exp(z.double())
+    top_p = ((w * (z > 0)).sum(1) / w.sum(1)).float()  # the cut falls on the first number that is not above zero, or next to it
+    top_k = torch.tensor([0, vocab - 1, vocab // 2 + 2000, 0], dtype=torch.int32)
+    check(z, u, top_p=top_p)
+    check(z, u, top_p=top_p, top_k=top_k, min_p=[0.0, 1e-4] * 2)
+    z, u, top_p, top_k = z.cuda().repeat(64, 1), u.cuda().repeat(64), top_p.cuda().repeat(64), top_k.cuda().repeat(64)
+    first = None
+    for _ in range(100):
+        tokens = torch.empty(64 * n, dtype=torch.int64).cuda()
+        cabi.sample(z, u, tokens, top_p=top_p, top_k=top_k)
+        first = tokens if first is None else first
+        assert torch.equal(tokens.view(64, n), first[:n].expand(64, n))
+
+
 def test_views_and_alignment():
     base, u = randn(12, 5, 3003), rand(13, 5)
     want = torch.empty(5, dtype=torch.int64)
