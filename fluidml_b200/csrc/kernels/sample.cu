@@ -502,6 +502,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
   s.warp = threadIdx.x >> 5; s.lane = threadIdx.x & 31;
   s.base = s.rank * a.slice; s.seg = a.slice / kWarps; s.phase = 0;
   const int64_t row = blockIdx.x / s.ranks;
+  // Nobody writes to another CTA's shared memory before that CTA runs: everyone says so here and asks below, behind the loads
+  s.cluster.barrier_arrive();
   pdl_prologue();
   float temperature = a.temperature ? a.temperature[row * a.temperature_s] : 1.0f;
   float p = a.top_p ? a.top_p[row * a.top_p_s] : 1.0f;
@@ -558,6 +560,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads) sample_kernel(
     }
   }
   if (threadIdx.x < 32) shared.roots[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32));
+  __syncwarp();
+  s.cluster.barrier_wait();
   const uint32_t top_key = s.largest(top);  // (its barriers publish the slice too)
   s.top_key = top_key;
   if (temperature > 0.0f) temperature = fmaxf(temperature, 1e-30f);  // (the bins' scale stays finite)

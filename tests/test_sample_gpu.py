@@ -142,6 +142,21 @@ def test_cuts_in_ranges_of_many_keys(dtype, vocab):
         assert torch.equal(tokens.view(64, n), first[:n].expand(64, n))
 
 
+@pytest.mark.parametrize("dtype,grain", [("f32", 1024), ("bf16", 2048)])
+@pytest.mark.parametrize("ctas", [2, 4, 8])
+def test_the_largest_logit_from_the_cta_that_has_least_to_do(dtype, grain, ctas):
+    """One token more than half as many CTAs take: the last ones have next to nothing to load and are the first to tell the others what
+    they found."""
+    n, v = 1200, grain * (ctas // 2) + 1
+    z = randn(23, n, v).to(TYPES[dtype]).cuda()
+    z[:, -1] = 20.0
+    u, tokens, p = rand(24, n).cuda(), torch.empty(n, dtype=torch.int64).cuda(), torch.empty(n).cuda()
+    for _ in range(20):
+        tokens.fill_(-7)
+        cabi.sample(z, u, tokens, temperature=torch.zeros(n).cuda(), probabilities=p)
+        assert (tokens == v - 1).all() and (p == 1).all()
+
+
 def test_views_and_alignment():
     base, u = randn(12, 5, 3003), rand(13, 5)
     want = torch.empty(5, dtype=torch.int64)
