@@ -58,13 +58,17 @@ template <typename T, int V> __global__ void __launch_bounds__(kThreads) rotary_
   const int n = (int)min((int64_t)a.tokens_per_cta, a.tokens - t0);
   for (int i = threadIdx.x; i < n * a.half; i += kThreads) {
     const int t = a.by_half(i), j = i - t * a.half;
-    // position * frequency / 2 pi with what each product rounds away (1 / 2 pi as two numbers): the fraction is good to 2^-50
-    // for any position that 64 bits hold
-    const double pos = (double)index_at(a.positions, t0 + t), f = (double)a.frequencies[j * a.freq_stride];
+    // position * frequency / 2 pi with what each product rounds away (1 / 2 pi as two numbers), and beyond 2^53 the position's low
+    // bits apart, which a double does not hold: the fraction is good to 2^-40 for frequencies up to one radian and any position
+    // that 64 bits hold, to 2^-50 below 2^53.  What was rounded away may be turns again, so the sum is reduced once more.
+    const int64_t at = index_at(a.positions, t0 + t), low = at >= (1ll << 53) || at <= -(1ll << 53) ? at & 2047 : 0;
+    const double pos = (double)(at - low), f = (double)a.frequencies[j * a.freq_stride];
     const double angle = pos * f, turns = angle * 0.15915494309189535;
-    const double rest = fma(angle, 0.15915494309189535, -turns) + (angle * -9.839338337591243e-18 + fma(pos, f, -angle) * 0.15915494309189535);
+    const double rest = fma(angle, 0.15915494309189535, -turns) + (angle * -9.839338337591243e-18 + fma(pos, f, -angle) * 0.15915494309189535) +
+                        (double)low * f * 0.15915494309189535;
+    const double part = (turns - rint(turns)) + rest;
     float s, c;
-    sincospif((float)(2.0 * ((turns - rint(turns)) + rest)), &s, &c);
+    sincospif((float)(2.0 * (part - rint(part))), &s, &c);
     table[i] = make_float2(a.magnitude * c, a.magnitude * s);
   }
   if (a.slots.p && threadIdx.x < n) {

@@ -131,6 +131,14 @@ def test_far_and_negative_positions():
     hold(out, *oracle(x, p, FREQ[64], 1.0, False))
 
 
+def test_positions_beyond_what_a_double_holds():
+    p = torch.tensor([1 << 53, (1 << 53) + 1, -(1 << 53) - 1, (1 << 57) + 2047, (1 << 60) + 1, (1 << 62) + 12345, (1 << 63) - 1, -(1 << 63), 1 - (1 << 63)])
+    x = randn(14, len(p), 1, 128)
+    out = torch.empty_like(x)
+    cabi.rotary_positions(x, None, None, p.cuda(), None, FREQ[64].cuda(), out, None, None)
+    hold(out, *oracle(x, p, FREQ[64], 1.0, False))
+
+
 def test_a_stream_of_its_own_and_a_captured_graph():
     x, p, f = randn(13, 8, 2, 64), torch.arange(8).cuda(), FREQ[16].cuda()
     out = torch.zeros_like(x)
