@@ -76,7 +76,7 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, const Request &x, int j,
   const int i = key - x.context;
   return a.tree ? i < 64 && (mask_of(a, x, j) >> i & 1ull) : i <= j;
 }
-// Element offsets of a key's rows in the caches, -1 for a page that is not there.
+// The page that holds a key, -1 for one that is not there.
 __device__ __forceinline__ int64_t page_of(const TreeArgs &a, int r, int key) {
   const int64_t page = a.table[r * a.table_r + (key / a.page) * a.table_c];
   return page >= 0 && page < a.pages ? page : -1;
@@ -499,10 +499,18 @@ template <typename T> int launch(const TreeArgs &a, int warps, cudaStream_t s) {
 
 using namespace fml;
 
+namespace {
+// Bytes of the counts of requests, and of them and the partial results for tiles of 16 * warps rows.
+size_t counts_bytes(int64_t requests) { return (size_t)((requests + 1) * 8 + 15) / 16 * 16; }
+size_t workspace_bytes_for(int64_t requests, int warps, int64_t head_size) {
+  return counts_bytes(requests) + (size_t)kCtas * 2 * 16 * warps * ((head_size <= 64 ? 64 : 128) + 2) * 4;
+}
+}  // namespace
+
+// The bound of every call of up to so many requests and tokens: all tokens may be one request's, and the tile is as high as its rows.
 extern "C" size_t fml_attention_tree_workspace(int64_t requests, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_size) {
   if (requests < 0 || tokens < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || head_size < 1 || head_size > 128) return 0;
-  const int64_t rows = 16 * row_warps(requests, tokens, heads / kv_heads), dp = head_size <= 64 ? 64 : 128;
-  return (size_t)((requests + 1) * 8 + 15) / 16 * 16 + (size_t)kCtas * 2 * rows * (dp + 2) * 4;
+  return workspace_bytes_for(requests, row_warps(1, tokens, heads / kv_heads), head_size);
 }
 
 extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache, const fml_tensor *v_cache, const fml_tensor *block_table,
@@ -541,7 +549,8 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
     for (int i = 0; i < 3; ++i) ok = ok && (t->shape[i] == 1 || t->stride[i] % per16 == 0);
     FML_REQUIRE(ok, FML_MISALIGNED, "fml_attention_tree: the caches' rows must lie on 16-byte boundaries");
   }
-  const size_t need = fml_attention_tree_workspace(requests, tokens, heads, kv_heads, d);
+  const int warps = row_warps(requests, tokens, heads / kv_heads);
+  const size_t need = workspace_bytes_for(requests, warps, d);
   FML_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, FML_BAD_ARG,
               "fml_attention_tree: a 16-byte aligned workspace of %zu bytes is needed", need);
   FML_REQUIRE(on_current_device(out->data) && on_current_device(workspace), FML_BAD_ARG,
@@ -572,10 +581,9 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.group = (int)(heads / kv_heads); a.D = (int)d;
   a.cap = Cap::make(rules->divisor, rules->cap);
   a.first = static_cast<long long *>(workspace);
-  a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + ((requests + 1) * 8 + 15) / 16 * 16);
+  a.partial = reinterpret_cast<float *>(static_cast<char *>(workspace) + counts_bytes(requests));
   a.status = device_status_word();
   FML_REQUIRE(a.status, FML_CUDA_ERROR, "fml_attention_tree: no device status word");
-  const int warps = row_warps(requests, tokens, a.group);
   if (q->dtype == FML_F32) return launch<float>(a, warps, as_stream(stream));
   if (q->dtype == FML_F16) return launch<__half>(a, warps, as_stream(stream));
   return launch<__nv_bfloat16>(a, warps, as_stream(stream));

@@ -581,7 +581,8 @@ int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, const fml_tens
  * index; context + depth for a new one, depth = how many of its request's tokens it sees, less one.
  * query_start, context: int32.  Rows of out outside every request stay as they are.  Page numbers, lengths and row ranges
  * beyond what the tensors hold are left out and recorded in the device status word.
- * `workspace`: fml_attention_tree_workspace bytes at most, 16-byte aligned, for partial results of one call at a time. */
+ * `workspace`: 16-byte aligned memory for partial results of one call at a time.  fml_attention_tree_workspace bytes are enough for
+ * every call of up to so many requests and tokens; a call may need less (fewer tokens per request), and refuses what is too small. */
 size_t fml_attention_tree_workspace(int64_t requests, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t head_size);
 int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache, const fml_tensor *v_cache, const fml_tensor *block_table,
                        const fml_tensor *context, const fml_tensor *query_start, const fml_tensor *tree, const fml_tensor *slopes,

@@ -160,6 +160,27 @@ def test_tree_workspace_sizes():
     assert 0 < small < large < 32 << 20
 
 
+@pytest.mark.parametrize("heads,kv,d", [(32, 8, 128), (16, 16, 64), (8, 1, 128), (4, 4, 32)])
+def test_a_workspace_for_many_requests_is_enough_for_fewer(heads, kv, d):
+    """The need of a call follows the rows that a request has on average, so it rises as requests fall; the query does not."""
+    def taken(requests, tokens, size):
+        """Whether a call takes a workspace of `size` bytes; without a device every call ends at the outputs' check, which follows."""
+        with pytest.raises(cabi.FmlError) as e:
+            cabi.attention_tree(**tree(q=described((tokens, heads, d)), out=described((tokens, heads, d)), k_cache=described((9, 16, kv, d)),
+                                       v_cache=described((9, 16, kv, d)), block_table=described((requests, 3), cabi.I32),
+                                       context=described((requests,), cabi.I32), query_start=described((requests + 1,), cabi.I32), tree=None,
+                                       workspace=Bytes(1 << 20, size)))
+        return "workspace of" not in str(e.value)
+
+    for requests, tokens in ((64, 64), (1, 1), (3, 64), (200, 1000)):
+        size = cabi.attention_tree_workspace(requests, tokens, heads, kv, d)
+        for fewer in {1, 2, requests // 8, requests // 2, requests} - {0}:
+            for t in {1, tokens // 3, tokens} - {0}:
+                assert taken(fewer, t, size), (requests, tokens, fewer, t)
+                assert cabi.attention_tree_workspace(fewer, t, heads, kv, d) <= size
+        assert not taken(requests, tokens, 4096)
+
+
 # ------------------------------------------------------------------ sampling
 def sampling(**kw):
     a = dict(logits=described((3, 100)), uniform=described((3,)), tokens=described((3,), cabi.I64))
