@@ -174,7 +174,7 @@ def test_a_workspace_for_many_requests_is_enough_for_fewer(heads, kv, d):
 
     for requests, tokens in ((64, 64), (1, 1), (3, 64), (200, 1000)):
         size = cabi.attention_tree_workspace(requests, tokens, heads, kv, d)
-        for fewer in {1, 2, requests // 8, requests // 2, requests} - {0}:
+        for fewer in {1, min(2, requests), requests // 8, requests // 2, requests} - {0}:
             for t in {1, tokens // 3, tokens} - {0}:
                 assert taken(fewer, t, size), (requests, tokens, fewer, t)
                 assert cabi.attention_tree_workspace(fewer, t, heads, kv, d) <= size
