@@ -207,6 +207,8 @@ extern "C" int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, con
               FML_BAD_ARG, "fml_attention_rules: documents must be [batch, length] of int32 or int64");
   FML_REQUIRE(batch <= 65535 && heads <= 65535 && sq < (1 << 30) && sk < (1 << 30), FML_UNSUPPORTED, "fml_attention_rules: too large");
   if (batch == 0 || sq == 0) return FML_OK;
+  FML_REQUIRE(inputs_on_current_device({q, k, v, slopes, prefix, q_documents, k_documents}), FML_BAD_ARG,
+              "fml_attention_rules: an input is not memory of the current device");
   FML_REQUIRE(on_current_device(out->data), FML_BAD_ARG, "fml_attention_rules: the output is not memory of the current device");
   RulesArgs a;
   memset(&a, 0, sizeof(a));

@@ -553,6 +553,8 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   const size_t need = workspace_bytes_for(requests, warps, d);
   FML_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, FML_BAD_ARG,
               "fml_attention_tree: a 16-byte aligned workspace of %zu bytes is needed", need);
+  FML_REQUIRE(inputs_on_current_device({q, k_cache, v_cache, block_table, context, query_start, tree, slopes}), FML_BAD_ARG,
+              "fml_attention_tree: an input is not memory of the current device");
   FML_REQUIRE(on_current_device(out->data) && on_current_device(workspace), FML_BAD_ARG,
               "fml_attention_tree: the output or the workspace is not memory of the current device");
   TreeArgs a;

@@ -243,6 +243,8 @@ extern "C" int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, co
     fits((int64_t)(reinterpret_cast<uintptr_t>(p.in) / esize));
     fits((int64_t)(reinterpret_cast<uintptr_t>(p.out) / esize));
   }
+  FML_REQUIRE(inputs_on_current_device({q, k, v, positions, slots, frequencies}), FML_BAD_ARG,
+              "fml_rotary_positions: an input is not memory of the current device");
   for (const RotaryPart &p : a.part)
     FML_REQUIRE(!p.in || !p.out || on_current_device(p.out), FML_BAD_ARG, "fml_rotary_positions: an output is not memory of the current device");
   a.status = device_status_word();

@@ -804,6 +804,8 @@ extern "C" int fml_sample(const fml_tensor *logits, const fml_tensor *uniform, c
               "fml_sample: probabilities must be [rows] of fp32");
   FML_REQUIRE(vocab >= 1 && vocab <= (1 << 18), FML_UNSUPPORTED, "fml_sample: 1 to %d tokens", 1 << 18);
   if (rows == 0) return FML_OK;
+  FML_REQUIRE(inputs_on_current_device({logits, uniform, temperature, top_k, top_p, min_p}), FML_BAD_ARG,
+              "fml_sample: an input is not memory of the current device");
   FML_REQUIRE(on_current_device(tokens->data) && (!probabilities || on_current_device(probabilities->data)), FML_BAD_ARG,
               "fml_sample: an output is not memory of the current device");
   SampleArgs a;

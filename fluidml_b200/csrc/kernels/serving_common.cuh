@@ -4,6 +4,7 @@
 #include "common.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <initializer_list>
 
 namespace fml {
 
@@ -36,6 +37,23 @@ inline bool on_current_device(const void *p) {
     return false;
   }
   return at.type == cudaMemoryTypeManaged || at.type == cudaMemoryTypeHost || (at.type == cudaMemoryTypeDevice && at.device == dev);
+}
+
+// The same of a call's inputs (null and empty ones are not read).  With one device they can only be its own, and are not asked:
+// that is a call into the driver for each.
+inline bool inputs_on_current_device(std::initializer_list<const fml_tensor *> inputs) {
+  static const int devices = [] {
+    int n = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    return n;
+  }();
+  if (devices == 1) return true;
+  for (const fml_tensor *t : inputs)
+    if (t && numel(t) > 0 && !on_current_device(t->data)) return false;
+  return true;
 }
 
 // Integers of either width, read one by one.

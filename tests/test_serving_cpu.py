@@ -4,6 +4,7 @@ import math
 
 import numpy as np
 import pytest
+import torch
 
 from fluidml_b200 import cabi
 
@@ -197,6 +198,17 @@ def sampling(**kw):
 ])
 def test_sample_refusals(status, kw):
     refused(status, cabi.sample, **sampling(**kw))
+
+
+# ------------------------------------------------------------------ where tensors are
+@pytest.mark.skipif(torch.cuda.device_count() == 1, reason="with one device its memory is the only one there is")
+@pytest.mark.parametrize("call,args", [(cabi.rotary_positions, rotary()), (cabi.attention_rules, rules()), (cabi.attention_tree, tree()),
+                                       (cabi.sample, sampling())])
+def test_inputs_elsewhere_are_refused(call, args):
+    """The descriptions' memory is no device's: a launch on it would fault."""
+    with pytest.raises(cabi.FmlError) as e:
+        call(**args)
+    assert e.value.status == BAD_ARG and "an input is not memory of the current device" in str(e.value)
 
 
 def test_structures_are_the_headers(tmp_path):
