@@ -195,6 +195,7 @@ extern "C" int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, con
     FML_REQUIRE(out->shape[i] == q->shape[i], FML_BAD_ARG, "fml_attention_rules: shape of out");
     FML_REQUIRE(v->shape[i] == k->shape[i], FML_BAD_ARG, "fml_attention_rules: shapes of k and v differ");
   }
+  FML_REQUIRE(elements_apart(out), FML_BAD_ARG, "fml_attention_rules: out has a stride of 0");
   FML_REQUIRE(k->shape[0] == batch && k->shape[3] == d, FML_BAD_ARG, "fml_attention_rules: batch or head size of k and v");
   FML_REQUIRE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, FML_BAD_ARG, "fml_attention_rules: heads must be a multiple of the heads of k and v");
   FML_REQUIRE(d >= 4 && d <= 128 && d % 4 == 0, FML_UNSUPPORTED, "fml_attention_rules: head sizes that are multiples of 4 up to 128");

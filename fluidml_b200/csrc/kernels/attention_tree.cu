@@ -524,6 +524,7 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   const int64_t tokens = q->shape[0], heads = q->shape[1], d = q->shape[2], pages = k_cache->shape[0], page = k_cache->shape[1],
                 kv_heads = k_cache->shape[2];
   for (int i = 0; i < 3; ++i) FML_REQUIRE(out->shape[i] == q->shape[i], FML_BAD_ARG, "fml_attention_tree: shape of out");
+  FML_REQUIRE(elements_apart(out), FML_BAD_ARG, "fml_attention_tree: out has a stride of 0");
   for (int i = 0; i < 4; ++i) FML_REQUIRE(v_cache->shape[i] == k_cache->shape[i], FML_BAD_ARG, "fml_attention_tree: the caches' shapes differ");
   FML_REQUIRE(k_cache->shape[3] == d, FML_BAD_ARG, "fml_attention_tree: head size of the caches");
   FML_REQUIRE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, FML_BAD_ARG, "fml_attention_tree: heads must be a multiple of the caches' heads");

@@ -220,6 +220,7 @@ extern "C" int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, co
     const int r = paged ? 2 : 1;
     FML_REQUIRE(out[i]->shape[r] == in[i]->shape[1] && out[i]->shape[r + 1] == head && (paged || out[i]->shape[0] == tokens), FML_BAD_ARG,
                 "fml_rotary_positions: shape of %s's output", name);
+    FML_REQUIRE(elements_apart(out[i]), FML_BAD_ARG, "fml_rotary_positions: %s's output has a stride of 0", name);
     RotaryPart &p = a.part[i];
     p.in = in[i]->data; p.out = out[i]->data;
     p.heads = (int)in[i]->shape[1]; p.paged = paged;

@@ -802,6 +802,7 @@ extern "C" int fml_sample(const fml_tensor *logits, const fml_tensor *uniform, c
   FML_REQUIRE(index_tensor(tokens, 1) && per_row(tokens), FML_BAD_ARG, "fml_sample: tokens must be [rows] of int32 or int64");
   FML_REQUIRE(!probabilities || (float_tensor(probabilities, 1) && per_row(probabilities)), FML_BAD_ARG,
               "fml_sample: probabilities must be [rows] of fp32");
+  FML_REQUIRE(elements_apart(tokens) && (!probabilities || elements_apart(probabilities)), FML_BAD_ARG, "fml_sample: an output has a stride of 0");
   FML_REQUIRE(vocab >= 1 && vocab <= (1 << 18), FML_UNSUPPORTED, "fml_sample: 1 to %d tokens", 1 << 18);
   if (rows == 0) return FML_OK;
   FML_REQUIRE(inputs_on_current_device({logits, uniform, temperature, top_k, top_p, min_p}), FML_BAD_ARG,

@@ -27,6 +27,13 @@ inline bool data_tensor(const fml_tensor *t, int rank) { return t && described(t
 inline bool index_tensor(const fml_tensor *t, int rank) { return t && described(t, rank, t->dtype == FML_I64 ? 8 : t->dtype == FML_I32 ? 4 : 0); }
 inline bool float_tensor(const fml_tensor *t, int rank) { return t && described(t, rank, t->dtype == FML_F32 ? 4 : 0); }
 
+// Whether an output's elements along each dim are apart: with a stride of 0 several results would go to one place.
+inline bool elements_apart(const fml_tensor *t) {
+  for (int i = 0; i < t->rank; ++i)
+    if (t->shape[i] > 1 && t->stride[i] == 0) return false;
+  return true;
+}
+
 // Whether memory of the current device (or memory every device sees) is at `p`: a launch on another device's memory would
 // fault there.  Unregistered host memory is not.
 inline bool on_current_device(const void *p) {

@@ -520,9 +520,10 @@ int fml_pool2d(const fml_tensor *x, const fml_tensor *y, int mode, const int64_t
  *
  * Data (queries, keys, values, caches, logits, outputs) is fp32, fp16 or bf16, one type per call; indices are int32 or
  * int64.  Sums, softmax statistics and scores are fp32 or wider; a result is rounded once, to its type.  Strides are free
- * unless a function says otherwise; outputs must not overlap themselves or, but where it is said, inputs.  Tensors and
- * stream are the current device's (FML_BAD_ARG for a tensor elsewhere).  Nothing is allocated and nothing kept between
- * calls, so calls may run on several streams at once and in captured graphs; a workspace belongs to one call at a time. */
+ * unless a function says otherwise; outputs must not overlap themselves (a stride of 0 is FML_BAD_ARG) or, but where it
+ * is said, inputs.  Tensors and stream are the current device's (FML_BAD_ARG for a tensor elsewhere).  Nothing is
+ * allocated and nothing kept between calls, so calls may run on several streams at once and in captured graphs; a
+ * workspace belongs to one call at a time. */
 
 /* Rotary positions: x [tokens, heads, head size], its first 2 * n features turned by the n `frequencies` (fp32, radians per
  * position):  (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),  c, s = magnitude * cos, sin(positions[t] * frequency), the rest copied.

@@ -201,6 +201,21 @@ def test_sample_refusals(status, kw):
 
 
 # ------------------------------------------------------------------ where tensors are
+@pytest.mark.parametrize("call,args", [
+    (cabi.rotary_positions, rotary(q_out=described((5, 4, 64), strides=[64, 0, 1]))),
+    (cabi.rotary_positions, rotary(**dict(PAGED, k_out=described((3, 4, 2, 64), data=2 << 20),
+                                        v_out=described((3, 4, 2, 64), strides=[0, 128, 64, 1], data=3 << 20)))),
+    (cabi.attention_rules, rules(out=described((2, 4, 7, 64), strides=[0, 448, 64, 1]))),
+    (cabi.attention_tree, tree(out=described((6, 4, 64), strides=[256, 64, 0]))),
+    (cabi.sample, sampling(tokens=described((3,), cabi.I64, strides=[0]))),
+    (cabi.sample, sampling(probabilities=described((3,), strides=[0]))),
+])
+def test_outputs_whose_elements_share_a_place_are_refused(call, args):
+    with pytest.raises(cabi.FmlError) as e:
+        call(**args)
+    assert e.value.status == BAD_ARG and "stride of 0" in str(e.value)
+
+
 @pytest.mark.skipif(torch.cuda.device_count() == 1, reason="with one device its memory is the only one there is")
 @pytest.mark.parametrize("call,args", [(cabi.rotary_positions, rotary()), (cabi.attention_rules, rules()), (cabi.attention_tree, tree()),
                                        (cabi.sample, sampling())])
