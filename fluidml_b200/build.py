@@ -116,18 +116,24 @@ def build_host(verbose: bool = False) -> str:
 
 
 def build_serving(verbose: bool = False) -> str:
+    """The serving operators' calls from Python; "" where Python's headers are not installed: nothing else needs them, and the
+    calls say that the extension is missing."""
+    include = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(include, "Python.h")):
+        sys.stderr.write(f"{SERVING_SO} is not built: no Python.h in {include}\n")
+        return ""
     src = os.path.join(CSRC, "python", "serving.cpp")
     if _newer(SERVING_SO, [src, KERNELS_SO, *glob.glob(os.path.join(INCLUDE, "*.h"))]):
-        _run([CXX, "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], src, "-o",
+        _run([CXX, "-O2", "-std=c++17", "-fPIC", "-Wall", "-shared", "-I", INCLUDE, "-I", include, src, "-o",
               SERVING_SO, "-L", LIBDIR, "-lfluidml_b200_kernels", "-Wl,-rpath,$ORIGIN"], verbose)
     return SERVING_SO
 
 
 def build_all(verbose: bool = False) -> None:
     build_kernels(verbose)
-    build_serving(verbose)
     build_host(verbose)
     build_cli(verbose)
+    build_serving(verbose)
 
 
 if __name__ == "__main__":

@@ -1,6 +1,8 @@
 """Arguments that the serving operators refuse, and their host computations: no device needed."""
 import ctypes
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -200,6 +202,18 @@ def test_sample_refusals(status, kw):
     refused(status, cabi.sample, **sampling(**kw))
 
 
+# ------------------------------------------------------------------ the extension behind the calls
+def test_everything_else_builds_without_the_headers_of_python(monkeypatch, tmp_path):
+    import fluidml_b200.build as b
+    built = []
+    for name in ("build_kernels", "build_host", "build_cli"):
+        monkeypatch.setattr(b, name, lambda verbose=False, name=name: built.append(name))
+    monkeypatch.setattr(b, "SERVING_SO", str(tmp_path / os.path.basename(b.SERVING_SO)))
+    monkeypatch.setattr(b.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    b.build_all()
+    assert built == ["build_kernels", "build_host", "build_cli"] and not os.path.exists(b.SERVING_SO)
+
+
 # ------------------------------------------------------------------ where tensors are
 @pytest.mark.parametrize("call,args", [
     (cabi.rotary_positions, rotary(q_out=described((5, 4, 64), strides=[64, 0, 1]))),
@@ -227,8 +241,6 @@ def test_inputs_elsewhere_are_refused(call, args):
 
 
 def test_structures_are_the_headers(tmp_path):
-    import os
-    import subprocess
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     source = tmp_path / "sizes.c"
     source.write_text('#include <stdio.h>\n#include "fluidml_cuda.h"\nint main(void) { printf("%zu %zu %d %d %d %d", sizeof(fml_rotary_spec), '
