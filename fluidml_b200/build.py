@@ -1,7 +1,7 @@
 """In-tree build of the native libraries (nvcc cross-compiles sm_100a without a GPU).
 
     libfluidml_b200_kernels.so   the CUDA kernel library behind include/fluidml_cuda.h
-    _serving.so                  the Python calls of a decoder's serving step onto that library (needs Python's headers)
+    _serving.<interpreter>.so    the Python calls of a decoder's serving step onto that library (needs Python's headers)
     libfluidml_b200.so           the C++ host (parser, converter, planners, executor) behind
                                  include/worker/executor.h and include/fluidml_executor.h
 
@@ -16,6 +16,7 @@ import subprocess
 import sys
 import sysconfig
 from concurrent.futures import ThreadPoolExecutor
+from importlib.machinery import EXTENSION_SUFFIXES
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "fluidml_b200")
@@ -30,7 +31,7 @@ CXX = os.environ.get("FLUIDML_CXX", "/usr/bin/g++" if os.path.exists("/usr/bin/g
 
 KERNELS_SO = os.path.join(LIBDIR, "libfluidml_b200_kernels.so")
 HOST_SO = os.path.join(LIBDIR, "libfluidml_b200.so")
-SERVING_SO = os.path.join(LIBDIR, "_serving.so")
+SERVING_SO = os.path.join(LIBDIR, "_serving" + EXTENSION_SUFFIXES[0])  # (its name says for which interpreter)
 
 NVCC_FLAGS = ["-ccbin", CXX, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-I", INCLUDE, "-I", os.path.join(CSRC, "kernels"),

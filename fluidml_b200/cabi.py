@@ -7,6 +7,7 @@ path behind these functions.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
 import importlib.util
 import os
 import struct
@@ -464,7 +465,7 @@ def _serving():
     global _native
     if _native is None:
         lib()  # the kernel library first, so that the extension resolves against it
-        path = os.path.join(os.path.dirname(_LIB_PATH), "_serving.so")
+        path = os.path.join(os.path.dirname(_LIB_PATH), "_serving" + importlib.machinery.EXTENSION_SUFFIXES[0])
         if not os.path.exists(path):
             raise ImportError(f"{path} is missing: run `python -m fluidml_b200.build` (there is no fallback implementation)")
         spec = importlib.util.spec_from_file_location("_serving", path)

@@ -3,6 +3,7 @@ import ctypes
 import math
 import os
 import subprocess
+import sysconfig
 
 import numpy as np
 import pytest
@@ -212,6 +213,15 @@ def test_everything_else_builds_without_the_headers_of_python(monkeypatch, tmp_p
     monkeypatch.setattr(b.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
     b.build_all()
     assert built == ["build_kernels", "build_host", "build_cli"] and not os.path.exists(b.SERVING_SO)
+
+
+def test_the_extension_is_this_interpreters():
+    """Another version of Python has another layout of its objects: it must not load what was built for this one."""
+    import fluidml_b200.build as b
+    assert os.path.basename(b.SERVING_SO) == "_serving" + sysconfig.get_config_var("EXT_SUFFIX")
+    with pytest.raises(cabi.FmlError):
+        cabi.sample(**sampling(uniform=None))  # loads it
+    assert os.path.realpath(cabi._native.__file__) == os.path.realpath(b.SERVING_SO)
 
 
 # ------------------------------------------------------------------ where tensors are
