@@ -203,6 +203,7 @@ extern "C" int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, co
   a.half = (int)frequencies->shape[0];
   a.interleaved = layout == FML_ROTARY_INTERLEAVED;
   const int rot = 2 * a.half, esize = (int)data_size(first->dtype);
+  int64_t features = 0;  // of a token
   // the widest access that rotated part, rest, strides and addresses allow
   int width = 16 / esize;
   auto fits = [&](int64_t x) { while (width > 1 && x % width != 0) width >>= 1; };
@@ -217,6 +218,8 @@ extern "C" int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, co
                 FML_BAD_ARG, "fml_rotary_positions: %s and its output must be of one type and rank 3 (a paged cache: 4)", name);
     FML_REQUIRE(in[i]->shape[0] == tokens && in[i]->shape[2] == head && in[i]->shape[1] < (1 << 20), FML_BAD_ARG,
                 "fml_rotary_positions: shape of %s", name);
+    features += in[i]->shape[1] * head;
+    FML_REQUIRE(features < (1ll << 31), FML_UNSUPPORTED, "fml_rotary_positions: too many features");  // (units are counted in 32 bits)
     const int r = paged ? 2 : 1;
     FML_REQUIRE(out[i]->shape[r] == in[i]->shape[1] && out[i]->shape[r + 1] == head && (paged || out[i]->shape[0] == tokens), FML_BAD_ARG,
                 "fml_rotary_positions: shape of %s's output", name);

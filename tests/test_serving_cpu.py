@@ -61,6 +61,12 @@ def test_rotary_slots_need_keys_or_values():
     refused(BAD_ARG, cabi.rotary_positions, **rotary(k=None, v=None, k_out=None, v_out=None, slots=described((5,), cabi.I32)))
 
 
+@pytest.mark.parametrize("heads,head", [(1, 1 << 34), ((1 << 20) - 1, 1 << 15), (1 << 16, 1 << 15)])
+def test_rotary_features_beyond_32_bits(heads, head):
+    x = described((1, heads, head), cabi.F16)
+    refused(UNSUPPORTED, cabi.rotary_positions, **rotary(q=x, q_out=x, k=None, k_out=None, v=None, v_out=None, positions=described((1,), cabi.I64)))
+
+
 def test_frequencies_of_every_scaling():
     rot, base, factor, length = 64, 10000.0, 8.0, 4096.0
     i = np.arange(rot // 2)
