@@ -531,7 +531,7 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   const int esize = (int)data_size(q->dtype), per16 = 16 / esize;
   FML_REQUIRE(d >= 1 && d <= 128 && d % per16 == 0, FML_UNSUPPORTED, "fml_attention_tree: head sizes that are multiples of %d up to 128", per16);
   FML_REQUIRE(page >= 1 && page < (1ll << 31) && pages < (1ll << 31), FML_BAD_ARG, "fml_attention_tree: shape of the caches");
-  FML_REQUIRE(tokens < (1ll << 24) && heads < (1 << 16) && tokens * heads < (1ll << 31), FML_UNSUPPORTED, "fml_attention_tree: too many tokens or heads");
+  FML_REQUIRE(tokens < (1ll << 24) && heads < (1 << 16) && tokens * heads < (1ll << 31) - 256, FML_UNSUPPORTED, "fml_attention_tree: too many tokens or heads");
   FML_REQUIRE(block_table && block_table->dtype == FML_I32 && index_tensor(block_table, 2), FML_BAD_ARG,
               "fml_attention_tree: block_table must be [requests, pages of a request] of int32");
   const int64_t requests = block_table->shape[0], columns = block_table->shape[1];

@@ -164,6 +164,12 @@ def test_tree_refusals(status, kw):
     refused(status, cabi.attention_tree, **tree(**kw))
 
 
+def test_tree_rows_next_to_what_32_bits_count():
+    tokens, heads = 151 * 331, 2 * 9 * 7 * 11 * 31  # 2^31 - 2 rows of one kv head, in tiles that end behind 2^31
+    refused(UNSUPPORTED, cabi.attention_tree, **tree(q=described((tokens, heads, 8), cabi.F16), out=described((tokens, heads, 8), cabi.F16), tree=None,
+                                                     k_cache=described((9, 16, 1, 8), cabi.F16), v_cache=described((9, 16, 1, 8), cabi.F16)))
+
+
 def test_tree_workspace_sizes():
     assert cabi.attention_tree_workspace(1, 1, 8, 3, 64) == 0 and cabi.attention_tree_workspace(1, 1, 8, 8, 129) == 0
     small, large = cabi.attention_tree_workspace(4, 4, 8, 2, 64), cabi.attention_tree_workspace(4, 400, 8, 2, 128)
