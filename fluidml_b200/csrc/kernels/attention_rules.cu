@@ -190,6 +190,8 @@ extern "C" int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, con
   FML_REQUIRE(k->dtype == q->dtype && v->dtype == q->dtype && out->dtype == q->dtype, FML_BAD_ARG, "fml_attention_rules: one type per call");
   FML_REQUIRE(rules && std::isfinite(rules->divisor) && rules->divisor != 0.0f && std::isfinite(rules->cap) && rules->cap >= 0.0f, FML_BAD_ARG,
               "fml_attention_rules: divisor must be finite and not zero, cap finite and not negative");
+  FML_REQUIRE(factors_in_range(rules->divisor, rules->cap), FML_UNSUPPORTED,
+              "fml_attention_rules: caps of 2^-64 to 2^64 (0: none), divisors with 1 / divisor and 1 / (divisor cap) in fp32's range");
   const int64_t batch = q->shape[0], heads = q->shape[1], sq = q->shape[2], d = q->shape[3], kv_heads = k->shape[1], sk = k->shape[2];
   for (int i = 0; i < 4; ++i) {
     FML_REQUIRE(out->shape[i] == q->shape[i], FML_BAD_ARG, "fml_attention_rules: shape of out");

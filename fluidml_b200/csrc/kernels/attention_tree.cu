@@ -521,6 +521,8 @@ extern "C" int fml_attention_tree(const fml_tensor *q, const fml_tensor *k_cache
   FML_REQUIRE(out->dtype == q->dtype && k_cache->dtype == q->dtype && v_cache->dtype == q->dtype, FML_BAD_ARG, "fml_attention_tree: one type per call");
   FML_REQUIRE(rules && std::isfinite(rules->divisor) && rules->divisor != 0.0f && std::isfinite(rules->cap) && rules->cap >= 0.0f, FML_BAD_ARG,
               "fml_attention_tree: divisor must be finite and not zero, cap finite and not negative");
+  FML_REQUIRE(factors_in_range(rules->divisor, rules->cap), FML_UNSUPPORTED,
+              "fml_attention_tree: caps of 2^-64 to 2^64 (0: none), divisors with 1 / divisor and 1 / (divisor cap) in fp32's range");
   const int64_t tokens = q->shape[0], heads = q->shape[1], d = q->shape[2], pages = k_cache->shape[0], page = k_cache->shape[1],
                 kv_heads = k_cache->shape[2];
   for (int i = 0; i < 3; ++i) FML_REQUIRE(out->shape[i] == q->shape[i], FML_BAD_ARG, "fml_attention_tree: shape of out");

@@ -254,6 +254,13 @@ struct Cap {
     return c;
   }
 };
+// Whether the kernels' factors are normal fp32 numbers (an overflow or a flush to zero would make every score the same, or NaN).  A cap
+// within 2^64 of one leaves room for the factors that packed pairs put before it.
+inline bool factors_in_range(float divisor, float cap) {
+  auto normal = [](double x) { return x >= 1.1754943508222875e-38 && x <= 3.4028234663852886e38; };
+  const double inv = 1.0 / (divisor < 0 ? -(double)divisor : (double)divisor);
+  return normal(inv) && normal(inv * kLog2e) && (cap == 0.0f || (cap >= 0x1p-64f && cap <= 0x1p64f && normal(inv / cap)));
+}
 template <bool EXACT> __device__ __forceinline__ float tanh_of(float x) {
   if (EXACT) return tanhf(x);
   // 1 - 2 / (e^2x + 1): 1e-7 of the whole, where 16-bit weights carry 2^-9 and more

@@ -558,7 +558,7 @@ int fml_rotary_frequencies(const fml_rotary_spec *spec, float *frequencies, floa
  * does not see add nothing to it, whatever they hold (a row that they, or its own, make infinite or NaN is computed again by
  * itself, some hundred times slower). */
 typedef struct fml_score_rules {
-  float divisor, cap; /* cap 0: none */
+  float divisor, cap; /* cap 0: none, else 2^-64 to 2^64; 1 / divisor and 1 / (divisor * cap) normal fp32 numbers (FML_UNSUPPORTED) */
   int32_t causal;     /* fml_attention_rules only */
 } fml_score_rules;
 

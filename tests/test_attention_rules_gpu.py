@@ -238,6 +238,38 @@ def test_large_scores():
             assert ((out[0, h].double().cpu() - want).abs() <= (step * (dtype != torch.float32) + 16 * 3e-4) * size + step * want.abs() + 1e-7).all()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("cap,divisor", [(2.0 ** 64, 8.0), (2.0 ** -64, 8.0), (50.0, 2.0 ** 120), (30.0, -8.0)])
+def test_factors_at_their_ends(dtype, d, cap, divisor):
+    """A cap that changes nothing, one that makes all scores alike, a divisor that does."""
+    q, k, v = (randn(60 + i, 1, 2, 300, d, dtype=TYPES[dtype]) for i in range(3))
+    run(q, k, v, divisor=divisor, cap=cap, causal=True)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("bias", [False, True])
+def test_scores_beyond_the_cap(dtype, d, bias):
+    """Scores of up to some 70, a cap of 10: most lie where tanh is flat, some in its bend, over more keys than a tile has."""
+    t, n, cap = TYPES[dtype], 2100, 10.0
+    q, k, v = randn(63, 1, 4, n, d, dtype=t) * 16, randn(64, 1, 2, n, d, dtype=t), randn(65, 1, 2, n, d, dtype=t)
+    out = torch.empty(1, 4, n, d, dtype=t).cuda()
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, math.sqrt(d), cap=cap, causal=True, slopes=SLOPES.cuda() if bias else None)
+    cabi.check_device()
+    rows = torch.cat((torch.arange(0, n, 97), torch.tensor([n - 1])))
+    step = torch.finfo(t).eps / 2
+    for h in (0, 3):
+        distance = (rows[:, None] - torch.arange(n)).abs().double()
+        want, size = attention(q[0, h, rows], k[0, h // 2], v[0, h // 2], torch.arange(n) <= rows[:, None], math.sqrt(d), cap,
+                               -SLOPES[h].double() * distance if bias else None)
+        err = (out[0, h, rows].double().cpu() - want).abs()
+        # scores sixteen times as large as the bound is derived for, which the cap only brings nearer to one another; beside it the cap's
+        # own 2.4e-7 of 10, and a bias of up to 1050 in steps of 2^-24 of it, each twice (numerator and sum)
+        weight = step * (t != torch.float32) + 16 * 3e-4 + 2 * 2.4e-6 + (2 * 9 * 1050 * 1.4427 * 2.0 ** -24 if bias else 0.0)
+        assert (err <= weight * size + step * want.abs() + 1e-7).all(), float(err.max())
+
+
 def test_two_streams_and_a_captured_graph():
     t = torch.bfloat16
     x = [(randn(30 + i, 1, 8, 1000, 64, dtype=t).cuda(), randn(40 + i, 1, 8, 1000, 64, dtype=t).cuda()) for i in range(2)]

@@ -170,6 +170,13 @@ def test_tree_rows_next_to_what_32_bits_count():
                                                      k_cache=described((9, 16, 1, 8), cabi.F16), v_cache=described((9, 16, 1, 8), cabi.F16)))
 
 
+@pytest.mark.parametrize("kw", [dict(cap=1e30), dict(cap=3e38), dict(cap=1e-30), dict(divisor=1e-39), dict(divisor=-1e-40), dict(divisor=3e38),
+                                dict(divisor=1e25, cap=1e18), dict(divisor=1e-25, cap=1e-18)])
+def test_factors_beyond_fp32(kw):
+    refused(UNSUPPORTED, cabi.attention_rules, **rules(**kw))
+    refused(UNSUPPORTED, cabi.attention_tree, **tree(**kw))
+
+
 def test_tree_workspace_sizes():
     assert cabi.attention_tree_workspace(1, 1, 8, 3, 64) == 0 and cabi.attention_tree_workspace(1, 1, 8, 8, 129) == 0
     small, large = cabi.attention_tree_workspace(4, 4, 8, 2, 64), cabi.attention_tree_workspace(4, 400, 8, 2, 128)
