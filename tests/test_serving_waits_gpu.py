@@ -37,3 +37,16 @@ def test_attention_by_rules(d, length):
     call(want)
     expect_timeout_then_recover(lambda: call(out), lambda: None)
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("length", [100, 1200])
+def test_attention_by_rules_on_packed_pairs(length):
+    """fp32 of head size 64; 1200 keys are more blocks than one accumulator takes."""
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(1, 4, length, 64, generator=g).cuda() for _ in range(3))
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    prefix = torch.tensor([length // 3], dtype=torch.int32).cuda()
+    call = lambda o: cabi.attention_rules(q, k, v, o, 8.0, cap=30.0, causal=True, prefix=prefix)  # noqa: E731
+    call(want)
+    expect_timeout_then_recover(lambda: call(out), lambda: None)
+    assert torch.equal(out, want)
