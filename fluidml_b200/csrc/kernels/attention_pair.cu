@@ -37,7 +37,7 @@ constexpr int kHalfSplit = kSplit / 2;           // offset of lo
 constexpr uint32_t kColS = 0, kColO = 128, kColQ = 192;  // tensor memory: two score buffers (P over S), O, Q
 enum { kNoMask = 0, kKeyMask = 1, kFullMask = 2, kCausal = 3, kRules = 4 };
 constexpr int kMaxBlocks = 2048;  // of keys, with rules
-constexpr int kFold = 16;         // (rules) blocks of keys that one accumulator takes
+constexpr int kFold = 4;          // (rules) blocks of keys that one accumulator takes
 struct NoRules {};
 
 struct AttnPairArgs {
@@ -50,10 +50,94 @@ struct AttnPairArgs {
   int *status;
 };
 
-// With rules (fml_attention_rules; 4 x 16 heads of 512, prefix: 29 us, off by 1.2e-6 against 64 bits, three times a plain fp32
-// form's: the tensor cores cut what they add to an accumulator, 2^-24 of it by every instruction and always downwards, which is
-// why every 16 blocks the context moves to the output, in fp32, and begins anew): the blocks of keys that some query of the tile sees are listed first, heads share keys and
-// values in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.
+// Contexts that wait in the output while their accumulator takes other keys (rules): of a warp's 32 rows, row0 on, out = out * keep +
+// O * scale, and back, O = O + out * keep.  Where all 32 rows are there they wait in an order of their own, in which a warp's 16 bytes to a
+// thread are two rows from end to end: with every thread in its own row, 4 bytes at a time, a fold of all rows of 4 x 16 x 512 took 20 us.
+// Functions of their own, so that the loop over the keys keeps its registers.
+struct Folded {
+  float *at;
+  int64_t step;  // from one 16 bytes to the next of a thread's (0: by single features)
+  bool there;
+};
+__device__ __forceinline__ Folded folded_at(const AttnPairArgs &a, int b, int h, int row0) {
+  const int lane = threadIdx.x & 31;
+  Folded f;
+  f.at = a.out + (int64_t)b * a.o_s[0] + (int64_t)h * a.o_s[1] + (int64_t)row0 * a.o_s[2];
+  f.there = row0 + lane < a.Sq;
+  const bool vec = a.o_s[3] == 1 && (a.o_s[2] & 3) == 0 && (reinterpret_cast<uintptr_t>(f.at) & 15) == 0;
+  if (vec && row0 + 31 < a.Sq) {
+    f.step = 2 * a.o_s[2];
+    f.at += (lane >> 4) * a.o_s[2] + 4 * (lane & 15);
+  } else {
+    f.step = vec ? 4 : 0;
+    f.at += (f.there ? lane : 0) * a.o_s[2];
+  }
+  return f;
+}
+// All of a thread's 64 features, whose loads are in flight together.
+__device__ __forceinline__ void load_folded(const AttnPairArgs &a, const Folded &f, float (&x)[kD]) {
+  if (f.step) {
+#pragma unroll
+    for (int i = 0; i < kD / 4; ++i) {
+      const float4 y = f.there ? *reinterpret_cast<const float4 *>(f.at + i * f.step) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      x[4 * i] = y.x; x[4 * i + 1] = y.y; x[4 * i + 2] = y.z; x[4 * i + 3] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kD; ++i) x[i] = f.there ? f.at[i * a.o_s[3]] : 0.0f;
+  }
+}
+__device__ __noinline__ void fold_out(const AttnPairArgs &a, int b, int h, int row0, uint32_t col_o, bool more, float keep, float scale) {
+  const Folded f = folded_at(a, b, h, row0);
+  float x[kD];
+  if (more) {
+    load_folded(a, f, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kD; ++i) x[i] = 0.0f;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < kD; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(col_o + (uint32_t)c, o);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[c + i] = fmaf(x[c + i], keep, __uint_as_float(o[i]) * scale);
+  }
+  if (!f.there) {
+  } else if (f.step) {
+#pragma unroll
+    for (int i = 0; i < kD / 4; ++i)
+      *reinterpret_cast<float4 *>(f.at + i * f.step) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kD; ++i) f.at[i * a.o_s[3]] = x[i];
+  }
+  __syncwarp();
+}
+__device__ __noinline__ void fold_in(const AttnPairArgs &a, int b, int h, int row0, uint32_t col_o, float keep) {
+  const Folded f = folded_at(a, b, h, row0);
+  float x[kD];
+  load_folded(a, f, x);
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < kD; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(col_o + (uint32_t)c, o);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(fmaf(x[c + i], keep, __uint_as_float(o[i])));
+    tmem_st16(col_o + (uint32_t)c, o);
+  }
+  tmem_wait_st();
+  __syncwarp();  // (the warp's rows are read: now they may be written)
+}
+
+// With rules (fml_attention_rules): the blocks of keys that some query of the tile sees are listed first, heads share keys and values
+// in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.  The tensor
+// cores cut what they add to an accumulator, 2^-25 of it on average by every instruction and always downwards: every kFold blocks the context
+// moves to the output, in fp32, and begins anew.  4 x 16 heads of 512, prefix, against 64 bits (a plain fp32 form is off by 3.9e-7):
+// 16 blocks 30 us, 1.18e-6; 4 blocks 32.5 us, 9.3e-7; 2 blocks 37 us, 6.8e-7.  16 heads of 1500, every key seen (plain 7.5e-7): 16 blocks
+// 72 us, 3.3e-6; 8 blocks 75 us, 2.0e-6; 4 blocks 83 us, 1.1e-6.
 template <int MASK, typename Rules>
 __global__ void __launch_bounds__(kThreads, 2)
 attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -271,23 +355,9 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
           ok = mbar_wait_warp(bar_pv, (uint32_t)(j - 1) & 1u, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          const float keep = j > kFold ? exp2f((m_fold - m_ref) * kLog2e) : 0.0f, scale = pow2(-ev_ref);
+          const float keep = j > kFold ? exp2f((m_fold - m_ref) * kLog2e) : 0.0f;
           m_fold = m_ref;
-          float *dst = a.out + (int64_t)b * a.o_s[0] + (int64_t)h * a.o_s[1] + (int64_t)row_in * a.o_s[2];
-#pragma unroll 1
-          for (int c = 0; c < 64; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(lane_addr + kColO + (uint32_t)c, o);
-            if (grow < a.Sq) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                float *at = dst + (int64_t)(c + i) * a.o_s[3];
-                const float x = __uint_as_float(o[i]) * scale;
-                *at = j > kFold ? fmaf(*at, keep, x) : x;
-              }
-            }
-            __syncwarp();
-          }
+          fold_out(a, b, h, q0 + q * 32, lane_addr + kColO, j > kFold, keep, pow2(-ev_ref));
         }
       }
       const int ev = exp_s[2 * buf + 1];
@@ -397,6 +467,9 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
       const float inv = MASK == kRules && l == 0.0f ? 0.0f : pow2(-ev_ref) / l;
       bool bad = false;
       float largest = 0.0f;
+      if constexpr (MASK == kRules) {
+        if (n_blocks > kFold) fold_in(a, b, h, q0 + q * 32, lane_addr + kColO, exp2f((m_fold - m_ref) * kLog2e) * pow2(ev_ref));
+      }
       float *dst = a.out + (int64_t)b * a.o_s[0] + (int64_t)h * a.o_s[1] + (int64_t)row_in * a.o_s[2];
       const bool vec = a.o_s[3] == 1 && (a.o_s[2] & 3) == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
 #pragma unroll
@@ -405,11 +478,6 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         __syncwarp();
         tmem_ld32(lane_addr + kColO + (uint32_t)c, o);
         if constexpr (MASK == kRules) {
-          if (n_blocks > kFold && grow < a.Sq) {
-            const float keep = exp2f((m_fold - m_ref) * kLog2e) * pow2(ev_ref);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = fmaf(dst[(int64_t)(c + i) * a.o_s[3]], keep, o[i]);
-          }
           if (n_blocks == 0) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = 0.0f;

@@ -225,6 +225,25 @@ def test_sums_over_many_keys_in_fp32(kind):
         assert (err <= (2 * 7.2e-6 + 2.3e-5 + 1.2e-6 + 1e-6) * size + 1e-7).all(), float((err / size.clamp_min(1e-30)).max())
 
 
+@pytest.mark.parametrize("rows,stride", [(160, 64), (131, 64), (100, 66)])
+def test_few_keys_go_to_one_accumulator(rows, stride):
+    """fp32 of head size 64: scores of zero, so weights of one, and values of 21 bits, which pairs hold: nothing is rounded but sums.  The
+    tensor cores cut 2^-25 of the sum so far on average, which is on average half of what it becomes, in each of the eight
+    instructions of a block that add anything (the weights' low halves are zero): 4.8e-7 for the four blocks of an accumulator, however
+    many follow.  2048 keys are 32 blocks.  Rows that end inside a warp's, and an output whose rows are not on 16 bytes."""
+    n = 2048
+    q, k = torch.zeros(1, 2, rows, 64), randn(70, 1, 1, n, 64)
+    v = 1.0 + torch.randint(0, 1 << 20, (1, 1, n, 64), generator=torch.Generator().manual_seed(71)) / 2.0 ** 20
+    out = torch.full((1, 2, rows, stride), 7.0).cuda()
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out[..., :64], 8.0)
+    cabi.check_device()
+    want = v.double().mean(2, keepdim=True)
+    error = (out[..., :64].double().cpu() - want) / want
+    assert error.abs().max() <= 32 * 2.0 ** -23 + 10 * 2.0 ** -24  # if every instruction cut a whole unit; the roundings of eight folds
+    assert abs(float(error.mean())) <= 32 * 2.0 ** -26 + 2.0 ** -24, float(error.mean())
+    assert (out[..., 64:] == 7).all()
+
+
 def test_large_scores():
     """Scores of hundreds: the running maximum moves, and weights of distant keys vanish."""
     for dtype in TYPES.values():
