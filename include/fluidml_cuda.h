@@ -526,7 +526,8 @@ int fml_pool2d(const fml_tensor *x, const fml_tensor *y, int mode, const int64_t
  * workspace belongs to one call at a time. */
 
 /* Rotary positions: x [tokens, heads, head size], its first 2 * n features turned by the n `frequencies` (fp32, radians per
- * position):  (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),  c, s = magnitude * cos, sin(positions[t] * frequency), the rest copied.
+ * position, at most 2048 of them):  (x1, x2) -> (x1 c - x2 s, x2 c + x1 s),  c, s = magnitude * cos, sin(positions[t] *
+ * frequency), the rest copied.  A position is any integer of its type.
  * Pair i is features (i, i + n) or (2 i, 2 i + 1).  The angle is formed and reduced in 64 bits.  q and k are turned, v is
  * copied; each may be NULL together with its output.  Without `slots` an output has its input's shape and may be the input
  * itself (same strides).  With `slots` k_out and v_out are paged caches [pages, page size, kv heads, head size]: token t
@@ -575,11 +576,11 @@ int fml_attention_rules(const fml_tensor *q, const fml_tensor *k, const fml_tens
 
 /* Attention of new tokens over a paged cache: request r has context[r] cached tokens and the new ("drafted") tokens
  * query_start[r] .. query_start[r + 1] - 1 of q [tokens, heads, D], whose keys and values follow the context in the cache.
- * k_cache, v_cache [pages, page size, kv heads, D], unit stride along D and rows on 16-byte boundaries (FML_MISALIGNED
- * otherwise); block_table [requests, pages of a request] int32.  A new token sees the whole context and, with
- * tree [tokens] int64, the new tokens j < 64 of its request whose bit j is set (its own included, if it is to see itself);
- * without, those up to itself: the ordinary decoding step, for any number of tokens.  Positions for slopes: a cached token's
- * index; context + depth for a new one, depth = how many of its request's tokens it sees, less one.
+ * k_cache, v_cache [pages, page size, kv heads, D], D up to 128 and a multiple of 16 bytes (FML_UNSUPPORTED), unit stride along
+ * D and rows on 16-byte boundaries (FML_MISALIGNED); block_table [requests, pages of a request] int32.  A new token sees the
+ * whole context and, with tree [tokens] int64, the new tokens j < 64 of its request whose bit j is set (its own included,
+ * if it is to see itself); without, those up to itself: the ordinary decoding step, for any number of tokens.  Positions
+ * for slopes: a cached token's index; context + depth for a new one, depth = how many of its request's tokens it sees, less one.
  * query_start, context: int32.  Rows of out outside every request stay as they are.  Page numbers, lengths and row ranges
  * beyond what the tensors hold are left out and recorded in the device status word.
  * `workspace`: 16-byte aligned memory for partial results of one call at a time.  fml_attention_tree_workspace bytes are enough for
