@@ -38,6 +38,9 @@ constexpr uint32_t kColS = 0, kColO = 128, kColQ = 192;  // tensor memory: two s
 enum { kNoMask = 0, kKeyMask = 1, kFullMask = 2, kCausal = 3, kRules = 4 };
 constexpr int kMaxBlocks = 2048;  // of keys, with rules
 constexpr int kFold = 4;          // (rules) blocks of keys that one accumulator takes
+// (rules) P and the sums are 2^8 times as large, up to 2^15: a weight is held to 2^-33 of the row's largest where it would be to 2^-25, half
+// a step of the smallest half-precision numbers.  That counts where small weights meet values far above the others'.
+constexpr int kLift = 8;
 struct NoRules {};
 
 struct AttnPairArgs {
@@ -136,12 +139,13 @@ __device__ __noinline__ void fold_in(const AttnPairArgs &a, int b, int h, int ro
 // in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.  The tensor
 // cores cut what they add to an accumulator, 2^-25 of it on average by every instruction and always downwards: every kFold blocks the context
 // moves to the output, in fp32, and begins anew.  4 x 16 heads of 512, prefix, against 64 bits (a plain fp32 form is off by 3.9e-7):
-// 16 blocks 30 us, 1.18e-6; 4 blocks 32.5 us, 9.3e-7; 2 blocks 37 us, 6.8e-7.  16 heads of 1500, every key seen (plain 7.5e-7): 16 blocks
+// 16 blocks 30 us, 1.18e-6; 4 blocks 32.3 us, 9.3e-7; 2 blocks 37 us, 6.8e-7.  16 heads of 1500, every key seen (plain 7.5e-7): 16 blocks
 // 72 us, 3.3e-6; 8 blocks 75 us, 2.0e-6; 4 blocks 83 us, 1.1e-6.
 template <int MASK, typename Rules>
 __global__ void __launch_bounds__(kThreads, 2)
 attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                      const __grid_constant__ CUtensorMap map_v, const AttnPairArgs a, const __grid_constant__ Rules rules) {
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttnPairArgs a,
+                      const __grid_constant__ Rules rules) {
   extern __shared__ __align__(1024) uint8_t smem[];
   // [ raw stage 0 | raw stage 1 | split K | split V | mask | barriers ]
   const uint32_t raw0 = smem_u32(smem), split_k = raw0 + 2 * kRawStage, split_v = split_k + kSplit;
@@ -440,7 +444,7 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         tmem_wait_st();
       }
       const int xi = max(ev_ref - ev, -60);
-      const float x = (float)xi;
+      const float x = (float)(xi + (MASK == kRules ? kLift : 0));
       float sum = 0.0f;
       uint32_t hi[32], lo[32];
 #pragma unroll

@@ -9,7 +9,7 @@
 // Keys and values come through shared memory by 16-byte asynchronous copies (rows of a page are contiguous, pages are not).  One
 // bulk copy per row instead, which a warp issues lane by lane, took 289 us for 232 on 64 requests of one token.
 //
-// Measured (bf16, head size 128): 64 requests of one token over up to 8192, 32 kv heads 802 us, 5.1 TB/s; 8 kv heads 222 us, 4.6;
+// Measured (bf16, head size 128): 64 requests of one token over up to 8192, 32 kv heads 805 us, 5.0 TB/s; 8 kv heads 215 us, 4.7;
 // 48 requests of up to 16 drafts, 32 heads on 8, capped 380 us, 2.2 TB/s: there the instructions of softmax and cap, and one
 // barrier per tile for two CTAs of eight warps, bound it; one token over 1000 14 us, most of it the two launches' dependent loads.
 #include "flash_mma.cuh"

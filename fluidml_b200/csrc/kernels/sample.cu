@@ -14,7 +14,7 @@
 //   5  min-p, as a key; the draw: sums of the kept weights per warp, in the vocabulary's order (those above 4's bins are known),
 //      then the warp that holds the token walks its part
 //
-// Measured: 256 rows of 131072 bf16 logits, half of them with top-k, the others with top-p and min-p 225 us (a row of the former 60
+// Measured: 256 rows of 131072 bf16 logits, half of them with top-k, the others with top-p and min-p 227 us (a row of the former 60
 // instructions per 32 logits, of the latter 170: weights in 64 bits of every logit, for the sum that top-p is a share of); one row
 // of 50304 16 us, some ten cluster barriers and two small sorts.
 //

@@ -244,6 +244,27 @@ def test_few_keys_go_to_one_accumulator(rows, stride):
     assert (out[..., 64:] == 7).all()
 
 
+@pytest.mark.parametrize("kind", ["rising", "falling", "late documents"])
+def test_contexts_that_wait_while_scales_and_maxima_move(kind):
+    """fp32 of head size 64 over 21 blocks of keys: values whose scale changes by up to 2^40 from block to block, maxima that rise or fall
+    by a few units a block, and rows whose first key comes after several accumulators."""
+    n, h = 1340, 2
+    q, k, v = randn(73, 1, h, n, 64), randn(74, 1, h, n, 64), randn(75, 1, h, n, 64)
+    block = torch.arange(n) // 64
+    exponents = torch.randint(-20, 21, (22,), generator=torch.Generator().manual_seed(76))
+    v = v * (2.0 ** exponents[block].float())[:, None]
+    q[..., 0], k[..., 0] = 8.0, (block if kind == "rising" else -block).float() * 3.0  # scores move by three a block
+    documents = None
+    if kind == "late documents":
+        k[..., 0] = 0.0
+        documents = torch.zeros(1, n, dtype=torch.int32)
+        documents[:, 1000:] = torch.arange(n - 1000) % 3 + 1  # queries from 1000 on see nothing before
+        documents[:, 40:44] = torch.tensor([1, 2, 3, 9])  # but for one key each
+        documents[:, 1100] = 7  # and one sees itself alone
+    run(q, k, v, causal=True, qd=documents, kd=documents)
+    run(q[:, :, :70], k, v, qd=None if documents is None else documents[:, :70], kd=documents)
+
+
 def test_large_scores():
     """Scores of hundreds: the running maximum moves, and weights of distant keys vanish."""
     for dtype in TYPES.values():
