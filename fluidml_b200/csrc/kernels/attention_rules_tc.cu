@@ -577,7 +577,7 @@ attention_rules_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
               tmem_st16(col_o + (uint32_t)c, o);
             }
           }
-          const float2 base = both(m == -INFINITY ? 0.0f : -m), s2 = both(scale);
+          const float2 base = both((m == -INFINITY ? 0.0f : -m) + kLiftOf<T>), s2 = both(scale);
           float2 sum[2] = {both(0.0f), both(0.0f)};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {

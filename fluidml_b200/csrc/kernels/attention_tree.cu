@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(Shape<T, DP, WR>::kThreads, 2) attention_tree_
       const float v = l == 0.0f ? 0.0f : o / l;  // (no key seen: zeros)
       if (!(fabsf(v) <= 3.402823466e38f)) redo[row] = 1;
       if (d < a.D) put(row, d, v);
-      if (d == 0 && !whole) { part[row * (DP + 2) + DP] = m; part[row * (DP + 2) + DP + 1] = l; }
+      if (d == 0 && !whole) { part[row * (DP + 2) + DP] = m; part[row * (DP + 2) + DP + 1] = l * F::kUnlift; }
     }
     __syncthreads();
     for (int row = warp; row < n_rows; row += S::kWarps) {

@@ -45,6 +45,11 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo) 
   const float rest = x - __uint_as_float(hi);
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
 }
+// fp16 weights, and the sums with them, are 2^7 times as large: up to 2^15 (they reach 2^8, since the reference follows the maximum by
+// steps of more than 8), so that a small one is held to 2^-32 of the largest where it would be to 2^-25, half a step of the smallest
+// numbers.  That counts where small weights meet values far above the others'.  (bf16 has fp32's range.)
+template <typename T> constexpr float kLiftOf = 0.0f;
+template <> constexpr float kLiftOf<__half> = 7.0f;
 template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
@@ -61,6 +66,7 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, fl
 // warps.
 template <typename T, int DP, bool HELD> struct Flash {
   static constexpr int kChunk = 8, kChunks = DP / 8, kPitch = DP * 2 + 16, kPitchV = kPitch;
+  static constexpr float kLift = kLiftOf<T>, kUnlift = kLift > 0.0f ? 1.0f / 128.0f : 1.0f;  // 2^-kLift
   struct Q { uint32_t r[HELD ? DP / 16 : 1][4]; };
   // rows are 16 bytes longer than their features: a matrix load of 8 rows meets 8 different bank groups
   __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + (chunk << 4)); }
@@ -117,6 +123,7 @@ template <typename T, int DP, bool HELD> struct Flash {
 template <int DP, bool HELD> struct Flash<float, DP, HELD> {
   // rows are padded so that the loads below meet every bank once: K by pairs of features, V by single ones
   static constexpr int kChunk = 4, kChunks = DP / 4, kPitch = (DP + 8) * 4, kPitchV = (DP + 4) * 4;
+  static constexpr float kLift = kLiftOf<float>, kUnlift = 1.0f;
   struct Q {};  // (hi and lo of 16 x DP queries would fill the registers: read again for every tile)
   __device__ __forceinline__ static uint32_t at(int row, int chunk) { return (uint32_t)(row * kPitch + (chunk << 4)); }
   __device__ __forceinline__ static uint32_t at_v(int row, int chunk) { return (uint32_t)(row * kPitchV + (chunk << 4)); }
@@ -198,7 +205,7 @@ template <int DP, bool HELD> struct Flash<float, DP, HELD> {
 
 // The two rows of a thread: lane / 4 and lane / 4 + 8 of the warp's 16.
 template <int DP> struct Running {
-  float o[DP / 8][4], m[2], l[2];  // m (what p refers to), and the scores, in units of ln 2; -infinity before the first visible key
+  float o[DP / 8][4], m[2], l[2];  // o and l times 2^kLift; m (what p refers to), and the scores, in units of ln 2; -infinity before the first visible key
   __device__ __forceinline__ void reset() {
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n)
@@ -230,7 +237,7 @@ __device__ __forceinline__ void flash_step(Running<DP> &r, const typename F::Q &
       keep = ex2_approx(r.m[h] - m);
       r.m[h] = m;
     }
-    const float base = r.m[h] == -INFINITY ? 0.0f : r.m[h];  // (no key so far: every p below is 2^-infinity)
+    const float base = (r.m[h] == -INFINITY ? 0.0f : r.m[h]) - F::kLift;  // (no key so far: every p below is 2^-infinity)
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {

@@ -265,6 +265,30 @@ def test_contexts_that_wait_while_scales_and_maxima_move(kind):
     run(q[:, :, :70], k, v, qd=None if documents is None else documents[:, :70], kd=documents)
 
 
+@pytest.mark.parametrize("dtype,d", [("f32", 80), ("f16", 64), ("f16", 96), ("f16", 128), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("rows", [70, 1340])
+def test_small_weights_beside_far_larger_values(dtype, d, rows):
+    """Weights fall by e^-2 and more from block to block, values change by up to 2^24 (2^40 where the type holds that): what a small weight
+    has lost would show.  Products of a score's sum reach 84, four times what the bound is derived for."""
+    t, n, h = TYPES[dtype], 1340, 2
+    q, k, v = randn(77, 1, h, rows, d), randn(78, 1, h, n, d), randn(79, 1, h, n, d)
+    block = torch.arange(n) // 64
+    reach = 12 if dtype == "f16" else 20
+    exponents = torch.randint(-reach, reach + 1, (22,), generator=torch.Generator().manual_seed(80))
+    q[..., 0], k[..., 0] = 8.0, -block.float() * 3.0
+    q, k, v = q.to(t), k.to(t), (v * (2.0 ** exponents[block].float())[:, None]).to(t)
+    out = torch.empty(1, h, rows, d, dtype=t).cuda()
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, math.sqrt(d), causal=True)
+    cabi.check_device()
+    step = torch.finfo(t).eps / 2
+    see = visible_of(rows, n, True, None, None, None)
+    for j in range(h):
+        want, size = attention(q[0, j], k[0, j], v[0, j], see, math.sqrt(d))
+        err = (out[0, j].double().cpu() - want).abs()
+        weight = 4 * 3e-4 if t == torch.float32 else step + 4e-4
+        assert (err <= weight * size + step * want.abs() + 1e-7).all(), float((err / size).max())
+
+
 def test_large_scores():
     """Scores of hundreds: the running maximum moves, and weights of distant keys vanish."""
     for dtype in TYPES.values():

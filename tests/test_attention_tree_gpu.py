@@ -121,6 +121,34 @@ def test_chains_longer_than_64():
     tree.check(tree.call())
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("contexts,drafts,heads,kv", [([1340], [1], 4, 1), ([1340, 200, 700], [5, 1, 9], 4, 2), ([1340, 1300], [40, 30], 4, 1)])
+def test_small_weights_beside_far_larger_values(dtype, contexts, drafts, heads, kv):
+    """Weights fall by e^-2 from page to page, values change by up to 2^24 (2^40 where the type holds that); parts of a request's keys are
+    joined.  Products of a score's sum reach 84, four times what the bound is derived for."""
+    t, d, page = TYPES[dtype], 128, 64
+    c = Case(contexts, drafts, heads, kv, d, page, torch.float32, False, seed=50)
+    reach = 12 if dtype == "f16" else 20
+    exponents = torch.randint(-reach, reach + 1, (24,), generator=torch.Generator().manual_seed(51)).float()
+    c.q[..., 0] = 8.0
+    for r in range(len(contexts)):
+        for b in range(-(-(contexts[r] + drafts[r]) // page)):
+            c.k[c.table[r, b], ..., 0] = -3.0 * b
+            c.v[c.table[r, b]] *= 2.0 ** exponents[b]
+    c.q, c.k, c.v = c.q.to(t), c.k.to(t), c.v.to(t)
+    got = c.call().double().cpu()
+    cabi.check_device()
+    step = torch.finfo(t).eps / 2
+    for r in range(len(contexts)):
+        for h in range(heads):
+            q, k, v, see, _ = c.rows(r, h)
+            want, size = attention(q, k, v, see, math.sqrt(d))
+            a = int(c.start[r])
+            err = (got[a:a + len(want), h] - want).abs()
+            weight = 4 * 3e-4 if t == torch.float32 else step + 4e-4
+            assert (err <= weight * size + step * want.abs() + 1e-7).all(), (r, h, float((err / size).max()))
+
+
 def test_tokens_that_see_nothing():
     for dtype in TYPES.values():
         c = Case([0, 0, 9], [3, 2, 2], 2, 2, 64, 16, dtype, True, seed=15)
