@@ -532,7 +532,8 @@ int fml_pool2d(const fml_tensor *x, const fml_tensor *y, int mode, const int64_t
  * copied; each may be NULL together with its output.  Without `slots` an output has its input's shape and may be the input
  * itself (same strides).  With `slots` k_out and v_out are paged caches [pages, page size, kv heads, head size]: token t
  * goes to position slots[t] % page size of page slots[t] / page size; a negative slot (padding) is skipped, one beyond the
- * cache is skipped and recorded in the device status word; which of several tokens with one slot stays is not defined. */
+ * cache is skipped and recorded in the device status word; of several tokens with one slot, which one's each feature is is not
+ * defined. */
 typedef enum fml_rotary_layout { FML_ROTARY_HALVES = 0, FML_ROTARY_INTERLEAVED = 1 } fml_rotary_layout;
 int fml_rotary_positions(const fml_tensor *q, const fml_tensor *k, const fml_tensor *v, const fml_tensor *positions,
                          const fml_tensor *slots, const fml_tensor *frequencies, float magnitude, int layout,
