@@ -139,7 +139,7 @@ __device__ __noinline__ void fold_in(const AttnPairArgs &a, int b, int h, int ro
 // in groups, scores are capped, biased and masked as attention_rules.cuh says, and rows that see nothing are zero.  The tensor
 // cores cut what they add to an accumulator, 2^-25 of it on average by every instruction and always downwards: every kFold blocks the context
 // moves to the output, in fp32, and begins anew.  4 x 16 heads of 512, prefix, against 64 bits (a plain fp32 form is off by 3.9e-7):
-// 16 blocks 30 us, 1.18e-6; 4 blocks 32.3 us, 9.3e-7; 2 blocks 37 us, 6.8e-7.  16 heads of 1500, every key seen (plain 7.5e-7): 16 blocks
+// 16 blocks 30 us, 1.18e-6; 4 blocks 32 us, 9.3e-7 (with the small products of scores first 8.5e-7); 2 blocks 37 us, 6.8e-7.  16 heads of 1500, every key seen (plain 7.5e-7): 16 blocks
 // 72 us, 3.3e-6; 8 blocks 75 us, 2.0e-6; 4 blocks 83 us, 1.1e-6.
 template <int MASK, typename Rules>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -273,7 +273,12 @@ attention_pair_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const uint64_t kh = desc_k + (uint64_t)(2 * k * (kKeys * 16) >> 4), kl = kh + (uint64_t)(kHalfSplit >> 4);
             umma_f16_ts(d, q_lo, kh, idesc, k ? 1u : 0u);
             umma_f16_ts(d, q_hi, kl, idesc, 1u);
-            umma_f16_ts(d, q_hi, kh, idesc, 1u);
+            if (MASK != kRules) umma_f16_ts(d, q_hi, kh, idesc, 1u);
+          }
+          if (MASK == kRules) {  // (the small products first, while little of the sum is cut)
+#pragma unroll
+            for (int k = 0; k < kD / 16; ++k)
+              umma_f16_ts(d, tmem_base + kColQ + 8u * k, desc_k + (uint64_t)(2 * k * (kKeys * 16) >> 4), idesc, 1u);
           }
           umma_commit(bar_s + 8u * ((uint32_t)j & 1u));
           umma_commit(bar_k_free);

@@ -4,7 +4,7 @@
 // layout: a CTA has 64 queries of a head, 16 to a warp, and keys pass in tiles through two stages of shared memory.  Large
 // 16-bit problems run on the fifth-generation tensor cores (attention_rules_tc.cu).
 //
-// Measured, fp32: 4 x 16 heads of 512 x 64 115 us, where fp32 of head size 64 on packed pairs (attention_pair.cu) takes 32; what
+// Measured, fp32: 4 x 16 heads of 512 x 64 119 us, where fp32 of head size 64 on packed pairs (attention_pair.cu) takes 32; what
 // bounds it is the split of every operand of every product into two TF32 numbers by each warp for itself.
 //
 // A tile of keys that no query of the CTA sees is not loaded: causal and prefix leave the tiles up to a last one, documents are

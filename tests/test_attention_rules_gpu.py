@@ -289,6 +289,20 @@ def test_small_weights_beside_far_larger_values(dtype, d, rows):
         assert (err <= weight * size + step * want.abs() + 1e-7).all(), float((err / size).max())
 
 
+@pytest.mark.parametrize("length,d", [(700, 128), (300, 96), (10, 128)])
+def test_how_far_fp32_is_off(length, d):
+    """fp32 scores lose little of what the tensor cores cut.  N(0, 1) throughout, so q . k is some 11.3 and a partial sum of 32 features
+    5.7: its four instructions cut 2^-25 of half of that each, 6e-8 of a score of one with four partial sums of either sign; five
+    rounded steps 1.5e-7, the splits to 2^-22 of either operand 1.7e-7; in the context twelve instructions of 2^-25 of half the sum,
+    1.8e-7, and the result's rounding 4e-8.  Together 3e-7 in the 2-norm; 5e-7 leaves room for few rows."""
+    q, k, v = randn(81, 1, 4, length, d), randn(82, 1, 4, length, d), randn(83, 1, 4, length, d)
+    out = torch.empty(1, 4, length, d).cuda()
+    cabi.attention_rules(q.cuda(), k.cuda(), v.cuda(), out, math.sqrt(d), causal=True)
+    cabi.check_device()
+    want = torch.stack([attention(q[0, h], k[0, h], v[0, h], visible_of(length, length, True, None, None, None), math.sqrt(d))[0] for h in range(4)])
+    assert float((out[0].double().cpu() - want).norm() / want.norm()) <= 5e-7
+
+
 def test_large_scores():
     """Scores of hundreds: the running maximum moves, and weights of distant keys vanish."""
     for dtype in TYPES.values():

@@ -149,6 +149,25 @@ def test_small_weights_beside_far_larger_values(dtype, contexts, drafts, heads, 
             assert (err <= weight * size + step * want.abs() + 1e-7).all(), (r, h, float((err / size).max()))
 
 
+@pytest.mark.parametrize("contexts,drafts,heads,kv", [([258, 100, 31, 200, 90, 150], [1] * 6, 2, 2), ([700, 300], [20, 9], 4, 1)])
+def test_how_far_fp32_is_off(contexts, drafts, heads, kv):
+    """fp32 scores lose little of what the tensor cores cut.  N(0, 1) throughout, so q . k is some 11.3 and a partial sum of 32 features
+    5.7: its four instructions cut 2^-25 of half of that each, 6e-8 of a score of one with four partial sums of either sign; five
+    rounded steps 1.5e-7, the splits to 2^-22 of either operand 1.7e-7; in the context twelve instructions of 2^-25 of half the sum,
+    1.8e-7, and the result's rounding 4e-8.  Together 3e-7 in the 2-norm; 5e-7 leaves room for few rows."""
+    c = Case(contexts, drafts, heads, kv, 128, 16, torch.float32, False, seed=52)
+    got = c.call().double().cpu()
+    cabi.check_device()
+    err = size = 0.0
+    for r in range(len(contexts)):
+        for h in range(heads):
+            q, k, v, see, _ = c.rows(r, h)
+            want, a = attention(q, k, v, see, math.sqrt(128))[0], int(c.start[r])
+            err += float((got[a:a + len(want), h] - want).square().sum())
+            size += float(want.square().sum())
+    assert math.sqrt(err / size) <= 5e-7, math.sqrt(err / size)
+
+
 def test_tokens_that_see_nothing():
     for dtype in TYPES.values():
         c = Case([0, 0, 9], [3, 2, 2], 2, 2, 64, 16, dtype, True, seed=15)
